@@ -403,6 +403,64 @@ int ss2d_seg_loss_stats(int dtype, const void *logits, const void *labels, int l
 int ss2d_seg_loss_bwd(int dtype, const void *logits, const void *labels, int label_bytes, const float *gstats, void *dlogits,
                       int B, int C, long long HW, void *stream);
 
+/* ---- Linear attention with a decay for each head (beside the selective scan: one decay per head and token, a dk x dv state):
+ *        S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t
+ * q, k (rows, tokens, G, dk) and v (rows, tokens, H, dv) in the storage type, strided (the last axis dense); value head h uses key head
+ * h / (H / G); g (rows, tokens, H) fp32, any strides (0 broadcasts).  strides[12] (host memory): elements between batch rows, tokens and heads
+ * of q, k, v, g.  1 <= dk, dv <= 128.  States are fp32 (N, H, dk, dv).
+ * cu_seqlens null: N sequences of `tokens` tokens, rows = N.  Else N + 1 non-decreasing row offsets (device memory, clamped to [0, tokens]) of
+ * sequences packed into rows = 1 row; rows outside every sequence get zero outputs and gradients.  Sequences may be empty.
+ * A decay below -150 (exp underflows in fp32; -inf: a reset) counts as -150.
+ * Segments: a sequence is walked in nseg pieces of seg_chunks chunks (ss2d_linattn_segment_chunks for the longest sequence; the last piece takes
+ * the rest); nseg > 1 needs seg_states (N * H * nseg * dk * dv floats) and seg_decay (N * H * nseg doubles) as scratch memory.
+ * chunk_states (null: none): the forward leaves the state in front of every chunk of ss2d_linattn_chunk(dk, dv) tokens there for the backward:
+ * slots * H * dk * dv floats with slots = N * ceil(tokens / chunk), packed: tokens / chunk + N. */
+int ss2d_linattn_chunk(int dk, int dv);
+int ss2d_linattn_segment_chunks(int N, long long max_len, int H, int dk, int dv, int backward);
+int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const void *v, const float *g, const long long *strides, const int *cu_seqlens,
+                     const float *s0 /* (N, H, dk, dv) or null: 0 */, void *out /* (rows, tokens, H, dv) */, float *last /* (N, H, dk, dv) or null */,
+                     float *chunk_states, float *seg_states, double *seg_decay, int N, long long tokens, int H, int G, int dk, int dv, float scale,
+                     int nseg, int seg_chunks, void *stream);
+/* dout (rows, tokens, H, dv) and dlast (null: 0) -> dq, dk (rows, tokens, G, dk), dv (rows, tokens, H, dv), dg (rows, tokens, H) fp32, ds0 (null: not
+ * wanted).  With H > G the value heads' dq / dk go to dq_heads / dk_heads (rows, tokens, H, dk) fp32 first and are added in head order.
+ * No atomics: results do not depend on the order of execution. */
+int ss2d_linattn_bwd(int dtype, const void *q, const void *k, const void *v, const float *g, const long long *strides, const int *cu_seqlens,
+                     const void *dout, const float *dlast, const float *chunk_states, void *dq, void *dk_out, void *dv_out, float *dg, float *ds0,
+                     float *dq_heads, float *dk_heads, float *seg_states, double *seg_decay, int N, long long tokens, int H, int G, int dk, int dv,
+                     float scale, int nseg, int seg_chunks, void *stream);
+
+/* One new token for each of B requests: S <- exp(g) S + k v^T in place, out = scale * S^T q.  state: `pool` slots, slot_stride >= H * dk * dv
+ * floats apart, each (H, dk, dv) dense fp32.  q, k (B, G, dk), v (B, H, dv) with dense last axes, g (B, H); strides[8] (host memory): elements
+ * between requests and heads of q, k, v, g.  slots: B slot indices (device memory, int32, or int64 with slots64 != 0), or null: slot = request.  A
+ * request whose slot lies outside [0, pool) changes no state and gets zeros; requests that name the same slot are applied in request order. */
+int ss2d_linattn_step(int dtype, float *state, const void *q, const void *k, const void *v, const float *g, const long long *strides,
+                      const void *slots, int slots64, void *out /* (B, H, dv) */, long long pool, long long slot_stride, int B, int H, int G, int dk,
+                      int dv, float scale, void *stream);
+
+/* ---- The norms around a block with its gate and residual scale (beside ss2d_outnorm_gate and ss2d_layernorm):
+ *        u = norm(y; w1, b1) * SiLU(z),   x_out = x + drop[sample] * res_scale * u,   h = norm(x_out; w2, b2)
+ * norm over the last axis (D <= 8192): LayerNorm, or with rms != 0 RMS norm.  x, x_out in res_dtype; y, z, h in dtype; parameters fp32.  x, y, z: rows
+ * ldx / ldy / ldz elements apart.  Null: z (no gate), b1, b2, res_scale, drop (1 factor per rows_per_sample rows).  stats (rows, 4) fp32: what the
+ * backward needs, or null.
+ * Backward: dx_out, dh (dense; either may be null: 0) -> dx, dy, dz (dense) and dparams (5, D) fp32 = dw1, db1, dres_scale, dw2, db2, summed in a
+ * fixed order through the workspace. */
+int ss2d_block_norm_fwd(int res_dtype, int dtype, const void *x, const void *y, const void *z, const float *w1, const float *b1, const float *w2,
+                        const float *b2, const float *res_scale, const float *drop, long long rows_per_sample, void *x_out, void *h, float *stats,
+                        long long rows, int D, long long ldx, long long ldy, long long ldz, float eps, int rms, void *stream);
+size_t ss2d_block_norm_bwd_workspace_floats(long long rows, int D);
+int ss2d_block_norm_bwd(int res_dtype, int dtype, const void *dx_out, const void *dh, const void *x, const void *y, const void *z, const float *w1,
+                        const float *b1, const float *w2, const float *res_scale, const float *drop, long long rows_per_sample, const float *stats,
+                        void *dx, void *dy, void *dz, float *dparams, float *workspace, long long rows, int D, long long ldx, long long ldy,
+                        long long ldz, int rms, void *stream);
+
+/* ---- Gradient clipping by the global norm of n tensors: *norm = sqrt(sum g^2) (inf_norm != 0: max |g|), then, with scale != 0,
+ * g *= min(1, max_norm / (*norm + 1e-6)) in place.  ptrs (device addresses), sizes (elements) and is_bf16 (else fp32) are HOST arrays of n entries;
+ * the tensors must not share memory.  norm: device fp32 scalar; workspace: device memory.  Sums in 64 bits, in a fixed order.  A norm that
+ * is not a number makes every gradient not a number. */
+size_t ss2d_grad_clip_workspace_bytes(int n);
+int ss2d_grad_clip(const unsigned char *is_bf16, const unsigned long long *ptrs, const long long *sizes, int n, int inf_norm, float max_norm, int scale,
+                   float *norm, double *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -72,6 +72,16 @@ _SIGNATURES = {
     "ss2d_layernorm_unshuffle_bwd": (_i, [_i, _i] + [_vp] * 8 + [ctypes.c_longlong, _i, _i, _i, _i, _vp]),
     "ss2d_layernorm_merge_fwd": (_i, [_i, _i, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_longlong, _i, _i, _i, ctypes.c_float, _vp]),
     "ss2d_layernorm_merge_bwd": (_i, [_i, _i] + [_vp] * 8 + [ctypes.c_longlong, _i, _i, _i, _vp]),
+    "ss2d_linattn_chunk": (_i, [_i, _i]),
+    "ss2d_linattn_segment_chunks": (_i, [_i, ctypes.c_longlong, _i, _i, _i, _i]),
+    "ss2d_linattn_fwd": (_i, [_i] + [_vp] * 12 + [_i, ctypes.c_longlong, _i, _i, _i, _i, ctypes.c_float, _i, _i, _vp]),
+    "ss2d_linattn_bwd": (_i, [_i] + [_vp] * 18 + [_i, ctypes.c_longlong, _i, _i, _i, _i, ctypes.c_float, _i, _i, _vp]),
+    "ss2d_linattn_step": (_i, [_i] + [_vp] * 7 + [_i, _vp, ctypes.c_longlong, ctypes.c_longlong] + [_i] * 5 + [ctypes.c_float, _vp]),
+    "ss2d_block_norm_fwd": (_i, [_i, _i] + [_vp] * 9 + [ctypes.c_longlong] + [_vp] * 3 + [ctypes.c_longlong, _i] + [ctypes.c_longlong] * 3 + [ctypes.c_float, _i, _vp]),
+    "ss2d_block_norm_bwd_workspace_floats": (_sz, [ctypes.c_longlong, _i]),
+    "ss2d_block_norm_bwd": (_i, [_i, _i] + [_vp] * 10 + [ctypes.c_longlong] + [_vp] * 6 + [ctypes.c_longlong, _i] + [ctypes.c_longlong] * 3 + [_i, _vp]),
+    "ss2d_grad_clip_workspace_bytes": (_sz, [_i]),
+    "ss2d_grad_clip": (_i, [_vp, _vp, _vp, _i, _i, ctypes.c_float, _i, _vp, _vp, _sz, _vp]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

@@ -1,0 +1,222 @@
+// Clipping by the global norm of many gradients, for gfx950:  n = sqrt(sum over all tensors of sum g^2)  (or max |g|),
+// g <- g * min(1, max_norm / (n + 1e-6)).  Two passes over the gradients, no host read in between:
+//   * grad_norm_kernel: a workgroup takes a run of CHUNK-element pieces of the tensors in the launch's table (kernel arguments: up to
+//     MAXT tensors a launch, no device-side table to copy), sums squares in 64 bits and leaves one partial;
+//   * grad_scale_kernel: every workgroup adds the partials in the same fixed order, so all of them get the same factor and the norm does not
+//     depend on the order of execution, and scales its run.  A factor of 1 leaves the gradients untouched.
+// Memory-bound: read, then read and write.  The second pass runs through the pieces from the last to the first: what the
+// first pass read last is still in the last-level cache.
+// A gradient may start at any element (a piece of a flat bucket): a piece's unaligned ends are done by single elements.
+#include <algorithm>
+#include "ss2d_common.h"
+#include "../../include/ss2d.h"
+
+namespace {
+
+constexpr int NT = 256, CHUNK = 16384, MAXT = 240, MAX_WGS = 1024;
+
+struct Table {
+    unsigned long long ptr[MAXT];      // address; bit 63: bf16
+    unsigned piece[MAXT];              // index of a tensor's first piece; the last entry's end is `pieces`
+    unsigned tail[MAXT];               // elements of the last piece
+    int n;
+    unsigned pieces;
+};
+struct Range { unsigned first, count; int wgs; };
+
+__device__ __forceinline__ int find_tensor(const Table &t, unsigned piece) {
+    int lo = 0, hi = t.n - 1;
+    while (lo < hi) {
+        const int m = (lo + hi + 1) / 2;
+        if (t.piece[m] <= piece) lo = m; else hi = m - 1;
+    }
+    return lo;
+}
+
+// f(pointer, count, vector?) over the aligned middle and the unaligned ends of one piece
+template <typename T, typename Vec, typename One>
+__device__ __forceinline__ void walk_piece(T *p, unsigned n, Vec vec, One one) {
+    constexpr unsigned V = 16 / sizeof(T);
+    unsigned head = (unsigned)((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T);
+    head = head < n ? head : n;
+    const unsigned nv = (n - head) / V, done = head + nv * V;
+    T *m = p + head;
+    for (unsigned i = threadIdx.x; i < nv; i += 4 * NT) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i + u * NT < nv) vec(m + (size_t)(i + u * NT) * V);
+    }
+    if (threadIdx.x < head) one(p + threadIdx.x);
+    if (threadIdx.x < n - done) one(p + done + threadIdx.x);
+}
+
+__device__ __forceinline__ double block_sum(double v, double *red) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (red[0] + red[1]) + (red[2] + red[3]);
+    __syncthreads();
+    return v;
+}
+__device__ __forceinline__ double nan_max(double a, double b) { return (b > a || b != b) ? b : a; }
+__device__ __forceinline__ double block_max(double v, double *red) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = nan_max(v, __shfl_xor(v, d, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = nan_max(nan_max(red[0], red[1]), nan_max(red[2], red[3]));
+    __syncthreads();
+    return v;
+}
+
+template <bool INF, typename T>
+__device__ __forceinline__ double piece_norm(const T *p, unsigned n) {
+    double acc = 0.0;
+    auto add = [&](float x) {
+        if (INF) acc = nan_max(acc, (double)fabsf(x));
+        else acc = fma((double)x, (double)x, acc);
+    };
+    walk_piece<const T>(p, n,
+        [&](const T *q) {
+#pragma unroll
+            for (unsigned e = 0; e < 16 / sizeof(T); e += 4) { const f4 v = ld4(q + e); add(v.x); add(v.y); add(v.z); add(v.w); }
+        },
+        [&](const T *q) { add(ld1(q)); });
+    return acc;
+}
+
+template <bool INF>
+__global__ __launch_bounds__(NT) void grad_norm_kernel(const Table t, double *partials, unsigned per) {
+    __shared__ double red[4];
+    const unsigned a = blockIdx.x * per, e = a + per < t.pieces ? a + per : t.pieces;
+    double acc = 0.0;
+    int i = a < e ? find_tensor(t, a) : 0;
+    for (unsigned c = a; c < e; ++c) {
+        while (i + 1 < t.n && t.piece[i + 1] <= c) ++i;
+        const unsigned stop = i + 1 < t.n ? t.piece[i + 1] : t.pieces, k = c - t.piece[i];
+        const unsigned n = c + 1 == stop ? t.tail[i] : CHUNK;
+        const unsigned long long u = t.ptr[i];
+        const double v = u >> 63 ? piece_norm<INF>(reinterpret_cast<const bf16 *>(u & ~(1ull << 63)) + (size_t)k * CHUNK, n)
+                                 : piece_norm<INF>(reinterpret_cast<const float *>(u) + (size_t)k * CHUNK, n);
+        acc = INF ? nan_max(acc, v) : acc + v;
+    }
+    acc = INF ? block_max(acc, red) : block_sum(acc, red);
+    if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+}
+
+template <typename T>
+__device__ __forceinline__ void piece_scale(T *p, unsigned n, float f) {
+    walk_piece<T>(p, n,
+        [&](T *q) {
+#pragma unroll
+            for (unsigned e = 0; e < 16 / sizeof(T); e += 4) st4(q + e, ld4(q + e) * f);
+        },
+        [&](T *q) { st1(q, ld1(q) * f); });
+}
+
+template <bool INF>
+__global__ __launch_bounds__(NT) void grad_scale_kernel(const Table t, const double *partials, int nparts, float max_norm, float *norm, int write_norm,
+                                                       unsigned per) {
+    __shared__ double red[4];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < nparts; i += NT) s = INF ? nan_max(s, partials[i]) : s + partials[i];
+    s = INF ? block_max(s, red) : block_sum(s, red);
+    const float nrm = (float)(INF ? s : sqrt(s));
+    if (write_norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = nrm;
+    const float f = (float)((double)max_norm / ((double)nrm + 1e-6));
+    if (f >= 1.0f) return;                                  // (NaN scales: a norm that is not a number reaches every gradient)
+    const unsigned blk = gridDim.x - 1 - blockIdx.x;
+    const unsigned a = blk * per, e = a + per < t.pieces ? a + per : t.pieces;
+    if (a >= e) return;
+    int i = find_tensor(t, e - 1);
+    for (unsigned c = e; c-- > a;) {
+        while (t.piece[i] > c) --i;
+        const unsigned stop = i + 1 < t.n ? t.piece[i + 1] : t.pieces, k = c - t.piece[i];
+        const unsigned n = c + 1 == stop ? t.tail[i] : CHUNK;
+        const unsigned long long u = t.ptr[i];
+        if (u >> 63) piece_scale(reinterpret_cast<bf16 *>(u & ~(1ull << 63)) + (size_t)k * CHUNK, n, f);
+        else piece_scale(reinterpret_cast<float *>(u) + (size_t)k * CHUNK, n, f);
+    }
+}
+
+// one launch's table from tensors [i, ...): as many as fit
+int fill(Table &t, const unsigned char *bf, const unsigned long long *ptrs, const long long *sizes, int n, int i) {
+    t.n = 0;
+    t.pieces = 0;
+    for (; i < n && t.n < MAXT; ++i) {
+        if (sizes[i] == 0) continue;
+        const long long np = (sizes[i] + CHUNK - 1) / CHUNK;
+        if (t.pieces + np > 0x7fffffffLL) break;
+        t.ptr[t.n] = ptrs[i] | (bf[i] ? 1ull << 63 : 0);
+        t.piece[t.n] = t.pieces;
+        t.tail[t.n] = (unsigned)(sizes[i] - (np - 1) * CHUNK);
+        t.pieces += (unsigned)np;
+        ++t.n;
+    }
+    return i;
+}
+unsigned wgs_of(const Table &t, unsigned &per) {
+    per = (t.pieces + MAX_WGS - 1) / MAX_WGS;
+    return (t.pieces + per - 1) / per;
+}
+
+}  // namespace
+
+extern "C" size_t ss2d_grad_clip_workspace_bytes(int n) { return n < 0 ? 0 : (size_t)(n / MAXT + 2) * MAX_WGS * sizeof(double); }
+
+extern "C" int ss2d_grad_clip(const unsigned char *is_bf16, const unsigned long long *ptrs, const long long *sizes, int n, int inf_norm, float max_norm,
+                              int scale, float *norm, double *workspace, size_t workspace_bytes, void *stream) {
+    if (!is_bf16 || !ptrs || !sizes || !norm || !workspace || n <= 0) { ss2d_set_error("grad_clip: null pointer or no tensors"); return -2; }
+    if (workspace_bytes < ss2d_grad_clip_workspace_bytes(n)) { ss2d_set_error("grad_clip: workspace too small"); return -8; }
+    if (!(max_norm >= 0.0f)) { ss2d_set_error("grad_clip: max_norm must be >= 0"); return -3; }
+    for (int i = 0; i < n; ++i) {
+        const int es = is_bf16[i] ? 2 : 4;
+        if (sizes[i] < 0 || sizes[i] > (1LL << 45) || (sizes[i] && (!ptrs[i] || ptrs[i] % es || ptrs[i] >> 63))) {
+            ss2d_set_error("grad_clip: tensor %d has a bad address or size", i); return -3; }
+    }
+    int order_ok = 1;                                       // ascending and disjoint, as pieces of a bucket are: nothing to sort
+    for (int i = 1; i < n && order_ok; ++i) order_ok = ptrs[i] >= ptrs[i - 1] + (unsigned long long)sizes[i - 1] * (is_bf16[i - 1] ? 2 : 4);
+    if (!order_ok) {
+        int *ord = static_cast<int *>(malloc(sizeof(int) * (size_t)n));
+        if (!ord) { ss2d_set_error("grad_clip: out of host memory"); return -9; }
+        for (int i = 0; i < n; ++i) ord[i] = i;
+        std::sort(ord, ord + n, [&](int a, int b) { return ptrs[a] != ptrs[b] ? ptrs[a] < ptrs[b] : sizes[a] < sizes[b]; });
+        int bad = -1;
+        unsigned long long end = 0;
+        for (int j = 0; j < n && bad < 0; ++j) {
+            const int i = ord[j];
+            if (!sizes[i]) continue;
+            if (ptrs[i] < end) bad = i;
+            end = ptrs[i] + (unsigned long long)sizes[i] * (is_bf16[i] ? 2 : 4);
+        }
+        free(ord);
+        if (bad >= 0) { ss2d_set_error("grad_clip: tensor %d shares memory with another one", bad); return -4; }
+    }
+    hipStream_t s = (hipStream_t)stream;
+    Table t;
+    int parts = 0;
+    unsigned per;
+    for (int i = 0; i < n;) {
+        i = fill(t, is_bf16, ptrs, sizes, n, i);
+        if (!t.n) break;
+        const unsigned w = wgs_of(t, per);
+        if (inf_norm) ss2d_launch(grad_norm_kernel<true>, dim3(w), dim3(NT), 0, s, t, workspace + parts, per);
+        else ss2d_launch(grad_norm_kernel<false>, dim3(w), dim3(NT), 0, s, t, workspace + parts, per);
+        parts += (int)w;
+    }
+    int first = 1;
+    for (int i = 0; i < n || first;) {
+        i = fill(t, is_bf16, ptrs, sizes, n, i);
+        if (!t.n && !first) break;
+        unsigned w = t.n && scale ? wgs_of(t, per) : 1;
+        if (!t.n || !scale) { t.n = 0; t.pieces = 0; per = 0; }
+        if (inf_norm) ss2d_launch(grad_scale_kernel<true>, dim3(w), dim3(NT), 0, s, t, workspace, parts, max_norm, norm, first, per);
+        else ss2d_launch(grad_scale_kernel<false>, dim3(w), dim3(NT), 0, s, t, workspace, parts, max_norm, norm, first, per);
+        first = 0;
+        if (!scale) break;
+    }
+    const int rc = ss2d_take_launch_rc();
+    if (rc) ss2d_set_error("grad_clip: launch failed: %s", hipGetErrorString((hipError_t)rc));
+    return rc;
+}

@@ -765,6 +765,103 @@ def outnorm_gate(y: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, bias: t
     return _OutNormGate.apply(y, z, weight, bias, eps, holder, scale)
 
 
+def _norm_rows(t, io, D):
+    """t as (rows, D) rows in the storage type with a dense last axis and one distance between rows: in place where t has that
+    layout (a channel slice of a wider tensor), else a copy.  Returns the tensor and the distance."""
+    t = t if t.dtype == io else t.to(io)
+    if t.is_contiguous():
+        ld = D
+    else:
+        ld = t.stride(-2) if t.dim() > 1 else D
+        rows = all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 2))
+        if t.stride(-1) != 1 or not rows or ld < D or (D % 8 == 0 and ld % 8):
+            t, ld = t.contiguous(), D
+    if D % 8 == 0 and t.data_ptr() % 16:
+        t, ld = t.clone(memory_format=torch.contiguous_format), D
+    return t, ld
+
+
+class _NormGateResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, z, w1, b1, a, w2, b2, drop, eps, rms):
+        ctx.set_materialize_grads(False)
+        D = x.shape[-1]
+        rows = x.numel() // D
+        (rt, rcode), (io, code) = _io(x), _io(y)
+        (x_, ldx), (y_, ldy) = _norm_rows(x, rt, D), _norm_rows(y, io, D)
+        z_, ldz = (None, D) if z is None else _norm_rows(z, io, D)
+        f32 = lambda t: None if t is None else t.detach().float().contiguous()  # noqa: E731
+        w1_, b1_, a_, w2_, b2_, drop_ = f32(w1), f32(b1), f32(a), f32(w2), f32(b2), f32(drop)
+        x_out, h = torch.empty(x.shape, device=x.device, dtype=rt), torch.empty(x.shape, device=x.device, dtype=io)
+        stats = torch.empty((rows, 4), device=x.device, dtype=torch.float32) if any(ctx.needs_input_grad) else None
+        rps = rows // drop.numel() if drop is not None and drop.numel() else 0
+        ctx.rows = rows
+        if rows:
+            p = _lib.ptr
+            with _lib.on_device(x.device):
+                rc = _lib.load().ss2d_block_norm_fwd(rcode, code, p(x_), p(y_), p(z_), p(w1_), p(b1_), p(w2_), p(b2_), p(a_), p(drop_), rps, p(x_out), p(h),
+                                                     p(stats), rows, D, ldx, ldy, ldz, float(eps), int(rms), _stream())
+            _lib.check(rc, "ss2d_block_norm_fwd")
+        if stats is not None:
+            ctx.save_for_backward(x_, y_, z_, w1_, b1_, a_, w2_, drop_, stats)
+        ctx.meta = (rcode, code, D, ldx, ldy, ldz, rps, int(rms), x.shape, [None if t is None else t.dtype for t in (x, y, z, w1, b1, a, w2, b2)])
+        return x_out.to(x.dtype), h.to(y.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dx_out, dh):
+        if dx_out is None and dh is None:
+            return (None,) * 11
+        x, y, z, w1, b1, a, w2, drop, stats = ctx.saved_tensors
+        rcode, code, D, ldx, ldy, ldz, rps, rms, shape, dt = ctx.meta
+        dev, rows = x.device, ctx.rows
+        aligned = lambda t: t.clone() if t is not None and t.data_ptr() % 16 else t  # noqa: E731
+        gx = aligned(None if dx_out is None else dx_out.to(x.dtype).contiguous())
+        gh = aligned(None if dh is None else dh.to(y.dtype).contiguous())
+        dx, dy = torch.empty(shape, device=dev, dtype=x.dtype), torch.empty(shape, device=dev, dtype=y.dtype)
+        dz = None if z is None else torch.empty(shape, device=dev, dtype=y.dtype)
+        if rows:
+            lib, p = _lib.load(), _lib.ptr
+            dp = torch.empty((5, D), device=dev, dtype=torch.float32)
+            ws = torch.empty(int(lib.ss2d_block_norm_bwd_workspace_floats(rows, D)), device=dev, dtype=torch.float32)
+            with _lib.on_device(dev):
+                rc = lib.ss2d_block_norm_bwd(rcode, code, p(gx), p(gh), p(x), p(y), p(z), p(w1), p(b1), p(w2), p(a), p(drop), rps, p(stats), p(dx), p(dy),
+                                             p(dz), p(dp), p(ws), rows, D, ldx, ldy, ldz, rms, _stream())
+            _lib.check(rc, "ss2d_block_norm_bwd")
+        else:
+            dp = torch.zeros((5, D), device=dev, dtype=torch.float32)
+        grads = (dx, dy, dz, dp[0], dp[1], dp[2], dp[3], dp[4])
+        return tuple(g.to(d) if d is not None and n else None for g, d, n in zip(grads, dt, ctx.needs_input_grad)) + (None, None, None)
+
+
+def norm_gate_residual(x, y, post_weight, pre_weight, post_bias=None, pre_bias=None, z=None, res_scale=None, drop_scale=None, eps: float = 1e-5,
+                       rms: bool = False):
+    """The norms on both sides of a block with its gate and residual scale, fused: with the residual stream x and the block's output y,
+
+        u = norm(y; post_weight, post_bias) * SiLU(z),   x' = x + drop_scale * res_scale * u,   h = norm(x'; pre_weight, pre_bias)
+
+    Returns (x', h): the new residual stream in x's dtype and the next block's input in y's dtype.  norm: LayerNorm over the last axis, or RMS norm
+    with `rms`; statistics in fp32, h from the unrounded x'.  z (y's shape; a channel slice of a wider tensor is read in place), the biases,
+    res_scale (D,) and drop_scale (one factor per sample, not differentiated) are optional.  bf16 x and y / z stay bf16 in memory (x may be fp32 with a bf16
+    branch); D <= 8192."""
+    for name, t in (("x", x), ("y", y), ("z", z), ("post_weight", post_weight), ("pre_weight", pre_weight), ("post_bias", post_bias), ("pre_bias", pre_bias),
+                    ("res_scale", res_scale), ("drop_scale", drop_scale)):
+        if t is None:
+            continue
+        _need_gpu(t, f"norm_gate_residual: `{name}`")
+        if t.device != x.device:
+            raise ValueError(f"norm_gate_residual: `{name}` is on {t.device}, x on {x.device}")
+        if name in ("y", "z") and t.shape != x.shape:
+            raise ValueError(f"norm_gate_residual: `{name}` must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
+        if name not in ("x", "y", "z", "drop_scale") and t.shape != x.shape[-1:]:
+            raise ValueError(f"norm_gate_residual: `{name}` must be ({x.shape[-1]},), got {tuple(t.shape)}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
+        raise ValueError(f"norm_gate_residual: the last axis must hold 1 ... 8192 channels, got {tuple(x.shape)}")
+    if drop_scale is not None and (x.dim() < 2 or drop_scale.numel() != x.shape[0]):
+        raise ValueError("norm_gate_residual: `drop_scale` must hold one factor per sample")
+    return _NormGateResidual.apply(x, y, z, post_weight, post_bias, res_scale, pre_weight, pre_bias, drop_scale, eps, bool(rms))
+
+
 class _LayerNorm(torch.autograd.Function):
     """LayerNorm over the last axis; with ps > 0 over the rows of a ps x ps pixel un-shuffle of x (B, H, W, ps*ps*D):
     out (B, H*ps, W*ps, D) = norm(rearrange(x, 'b h w (p1 p2 c) -> b (h p1) (w p2) c')), gathered inside the kernel;

@@ -8,10 +8,12 @@
 from __future__ import annotations
 
 import os as _os
+from array import array
 
 import torch
 import torch.nn.functional as F
 
+from . import _lib
 from .dist import all_reduce_sum
 from .ss2d_ops import seg_loss_stats
 
@@ -145,15 +147,75 @@ def set_lr(optimizer, lr: float):
             g["lr"] = lr
 
 
-def supervised_step(model, optimizer, images, labels, n_classes, it, max_it, base_lr=0.01, autocast_bf16=False):
+def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """Scales the gradients in place by min(1, max_norm / (norm + 1e-6)) with their global norm (2 or inf) and returns the norm, a 0-dim
+    fp32 tensor: what torch.nn.utils.clip_grad_norm_ computes, without a host read of the norm (so it can be captured in a HIP graph) and in two
+    launches for up to 240 tensors.  `grads`: tensors, or parameters, whose .grad is taken (None: left out); fp32 or bf16, on one
+    GPU, none sharing memory with another.  The norm is summed in 64 bits in a fixed order; one that is not a number makes every
+    gradient not a number.  max_norm = inf only measures."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    grads = [g.grad if type(g) is torch.nn.Parameter else g for g in grads]
+    grads = [g for g in grads if g is not None]
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    if not max_norm >= 0.0:
+        raise ValueError(f"clip_grad_norm: max_norm must be >= 0, got {max_norm}")
+    if norm_type not in (2.0, float("inf")):
+        raise ValueError(f"clip_grad_norm: norm_type must be 2 or inf, got {norm_type}")
+    if not grads:
+        return torch.tensor(0.0)
+    devs, types = set(map(torch.Tensor.get_device, grads)), [g.dtype for g in grads]
+    if min(devs) < 0:
+        raise RuntimeError("clip_grad_norm: GPU tensors required (no CPU path in mamba_unet_amd)")
+    if len(devs) > 1:
+        raise ValueError(f"clip_grad_norm: gradients on several devices: {sorted(devs)}")
+    if not set(types) <= {torch.float32, torch.bfloat16}:
+        raise ValueError(f"clip_grad_norm: fp32 or bf16 gradients required, got {set(types)}")
+    dev = grads[0].device
+    work = grads
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        # dense in another order (channels last): the elements are the same; anything else goes through a copy
+        work = [g if g.is_contiguous() else _dense_view(g) for g in grads]
+    n = len(grads)
+    lib = _lib.load()
+    ptrs = array("Q", map(torch.Tensor.data_ptr, work))
+    sizes = array("q", map(torch.Tensor.numel, work))
+    kinds = bytes([t is torch.bfloat16 for t in types])
+    nbytes = lib.ss2d_grad_clip_workspace_bytes(n)
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    ws = torch.empty(nbytes // 8, device=dev, dtype=torch.float64)
+    with _lib.on_device(dev):
+        rc = lib.ss2d_grad_clip(kinds, ptrs.buffer_info()[0], sizes.buffer_info()[0], n, int(norm_type != 2.0), max_norm, int(max_norm != float("inf")),
+                                norm.data_ptr(), ws.data_ptr(), nbytes, _lib.stream())
+    _lib.check(rc, "ss2d_grad_clip")
+    if max_norm != float("inf"):
+        if work is not grads:
+            with torch.no_grad():
+                for g, w in zip(grads, work):
+                    if w.data_ptr() != g.data_ptr():
+                        g.copy_(w)
+        torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+def _dense_view(g):
+    """g's elements as a dense tensor: a view where g fills its memory in some order of its axes, else a copy."""
+    order = sorted((i for i in range(g.dim()) if g.shape[i] != 1), key=lambda i: -g.stride(i))
+    v = g.detach().permute(order + [i for i in range(g.dim()) if g.shape[i] == 1])
+    return v if v.is_contiguous() else g.detach().contiguous()
+
+
+def supervised_step(model, optimizer, images, labels, n_classes, it, max_it, base_lr=0.01, autocast_bf16=False, max_grad_norm=None):
     """One iteration of train_fully_supervised_2D_VIM.py:150-164.  Returns the (detached) loss tensor; no
-    .item() here: the reference syncs every iteration for tensorboard (:172-174), the caller decides."""
+    .item() here: the reference syncs every iteration for tensorboard (:172-174), the caller decides.
+    `max_grad_norm`: clip the gradients to this global norm in front of the update (clip_grad_norm)."""
     with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast_bf16):
         out = model(images)
     loss_ce, loss_dice = ce_dice_loss(out, labels, n_classes)     # softmax, CE and the Dice sums: one pass over the logits
     loss = 0.5 * (loss_dice + loss_ce)
     optimizer.zero_grad(set_to_none=True)
     loss.backward()
+    if max_grad_norm is not None:
+        clip_grad_norm(model.parameters(), max_grad_norm)
     optimizer.step()
     set_lr(optimizer, poly_lr(base_lr, it, max_it))
     return loss.detach()
@@ -211,7 +273,8 @@ class GraphedSupervisedStep:
     package now (ss2d_seg_loss_stats, ss2d_colsum), and ten replays reproduce ten eager steps to the last bit of the
     loss (tests/test_configs_gpu.py::test_graphed_supervised_step_matches_eager, tools/graph_vs_eager.py)."""
 
-    def __init__(self, model, optimizer, images, labels, n_classes, max_it, base_lr=0.01, autocast_bf16=False, warmup=3):
+    def __init__(self, model, optimizer, images, labels, n_classes, max_it, base_lr=0.01, autocast_bf16=False, warmup=3,
+                 max_grad_norm=None):
         self.opt, self.max_it, self.base_lr = optimizer, max_it, base_lr
         self.images, self.labels = images.clone(), labels.clone()
         args = (model, optimizer, self.images, self.labels, n_classes)
@@ -219,12 +282,12 @@ class GraphedSupervisedStep:
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             for i in range(warmup):   # allocator, MIOpen / hipBLASLt heuristics and autograd warm up eagerly
-                supervised_step(*args, i, max_it, base_lr, autocast_bf16)
+                supervised_step(*args, i, max_it, base_lr, autocast_bf16, max_grad_norm)
         torch.cuda.current_stream().wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
         optimizer.zero_grad(set_to_none=True)
         with torch.cuda.graph(self.graph):
-            self.loss = supervised_step(*args, warmup, max_it, base_lr, autocast_bf16)
+            self.loss = supervised_step(*args, warmup, max_it, base_lr, autocast_bf16, max_grad_norm)
 
     def __call__(self, images, labels, it):
         if images is not self.images:
@@ -293,16 +356,20 @@ def semi_loss(o1, o2, labels, labeled_bs, n_classes, consistency_weight):
 
 
 def semi_step(model1, model2, opt1, opt2, images, labels, labeled_bs, n_classes, it, max_it, consistency_weight,
-              base_lr=0.01, autocast_bf16=False):
+              base_lr=0.01, autocast_bf16=False, max_grad_norm=None):
     """Cross pseudo supervision between two networks + ConstraLoss (train_Semi_Mamba_UNet.py:411-463).  `it` is the
     0-based iteration: the reference increments iter_num BEFORE it evaluates the poly schedule (:458-461), so the
-    learning rate set here is poly_lr(it + 1) (the supervised script evaluates it before the increment)."""
+    learning rate set here is poly_lr(it + 1) (the supervised script evaluates it before the increment).
+    `max_grad_norm`: clip each network's gradients to this global norm (clip_grad_norm)."""
     with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast_bf16):
         o1, o2 = model1(images), model2(images)
     loss = semi_loss(o1, o2, labels, labeled_bs, n_classes, consistency_weight)
     opt1.zero_grad(set_to_none=True)
     opt2.zero_grad(set_to_none=True)
     loss.backward()
+    if max_grad_norm is not None:
+        for m in (model1, model2):
+            clip_grad_norm(m.parameters(), max_grad_norm)
     opt1.step()
     opt2.step()
     for opt in (opt1, opt2):

@@ -72,8 +72,9 @@ _SIGNATURES = {
     "ss2d_layernorm_unshuffle_bwd": (_i, [_i, _i] + [_vp] * 8 + [ctypes.c_longlong, _i, _i, _i, _i, _vp]),
     "ss2d_layernorm_merge_fwd": (_i, [_i, _i, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_longlong, _i, _i, _i, ctypes.c_float, _vp]),
     "ss2d_layernorm_merge_bwd": (_i, [_i, _i] + [_vp] * 8 + [ctypes.c_longlong, _i, _i, _i, _vp]),
-    "ss2d_linattn_chunk": (_i, [_i, _i]),
-    "ss2d_linattn_segment_chunks": (_i, [_i, ctypes.c_longlong, _i, _i, _i, _i]),
+    "ss2d_linattn_chunk": (_i, [_i, _i, _i]),
+    "ss2d_linattn_state_floats": (ctypes.c_longlong, [_i, _i, _i]),
+    "ss2d_linattn_segment_chunks": (_i, [_i, ctypes.c_longlong, ctypes.c_longlong, _i, _i, _i, _i]),
     "ss2d_linattn_fwd": (_i, [_i] + [_vp] * 12 + [_i, ctypes.c_longlong, _i, _i, _i, _i, ctypes.c_float, _i, _i, _vp]),
     "ss2d_linattn_bwd": (_i, [_i] + [_vp] * 18 + [_i, ctypes.c_longlong, _i, _i, _i, _i, ctypes.c_float, _i, _i, _vp]),
     "ss2d_linattn_step": (_i, [_i] + [_vp] * 7 + [_i, _vp, ctypes.c_longlong, ctypes.c_longlong] + [_i] * 5 + [ctypes.c_float, _vp]),

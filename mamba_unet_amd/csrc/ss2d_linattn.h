@@ -69,15 +69,29 @@ __device__ __forceinline__ float limit_decay(float g) { return g < -150.0f ? -15
 // Inclusive prefix sums of log2(e) * g over the lanes of a wave (C <= 64 tokens), in 64 bits: the sum over a chunk that holds a
 // reset is ~200 per reset, and the decays behind the reset must not lose their last bits to it.  A pair's decay is
 // exp2((hi_i - hi_j) + (lo_i - lo_j)) with hi + lo = b.
-__device__ __forceinline__ double chunk_decay_scan(float g, int lane) {
-    double b = (double)g * 1.4426950408889634074;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(b, d, 64);
-        if (lane >= d) b += o;
-    }
-    return b;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double b) {          // b + (b of the lane that CTRL names; 0 where there is none or the row is not in ROWS)
+    const long long u = __builtin_bit_cast(long long, b);
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return b + __builtin_bit_cast(double, (long long)((unsigned long long)hi << 32 | lo));
 }
+__device__ __forceinline__ double chunk_decay_scan(float g) {
+    double b = (double)g * 1.4426950408889634074;
+    b = dpp_add<DPP_ROW_SHR(1), 0xf>(b);
+    b = dpp_add<DPP_ROW_SHR(2), 0xf>(b);
+    b = dpp_add<DPP_ROW_SHR(4), 0xf>(b);
+    b = dpp_add<DPP_ROW_SHR(8), 0xf>(b);
+    b = dpp_add<0x142, 0xa>(b);                                // lane 15 of rows 0 and 2 into rows 1 and 3
+    return dpp_add<0x143, 0xc>(b);                             // lane 31 into rows 2 and 3
+}
+__device__ __forceinline__ double lane63(double b) {
+    const long long u = __builtin_bit_cast(long long, b);
+    const unsigned lo = __builtin_amdgcn_readlane((int)u, 63), hi = __builtin_amdgcn_readlane((int)(u >> 32), 63);
+    return __builtin_bit_cast(double, (long long)((unsigned long long)hi << 32 | lo));
+}
+
+// a value that the compiler takes as new: addresses made from it are computed where they are used instead of living across a loop
+__device__ __forceinline__ int fresh(int v) { asm volatile("" : "+v"(v)); return v; }
 
 // rows [0, C) of `src` (row stride ld, D columns, rows >= n read as zero) -> fp32 tile in LDS, PITCH floats a row, columns
 // D .. DP-1 zero
@@ -101,20 +115,130 @@ __device__ __forceinline__ void load_tile(float *dst, const IO *src, long long l
     }
 }
 
+// ---- bf16 operands on v_mfma_f32_16x16x32_bf16.  A lane (l16 = lane & 15, gq = lane >> 4) holds row / column l16 of an operand and eight of the 32
+// contracted indices.  Here they are 4 gq + {0..3} and 16 + 4 gq + {0..3} for every operand: the two halves are then exactly the rows that
+// the lane holds of two neighbouring 16 x 16 results, so a state in accumulators is an operand without moving data.
+// fp32 factors (states, weighted values, weights) enter as sums of two or three bf16 values: two leave 2^-17 of a term, below the rounding
+// of a bf16 result; three leave nothing of its 24 bits, for what stays in fp32 (states, gradients of the decays).
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f4 mfma8(bf16x8 a, bf16x8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ bf16x8 join8(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ bf16x4 round4(f4 v) { return __builtin_convertvector(v, bf16x4); }
+// v minus its rounded value; the halves are taken from the packed words (converted back one by one, the compiler rounds them a second time)
+__device__ __forceinline__ f4 rest4(f4 v, bf16x4 h) {
+    const u32x2 w = __builtin_bit_cast(u32x2, h);
+    const unsigned a = w.x, b = w.y;
+    return f4{v.x - __builtin_bit_cast(float, a << 16), v.y - __builtin_bit_cast(float, a & 0xffff0000u), v.z - __builtin_bit_cast(float, b << 16),
+              v.w - __builtin_bit_cast(float, b & 0xffff0000u)};
+}
+__device__ __forceinline__ void widen8(bf16x8 v, f4 &a, f4 &b) {
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+    const unsigned w0 = w.x, w1 = w.y, w2 = w.z, w3 = w.w;
+    a = f4{__builtin_bit_cast(float, w0 << 16), __builtin_bit_cast(float, w0 & 0xffff0000u), __builtin_bit_cast(float, w1 << 16), __builtin_bit_cast(float, w1 & 0xffff0000u)};
+    b = f4{__builtin_bit_cast(float, w2 << 16), __builtin_bit_cast(float, w2 & 0xffff0000u), __builtin_bit_cast(float, w3 << 16), __builtin_bit_cast(float, w3 & 0xffff0000u)};
+}
+// eight fp32 values -> NT bf16 operands that add up to them
+template <int N>
+__device__ __forceinline__ void split8(f4 a, f4 b, bf16x8 (&o)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bf16x4 x = round4(a), y = round4(b);
+        o[i] = join8(x, y);
+        if (i + 1 < N) { a = rest4(a, x); b = rest4(b, y); }
+    }
+}
+// An operand from LDS, contracted index contiguous: row `row`, indices 32 s + ...  Two 8-byte reads that are kept apart: merged into one
+// instruction they cost 8 to 32 cycles by pitch, apart 4 to 8 (2 x 16 rows x 8 bytes).
+__device__ __forceinline__ bf16x8 frag(const unsigned char *tile, int pitch, int row, int s, int gq) {
+    const int at = row * pitch + (32 * s + 4 * gq) * 2;
+    return join8(*reinterpret_cast<const bf16x4 *>(tile + at), *reinterpret_cast<const bf16x4 *>(tile + fresh(at + 32)));
+}
+// the same from a tile whose 32-column blocks are stored in operand order (index 16 u + 4 a + r at 8 a + 4 u + r): one 16-byte read
+__device__ __forceinline__ bf16x8 frag_p(const unsigned char *tile, int pitch, int row, int s, int gq) {
+    return *reinterpret_cast<const bf16x8 *>(tile + row * pitch + (32 * s + 8 * gq) * 2);
+}
+__device__ __forceinline__ int operand_pos(int c) { return (c & ~31) + 8 * ((c >> 2) & 3) + 4 * ((c >> 4) & 1); }      // of a group of four, c % 4 == 0
+__device__ __forceinline__ int operand_index(int pos) { return (pos & ~31) + 16 * ((pos >> 2) & 1) + 4 * ((pos >> 3) & 3) + (pos & 3); }   // its inverse
+// an operand from LDS, contracted index along the rows (rows 32 s + ...), columns 16 c .. 16 c + 15: ds_read_b64_tr_b16 hands every lane of 16 its
+// column of four rows; lane 4 a + b of the 16 addresses row a, columns 4 b .. 4 b + 3
+__device__ __forceinline__ bf16x8 frag_t(const unsigned char *tile, int pitch, int c, int s, int lane) {
+    typedef s16x4 __attribute__((address_space(3))) *lp;
+    const unsigned char *q = tile + (32 * s + 4 * (lane >> 4) + ((lane >> 2) & 3)) * pitch + (16 * c + 4 * (lane & 3)) * 2;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 16 * pitch));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A C x DP tile of bf16 on its way from memory to LDS, 16-byte pieces; rows past n and columns past D are zero.  VEC: the pieces wait in registers, so
+// a chunk is in flight while the previous one is worked on; else (rows not made of 16-byte pieces) elements go straight to LDS.
+template <int C, int DP, int NT, bool VEC>
+struct TileRegs {
+    static constexpr int PR = DP / 8, N = C * PR / NT > 0 ? C * PR / NT : 1;      // pieces a row, pieces a thread
+    u32x4 v[VEC ? N : 1];
+    int voff;                                                      // bytes from the chunk's first row; pieces past D lie outside every descriptor
+    __device__ __forceinline__ void init(long long ld, int D) {
+        const int r = threadIdx.x / PR, c = 8 * (threadIdx.x % PR);
+        voff = c < D && r < C ? (r * (int)ld + c) * 2 : SS2D_BUF_OOR;
+    }
+    // a descriptor of n rows: later rows read as zero.  ld < 2^23 elements (host)
+    __device__ __forceinline__ void load(const bf16 *src, long long ld, int n) {
+        if (!VEC) return;
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(src, (unsigned)(n * (int)ld * 2));
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[VEC ? j : 0] = __builtin_amdgcn_raw_buffer_load_b128(rs, voff, j * (NT / PR) * (int)ld * 2, 0);
+    }
+    // ORDERED: 32-column blocks in operand order (frag_p)
+    template <bool ORDERED = false>
+    __device__ __forceinline__ void put(unsigned char *tile, int pitch, const bf16 *src, long long ld, int n, int D) const {
+        if (VEC) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int e = threadIdx.x + j * NT, r = e / PR, c = 8 * (e % PR);
+                if (C * PR % NT == 0 || r < C) {
+                    const u32x4 w = v[VEC ? j : 0];
+                    unsigned char *d = tile + r * pitch;
+                    if (ORDERED) {
+                        *reinterpret_cast<u32x2 *>(d + 2 * operand_pos(c)) = u32x2{w.x, w.y};
+                        *reinterpret_cast<u32x2 *>(d + 2 * operand_pos(c + 4)) = u32x2{w.z, w.w};
+                    } else {
+                        *reinterpret_cast<u32x4 *>(d + 2 * c) = w;
+                    }
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int e = threadIdx.x; e < C * DP / 2; e += NT) {
+                const int r = e / (DP / 2), c = 2 * (e % (DP / 2));
+                bf16x2 w = bf16x2{(bf16)0.0f, (bf16)0.0f};
+                if (r < n && c < D) w[0] = src[(long long)r * ld + c];
+                if (r < n && c + 1 < D) w[1] = src[(long long)r * ld + c + 1];
+                *reinterpret_cast<bf16x2 *>(tile + r * pitch + 2 * (ORDERED ? operand_pos(c & ~3) + (c & 3) : c)) = w;
+            }
+        }
+    }
+};
+
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // tokens of a chunk: the backward holds q, k, v, dout, a dk x dv state and two C x C matrices in 160 KB of LDS
-inline int linattn_chunk(int dk, int dv) { return dk <= 64 && dv <= 64 ? 64 : 32; }
+inline int linattn_chunk(int dtype, int dk, int dv) { return dtype || (dk <= 64 && dv <= 64) ? 64 : 32; }
 
-// Chunks a segment.  One workgroup walks a segment; fewer than about two workgroups a CU leave the card idle, and a segment costs
-// a second pass over k and v (q and dout in the backward) and a state's round trip, so it is at least four chunks long.
-inline int linattn_segment_chunks(int N, long long max_len, int H, int dk, int dv, int backward) {
-    const int C = linattn_chunk(dk, dv);
-    const long long nch = (max_len + C - 1) / C, walks = (long long)N * H * (backward ? 1 : (dv + 63) / 64);
-    const long long want = (512 + walks - 1) / walks;
-    long long segc = (nch + want - 1) / want;
+// Chunks a segment.  One workgroup walks a segment; with fewer workgroups than the card holds at once (two or three a CU) it idles, and a segment
+// costs a second pass over k and v (q and dout in the backward) and a state's round trip: so all tokens of all sequences and
+// heads are dealt to that many workgroups, at least four chunks each.
+inline int linattn_segment_chunks(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
+    const int C = linattn_chunk(dtype, dk, dv);
+    const long long nch = (max_len + C - 1) / C, all = (all_tokens + C - 1) / C * H * (backward || dtype ? 1 : (dv + 63) / 64);
+    const long long wgs = dtype && !backward && dv <= 64 ? 768 : 512;
+    long long segc = (all + wgs - 1) / wgs;
     if (segc < 4) segc = 4;
     return (int)(segc < nch ? segc : nch > 0 ? nch : 1);
+}
+
+// floats of one chunk's saved state.  bf16 kernels: accumulator order, padded to whole tiles (16-byte pieces of a wave side by side)
+inline long long linattn_state_floats(int dtype, int dk, int dv) {
+    return dtype ? (long long)(dk <= 32 ? 32 : dk <= 64 ? 64 : 128) * (dv <= 64 ? 64 : 128) : (long long)dk * dv;
 }
 
 inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, const void *v, const float *g, const long long *st, const int *cu,
@@ -131,8 +255,13 @@ inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, 
     const int m = 8;                                            // 16 bytes of bf16, 32 of fp32
     bool vec = dk % m == 0 && dv % m == 0 && ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0;
     for (int i = 0; i < 9; ++i) vec = vec && st[i] % m == 0;
+    // 16-byte pieces come through descriptors of a chunk's rows: dense enough not to overlap, and short of 2^31 bytes
+    vec = vec && st[1] >= dk && st[4] >= dk && st[7] >= dv && st[1] < (1 << 23) && st[4] < (1 << 23) && st[7] < (1 << 23);
     p.vec = vec;
     return 0;
 }
 
 }  // namespace linattn
+
+// the pass over bf16 segments that leaves their own contributions (forward: k v^T; reverse: q dout^T), defined beside the forward
+void linattn_segment_pass_bf16(const linattn::Problem &p, float *seg_states, double *seg_decay, const float *want_end, bool reverse, hipStream_t s);

@@ -83,10 +83,10 @@ __global__ __launch_bounds__(NT) void la_bwd_seg_kernel(const BwdArgs a) {
         load_tile<C, DK, PK, NT>(Qs, Q + r0 * p.ql, p.ql, nr, p.dk, p.vec);
         load_tile<C, 64, PV, NT>(Os, DO + r0 * ldo, ldo, nr, p.dv - 64 * vt, p.vec);
         const float gv = lane < nr ? limit_decay(g[(r0 + lane) * p.gl]) : 0.0f;
-        const double b = chunk_decay_scan(gv, lane), bend = __shfl(b, 63, 64);
+        const double b = chunk_decay_scan(gv), bend = lane63(b);
         total += bend;
-        const float eend = exp2f((float)bend);
-        if (wave == 0) eb[lane] = exp2f((float)b) * p.scale;
+        const float eend = hw_exp2((float)bend);
+        if (wave == 0) eb[lane] = hw_exp2((float)b) * p.scale;
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < KT; ++t) D[t] *= eend;
@@ -125,11 +125,23 @@ __global__ __launch_bounds__(NT) void la_join_bwd_kernel(const BwdArgs a, int C)
     const Seq s = get_seq(p, (int)(nh / p.H));
     const int nch = (s.len + C - 1) / C, ns = segments_of(p, nch);
     float v = a.dlast ? a.dlast[nh * sz + e] : 0.0f;
-    for (int i = ns - 1; i >= 0; --i) {
-        float *u = a.seg_states + (nh * p.nseg + i) * sz + e;
-        const float own = *u;
-        *u = v;
-        v = v * exp2f((float)a.seg_decay[nh * p.nseg + i]) + own;
+    float *u = a.seg_states + nh * p.nseg * sz + e;
+    const double *d = a.seg_decay + nh * p.nseg;
+    for (int i = ns - 1; i >= 0; i -= 8) {
+        float own[8], f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = i - j > 0 ? i - j : 0;
+            own[j] = u[k * sz];
+            f[j] = hw_exp2((float)d[k]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (i - j >= 0) {
+                u[(i - j) * sz] = v;
+                v = v * f[j] + own[j];
+            }
+        }
     }
     if (a.ds0) a.ds0[nh * sz + e] = v;
 }
@@ -205,14 +217,14 @@ __global__ __launch_bounds__(NT) void la_bwd_kernel(const BwdArgs a) {
             if (wave + 4 * m < VT)
                 each_tile_element<KT>([&](int t, int r) { Ds[(16 * t + 4 * gq + r) * PV + 16 * (wave + 4 * m) + l16] = D[m][t][r]; });
         const float gv = lane < nr ? limit_decay(g[(r0 + lane) * p.gl]) : 0.0f;
-        const double b = chunk_decay_scan(gv, lane), bend = __shfl(b, 63, 64);
-        const float eend = exp2f((float)bend);
+        const double b = chunk_decay_scan(gv), bend = lane63(b);
+        const float eend = hw_exp2((float)bend);
         if (wave == 0) {
             const float hi = (float)b;
             bh[lane] = hi;
             bl[lane] = (float)(b - hi);
-            eb[lane] = exp2f(hi) * p.scale;
-            wt[lane] = exp2f((float)(bend - b));
+            eb[lane] = hw_exp2(hi) * p.scale;
+            wt[lane] = hw_exp2((float)(bend - b));
         }
         parts[wave * 64 + lane] = 0.0f;                                  // gradient of b_i, a partial sum of every wave
         __syncthreads();
@@ -241,7 +253,7 @@ __global__ __launch_bounds__(NT) void la_bwd_kernel(const BwdArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * it + 4 * gq + r;
-                const float w = j <= i ? p.scale * exp2f((bh[i] - hj) + (bl[i] - lj)) : 0.0f;
+                const float w = j <= i ? p.scale * hw_exp2((bh[i] - hj) + (bl[i] - lj)) : 0.0f;
                 const float yw = j <= i ? y[r] * w : 0.0f, xw = j <= i ? x[r] * w : 0.0f;
                 const float m = j < i ? x[r] * yw : 0.0f;
                 Xs[i * PP + j] = xw;
@@ -391,6 +403,407 @@ __global__ __launch_bounds__(NT) void la_bwd_kernel(const BwdArgs a) {
     }
 }
 
+// The same walk for bf16 tensors on the bf16 matrix instruction: eight waves a workgroup, chunks of 64.  LDS holds the four tiles, X and Y (two terms
+// each) and the terms of ONE state at a time, transposed (dv x dk): first S (for dq), then D (for dk and dv); with NB = 1 (128 x 128) one
+// term at a time.  States enter with three terms where dg is taken from the product (q . S do, k . D v), with two in dv.
+// Orders: k, v, dout and the columns j of X and Y lie in operand order (one 16-byte read an operand); what is read transposed from such a
+// tile comes in that order too, so the rows of dq and dv and the columns of dk, dv and D are named by operand_index.
+template <int DK, int DV, bool VEC, typename QT>
+__global__ __launch_bounds__(512, 2) void la_bwd_bf16_kernel(const BwdArgs a) {
+    constexpr int NT = 512, C = 64, KT = DK / 16, KS = DK / 32, VT = DV / 16, VS = DV / 32;
+    constexpr int QP = 2 * DK + 32, VP = 2 * DV + 32, PP = 2 * C + 32, SP = 2 * DK + 16;      // bytes a row
+    constexpr int NB = DK == 128 && DV == 128 ? 1 : 3;                                        // terms of a state in LDS at once
+    constexpr int NI = KT / 2, NJ = VT / 2, TW = KT * VT / 8;                                 // tiles of a wave: rows of dq / dk, rows of dv, D
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * C * PP + NB * DV * SP + (10 * C + 8 * C + 8) * 4];
+    unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + C * PP, *Yh = Xl + C * PP,
+                  *Yl = Yh + C * PP, *St = Yl + C * PP;
+    float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + 8 * C;
+    const Problem &p = a.p;
+    const int tid = threadIdx.x, lane0 = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int walks = p.N * p.H * p.nseg;
+    const int hq = p.H > p.G ? p.H : p.G;                            // heads of dq / dk as written
+    if ((int)blockIdx.x >= walks) {                                  // packed rows that belong to no sequence
+        const int w = (int)blockIdx.x - walks;
+        zero_rows(p, static_cast<QT *>(a.dq), (long long)hq * p.dk, w, GAP_WGS);
+        zero_rows(p, static_cast<QT *>(a.dk_), (long long)hq * p.dk, w, GAP_WGS);
+        zero_rows(p, static_cast<bf16 *>(a.dv_), (long long)p.H * p.dv, w, GAP_WGS);
+        zero_rows(p, a.dg, p.H, w, GAP_WGS);
+        return;
+    }
+    int id = xcd_remap(blockIdx.x, walks);
+    const int h = id % p.H; id /= p.H;
+    const int seg = id % p.nseg, n = id / p.nseg;
+    const Seq s = get_seq(p, n);
+    const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
+    const int c1 = segment_end(p, seg, nch);
+    const bool empty = s.len == 0;
+    if (c0 >= c1 && !(empty && seg == 0)) return;
+    const int hk = h / (p.H / p.G);
+    const long long ldv = (long long)p.H * p.dv, ldq = (long long)hq * p.dk, nh = (long long)n * p.H + h, sz = (long long)p.dk * p.dv;
+    const long long t0 = s.row * p.tokens + s.start, e0 = (long long)(c1 - 1) * C;              // the tensors' pointers start at the last chunk
+    const bf16 *Q = static_cast<const bf16 *>(p.q) + s.row * p.qb + (s.start + e0) * p.ql + hk * p.qh;
+    const bf16 *K = static_cast<const bf16 *>(p.k) + s.row * p.kb + (s.start + e0) * p.kl + hk * p.kh;
+    const bf16 *V = static_cast<const bf16 *>(p.v) + s.row * p.vb + (s.start + e0) * p.vl + h * p.vh;
+    const bf16 *DO = static_cast<const bf16 *>(a.dout) + ((t0 + e0) * p.H + h) * (long long)p.dv;
+    const float *g = p.g + s.row * p.gb + s.start * p.gl + h * p.gh;
+    QT *DQ = static_cast<QT *>(a.dq) + ((t0 + e0) * hq + h) * (long long)p.dk;
+    QT *DKp = static_cast<QT *>(a.dk_) + ((t0 + e0) * hq + h) * (long long)p.dk;
+    bf16 *DVp = static_cast<bf16 *>(a.dv_) + ((t0 + e0) * p.H + h) * (long long)p.dv;
+    float *DG = a.dg + t0 * p.H + h;
+    const int kt = wave % KT, i0 = wave / KT * NI;                   // dq / dk: column tile, first row tile
+    const int vt = wave % VT, j0 = wave / VT * NJ, kd = VT == 8 ? 0 : wave / VT * TW;           // dv: column tile, first row tile; D: first row tile
+    f4 D[TW];
+    {
+        const int col = operand_index(16 * vt + (lane0 & 15));
+        const float *init = p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
+#pragma unroll
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = 16 * (kd + t) + 4 * (lane0 >> 4) + r;
+                D[t][r] = init && col < p.dv && k < p.dk ? init[k * p.dv + col] : 0.0f;
+            }
+    }
+    TileRegs<C, DK, NT, VEC> qr, kr;
+    TileRegs<C, DV, NT, VEC> vr, orr;
+    qr.init(p.ql, p.dk);
+    kr.init(p.kl, p.dk);
+    vr.init(p.vl, p.dv);
+    orr.init(ldv, p.dv);
+    f4 sr[TW];                                                       // S in D's arrangement
+    const f4 *saved = reinterpret_cast<const f4 *>(a.chunk_states) + ((chunk_base(p, s, n, C) + c1 - 1) * p.H + h) * (DK * DV / 4);
+    auto rows_of = [&](int c) { const int left = s.len - c * C; return left < C ? left : C; };
+    auto fetch = [&](int c) {
+        const int nr = rows_of(c);
+        qr.load(Q, p.ql, nr);
+        kr.load(K, p.kl, nr);
+        vr.load(V, p.vl, nr);
+        orr.load(DO, ldv, nr);
+        const int ln = fresh(lane0), col = operand_index(16 * vt + (ln & 15));
+        const f4 *src = saved + (col >> 4) * KT * 64 + (ln >> 4) * 16 + (col & 15);
+#pragma unroll
+        for (int t = 0; t < TW; ++t) sr[t] = src[64 * (kd + t)];
+    };
+    float gr = 0.0f;
+    auto fetch_g = [&](int c) {
+        if (wave == 0 && c >= c0) gr = lane0 < rows_of(c) ? limit_decay(g[((long long)c * C + lane0) * p.gl]) : 0.0f;
+    };
+    auto scan = [&](int c) {                                         // two chunks of: b (two terms), scale exp(b), exp(b_C - b), exp(b_C)
+        if (wave == 0 && c >= c0) {
+            float *d = decays + (c & 1) * 5 * C;
+            const double b = chunk_decay_scan(gr), bend = lane63(b);
+            const float hi = (float)b;
+            d[lane0] = hi;
+            d[C + lane0] = (float)(b - hi);
+            d[2 * C + lane0] = hw_exp2(hi) * p.scale;
+            d[3 * C + lane0] = hw_exp2((float)(bend - b));
+            if (lane0 == 63) d[4 * C] = hw_exp2((float)bend);
+        }
+    };
+    auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: gradients of b inside the chunk, summed from its end
+        if (wave == 1) {
+            double x = 0.0, e = 0.0;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) { x += (double)parts[w * C + lane0]; e += (double)corners[w]; }
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const double o = __shfl_down(x, d, 64);
+                if (lane0 + d < 64) x += o;
+            }
+            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(x + e);
+        }
+    };
+    auto put_terms = [&](const f4 (&x)[TW], int u0, bool ordered) {  // terms u0 ... u0 + NB - 1 of a state -> St, row dv, column k
+        const int ln = fresh(lane0), col = operand_index(16 * vt + (ln & 15));
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+            const int k = 16 * (kd + t) + 4 * (ln >> 4);
+            f4 v = x[t];
+            unsigned char *d = St + col * SP + 2 * (ordered ? operand_pos(k) : k);
+#pragma unroll
+            for (int u = 0; u < 3; ++u) {
+                if (u >= u0 + NB) break;
+                const bf16x4 w = round4(v);
+                if (u >= u0) *reinterpret_cast<bf16x4 *>(d + (NB == 3 ? u : 0) * DV * SP) = w;
+                v = rest4(v, w);
+            }
+        }
+    };
+    fetch_g(c1 - 1);
+    scan(c1 - 1);
+    fetch_g(c1 - 2);
+    if (c0 < c1) fetch(c1 - 1);
+#pragma unroll 1
+    for (int c = c1 - 1; c >= c0; --c) {
+        const int nr = rows_of(c);
+        const float *bh = decays + (c & 1) * 5 * C, *bl = bh + C, *eb = bl + C, *wt = eb + C, *tail = wt + C;
+        __syncthreads();
+        if (c + 1 < c1) finish_dg(c + 1);
+        qr.put(Qs, QP, Q, p.ql, nr, p.dk);
+        kr.template put<true>(Ks, QP, K, p.kl, nr, p.dk);
+        vr.template put<true>(Vs, VP, V, p.vl, nr, p.dv);
+        orr.template put<true>(Os, VP, DO, ldv, nr, p.dv);
+        float corner = 0.0f;                                         // <D, S>
+#pragma unroll
+        for (int t = 0; t < TW; ++t) corner += (sr[t].x * D[t].x + sr[t].y * D[t].y) + (sr[t].z * D[t].z + sr[t].w * D[t].w);
+        put_terms(sr, 0, true);
+        __syncthreads();
+        parts[wave * C + lane0] = 0.0f;
+        {   // X, Y and the sums of M below the diagonal (the even and the odd column tiles of a row tile are two waves')
+            const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
+            const int it = wave >> 1, i = 16 * it + l16;
+            bf16x8 qf[KS], of[VS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) qf[ks] = frag(Qs, QP, i, ks, gq);
+#pragma unroll
+            for (int vs = 0; vs < VS; ++vs) of[vs] = frag_p(Os, VP, i, vs, gq);
+            const float hi = bh[i], li = bl[i];
+            float rowsum = 0.0f;
+#pragma unroll 1
+            for (int jt = wave & 1; jt <= (it | 1); jt += 2) {
+                f4 x = f4{0, 0, 0, 0}, y = f4{0, 0, 0, 0};
+                if (jt <= it) {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) x = mfma8(frag_p(Ks, QP, 16 * jt + l16, ks, gq), qf[ks], x);
+#pragma unroll
+                    for (int vs = 0; vs < VS; ++vs) y = mfma8(frag_p(Vs, VP, 16 * jt + l16, vs, gq), of[vs], y);
+                    const f4 h4 = *reinterpret_cast<const f4 *>(bh + 16 * jt + 4 * gq), l4 = *reinterpret_cast<const f4 *>(bl + 16 * jt + 4 * gq);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = 16 * jt + 4 * gq + r;
+                        const float w = p.scale * hw_exp2((hi - h4[r]) + (li - l4[r]));
+                        const float yw = j <= i ? y[r] * w : 0.0f, m = j < i ? x[r] * yw : 0.0f;
+                        x[r] = j <= i ? x[r] * w : 0.0f;
+                        y[r] = yw;
+                        rowsum += m;
+                        const float cs = row16_sum(m);
+                        if (l16 == 0) parts[wave * C + j] -= cs;
+                    }
+                }
+                const int at = i * PP + 2 * operand_pos(16 * jt + 4 * gq);
+                const bf16x4 xh = round4(x), yh = round4(y);
+                *reinterpret_cast<bf16x4 *>(Xh + at) = xh;
+                *reinterpret_cast<bf16x4 *>(Xl + at) = round4(rest4(x, xh));
+                *reinterpret_cast<bf16x4 *>(Yh + at) = yh;
+                *reinterpret_cast<bf16x4 *>(Yl + at) = round4(rest4(y, yh));
+            }
+            rowsum += __shfl_xor(rowsum, 16, 64);
+            rowsum += __shfl_xor(rowsum, 32, 64);
+            if (gq == 0) parts[wave * C + i] += rowsum;
+        }
+        {   // dq
+            const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
+            f4 acc[NI];
+#pragma unroll
+            for (int m = 0; m < NI; ++m) acc[m] = f4{0, 0, 0, 0};
+#pragma unroll 1
+            for (int u0 = 0; u0 < 3; u0 += NB) {
+                if (u0 > 0) {
+                    __syncthreads();
+                    put_terms(sr, u0, true);
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int vs = 0; vs < VS; ++vs) {
+                    bf16x8 of[NI];
+#pragma unroll
+                    for (int m = 0; m < NI; ++m) of[m] = frag_p(Os, VP, 16 * (i0 + m) + l16, vs, gq);
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) {
+                        const bf16x8 sf = frag_t(St + u * DV * SP, SP, kt, vs, lane);
+#pragma unroll
+                        for (int m = 0; m < NI; ++m) acc[m] = mfma8(sf, of[m], acc[m]);
+                    }
+                }
+            }
+            const int k = operand_index(16 * kt + 4 * gq);
+#pragma unroll
+            for (int m = 0; m < NI; ++m) {
+                const int i = 16 * (i0 + m) + l16;
+                acc[m] *= eb[i];
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(Qs + i * QP + 2 * k);
+                const f2 q0 = bf16pair_to_f2(w.x), q1 = bf16pair_to_f2(w.y);
+                float d = (acc[m].x * q0.x + acc[m].y * q0.y) + (acc[m].z * q1.x + acc[m].w * q1.y);
+                d += __shfl_xor(d, 16, 64);
+                d += __shfl_xor(d, 32, 64);
+                if (gq == 0) parts[wave * C + i] += d;
+            }
+            __syncthreads();                                          // X, Y are there; S is done with
+            put_terms(D, 0, false);
+#pragma unroll
+            for (int js = 0; js < 2; ++js) {
+                const bf16x8 kf = frag_t(Ks, QP, kt, js, lane);
+#pragma unroll
+                for (int m = 0; m < NI; ++m) {
+                    if (js > (i0 + m) / 2) continue;
+                    acc[m] = mfma8(kf, frag_p(Yh, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
+                    acc[m] = mfma8(kf, frag_p(Yl, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < NI; ++m) {
+                const int i = 16 * (i0 + m) + l16;
+                if (i < nr) {
+                    QT *d = DQ + i * ldq + k;
+                    if (VEC) {
+                        if (k < p.dk) st4(d, acc[m]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (k + r < p.dk) st1(d + r, acc[m][r]);
+                    }
+                }
+            }
+        }
+        __syncthreads();                                              // D's terms are there
+        const float eend = tail[0];
+        Q -= C * p.ql; K -= C * p.kl; V -= C * p.vl; DO -= C * ldv; saved -= (long long)p.H * (DK * DV / 4);
+        if (NB == 3 && c > c0) fetch(c - 1);
+        {   // dk and dv
+            const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
+            f4 dk[NI], dv[NJ];
+#pragma unroll
+            for (int m = 0; m < NI; ++m) dk[m] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int m = 0; m < NJ; ++m) dv[m] = f4{0, 0, 0, 0};
+            const int vrow = operand_index(16 * vt + l16);
+#pragma unroll 1
+            for (int u0 = 0; u0 < 3; u0 += NB) {
+                if (u0 > 0) {
+                    __syncthreads();
+                    put_terms(D, u0, false);
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int vs = 0; vs < VS; ++vs) {
+                    bf16x8 vf[NI];
+#pragma unroll
+                    for (int m = 0; m < NI; ++m) vf[m] = frag_p(Vs, VP, operand_index(16 * (i0 + m) + l16), vs, gq);
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) {
+                        const bf16x8 df = frag_t(St + u * DV * SP, SP, kt, vs, lane);
+#pragma unroll
+                        for (int m = 0; m < NI; ++m) dk[m] = mfma8(df, vf[m], dk[m]);
+                    }
+                }
+                if (u0 < 2) {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        bf16x8 kf[NJ];
+#pragma unroll
+                        for (int m = 0; m < NJ; ++m) kf[m] = frag_p(Ks, QP, operand_index(16 * (j0 + m) + l16), ks, gq);
+#pragma unroll
+                        for (int u = 0; u < (NB == 3 ? 2 : 1); ++u) {
+                            const bf16x8 df = frag(St + u * DV * SP, SP, vrow, ks, gq);
+#pragma unroll
+                            for (int m = 0; m < NJ; ++m) dv[m] = mfma8(df, kf[m], dv[m]);
+                        }
+                    }
+                }
+            }
+            corner = lanes_sum<64>(corner) * eend;
+#pragma unroll
+            for (int m = 0; m < NI; ++m) {
+                const int j = operand_index(16 * (i0 + m) + l16);
+                dk[m] *= wt[j];
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(Ks + j * QP + 2 * operand_pos(16 * kt + 4 * gq));
+                const f2 k0 = bf16pair_to_f2(w.x), k1 = bf16pair_to_f2(w.y);
+                float d = (dk[m].x * k0.x + dk[m].y * k0.y) + (dk[m].z * k1.x + dk[m].w * k1.y);
+                corner += lanes_sum<64>(d);
+                d += __shfl_xor(d, 16, 64);
+                d += __shfl_xor(d, 32, 64);
+                if (gq == 0) parts[wave * C + j] -= d;
+            }
+            if (lane == 0) corners[wave] = corner;
+#pragma unroll
+            for (int m = 0; m < NJ; ++m) dv[m] *= wt[operand_index(16 * (j0 + m) + l16)];
+#pragma unroll
+            for (int is = 0; is < 2; ++is) {
+                const bf16x8 qf = frag_t(Qs, QP, kt, is, lane), of = frag_t(Os, VP, vt, is, lane);
+#pragma unroll
+                for (int m = 0; m < NI; ++m) {
+                    if (is < (i0 + m) / 2) continue;
+                    dk[m] = mfma8(qf, frag_t(Yh, PP, i0 + m, is, lane), dk[m]);
+                    dk[m] = mfma8(qf, frag_t(Yl, PP, i0 + m, is, lane), dk[m]);
+                }
+#pragma unroll
+                for (int m = 0; m < NJ; ++m) {
+                    if (is < (j0 + m) / 2) continue;
+                    dv[m] = mfma8(of, frag_t(Xh, PP, j0 + m, is, lane), dv[m]);
+                    dv[m] = mfma8(of, frag_t(Xl, PP, j0 + m, is, lane), dv[m]);
+                }
+            }
+            const int k = 16 * kt + 4 * gq, v = operand_index(16 * vt + 4 * gq);
+#pragma unroll
+            for (int m = 0; m < NI; ++m) {
+                const int j = operand_index(16 * (i0 + m) + l16);
+                if (j < nr) {
+                    QT *d = DKp + j * ldq + k;
+                    if (VEC) {
+                        if (k < p.dk) st4(d, dk[m]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (k + r < p.dk) st1(d + r, dk[m][r]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < NJ; ++m) {
+                const int j = operand_index(16 * (j0 + m) + l16);
+                if (j < nr) {
+                    bf16 *d = DVp + j * ldv + v;
+                    if (VEC) {
+                        if (v < p.dv) st4(d, dv[m]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (v + r < p.dv) st1(d + r, dv[m][r]);
+                    }
+                }
+            }
+        }
+        DQ -= C * ldq; DKp -= C * ldq; DVp -= C * ldv;
+        {   // D
+            const int lane = fresh(lane0), gq = lane >> 4;
+            if (NB == 1 && c > c0) fetch(c - 1);
+            scan(c - 1);
+            fetch_g(c - 2);
+            bf16x8 ow[2][3];
+#pragma unroll
+            for (int is = 0; is < 2; ++is) {
+                f4 x, y;
+                widen8(frag_t(Os, VP, vt, is, lane), x, y);
+                split8<3>(x * *reinterpret_cast<const f4 *>(eb + 32 * is + 4 * gq), y * *reinterpret_cast<const f4 *>(eb + 32 * is + 16 + 4 * gq), ow[is]);
+            }
+#pragma unroll
+            for (int t = 0; t < TW; ++t) {
+                D[t] *= eend;
+#pragma unroll
+                for (int is = 0; is < 2; ++is) {
+                    const bf16x8 qf = frag_t(Qs, QP, kd + t, is, lane);
+#pragma unroll
+                    for (int u = 0; u < 3; ++u) D[t] = mfma8(qf, ow[is][u], D[t]);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (c0 < c1) finish_dg(c0);
+    if (a.ds0 && p.nseg == 1) {
+        const int col = operand_index(16 * vt + (lane0 & 15));
+        float *d = a.ds0 + nh * sz;
+#pragma unroll
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = 16 * (kd + t) + 4 * (lane0 >> 4) + r;
+                if (col < p.dv && k < p.dk) d[k * p.dv + col] = D[t][r];
+            }
+    }
+}
+
 // dq / dk of the value heads that share a key head, summed: (rows, G, rep, dk) fp32 -> (rows, G, dk)
 template <typename IO>
 __global__ __launch_bounds__(NT) void la_head_sum_kernel(const float *a, const float *b, IO *oa, IO *ob, long long total, int rep, int dk) {
@@ -416,17 +829,45 @@ void launch_bwd(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     else ss2d_launch((la_bwd_kernel<DK, DV, C, IO, IO>), dim3(walks + gaps), dim3(NT), 0, s, a);
 }
 
-template <typename IO>
-void dispatch_bwd(const BwdArgs &a, unsigned gaps, hipStream_t s) {
+void dispatch_bwd_f32(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     const int dk = a.p.dk, dv = a.p.dv;
     if (dv <= 64) {
-        if (dk <= 16) launch_bwd<16, 64, 64, IO>(a, gaps, s);
-        else if (dk <= 64) launch_bwd<64, 64, 64, IO>(a, gaps, s);
-        else launch_bwd<128, 64, 32, IO>(a, gaps, s);
+        if (dk <= 16) launch_bwd<16, 64, 64, float>(a, gaps, s);
+        else if (dk <= 64) launch_bwd<64, 64, 64, float>(a, gaps, s);
+        else launch_bwd<128, 64, 32, float>(a, gaps, s);
     } else {
-        if (dk <= 16) launch_bwd<16, 128, 32, IO>(a, gaps, s);
-        else if (dk <= 64) launch_bwd<64, 128, 32, IO>(a, gaps, s);
-        else launch_bwd<128, 128, 32, IO>(a, gaps, s);
+        if (dk <= 16) launch_bwd<16, 128, 32, float>(a, gaps, s);
+        else if (dk <= 64) launch_bwd<64, 128, 32, float>(a, gaps, s);
+        else launch_bwd<128, 128, 32, float>(a, gaps, s);
+    }
+}
+
+template <int DK, int DV, bool VEC>
+void launch_bwd_bf16(const BwdArgs &a, unsigned gaps, hipStream_t s) {
+    const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg);
+    if (a.p.H > a.p.G) ss2d_launch((la_bwd_bf16_kernel<DK, DV, VEC, float>), dim3(walks + gaps), dim3(512), 0, s, a);
+    else ss2d_launch((la_bwd_bf16_kernel<DK, DV, VEC, bf16>), dim3(walks + gaps), dim3(512), 0, s, a);
+}
+template <bool VEC>
+void dispatch_bwd_bf16(const BwdArgs &a, unsigned gaps, hipStream_t s) {
+    const Problem &p = a.p;
+    if (p.nseg > 1) {
+        Problem r = p;                            // q in the place of k, dout in that of v
+        r.k = p.q; r.kb = p.qb; r.kl = p.ql; r.kh = p.qh;
+        r.v = a.dout; r.vb = p.tokens * p.H * p.dv; r.vl = (long long)p.H * p.dv; r.vh = p.dv;
+        linattn_segment_pass_bf16(r, a.seg_states, a.seg_decay, a.ds0, true, s);
+        const long long sz = (long long)p.dk * p.dv;
+        ss2d_launch(la_join_bwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(p.N * p.H)), dim3(NT), 0, s, a, 64);
+    }
+    const int dk = p.dk;
+    if (p.dv <= 64) {
+        if (dk <= 32) launch_bwd_bf16<32, 64, VEC>(a, gaps, s);
+        else if (dk <= 64) launch_bwd_bf16<64, 64, VEC>(a, gaps, s);
+        else launch_bwd_bf16<128, 64, VEC>(a, gaps, s);
+    } else {
+        if (dk <= 32) launch_bwd_bf16<32, 128, VEC>(a, gaps, s);
+        else if (dk <= 64) launch_bwd_bf16<64, 128, VEC>(a, gaps, s);
+        else launch_bwd_bf16<128, 128, VEC>(a, gaps, s);
     }
 }
 
@@ -448,7 +889,10 @@ extern "C" int ss2d_linattn_bwd(int dtype, const void *q, const void *k, const v
     a.p.vec = a.p.vec && (uintptr_t)dout % 16 == 0;
     const unsigned gaps = cu_seqlens ? GAP_WGS : 0;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == SS2D_DTYPE_BF16) dispatch_bwd<bf16>(a, gaps, s); else dispatch_bwd<float>(a, gaps, s);
+    a.p.vec = a.p.vec && (long long)H * dv < (1 << 23);
+    if (dtype == SS2D_DTYPE_F32) dispatch_bwd_f32(a, gaps, s);
+    else if (a.p.vec) dispatch_bwd_bf16<true>(a, gaps, s);
+    else dispatch_bwd_bf16<false>(a, gaps, s);
     if (H > G) {
         const long long rows = (cu_seqlens ? 1 : N) * tokens, total = rows * G * dk;
         const dim3 grid((unsigned)((total + NT - 1) / NT), 2);

@@ -36,7 +36,8 @@ __device__ void zero_gaps(const Problem &p, IO *o, long long row, int w) {
     for (long long e = hi * row + (long long)w * NT + threadIdx.x; e < p.tokens * row; e += step) st1(o + e, 0.0f);
 }
 
-// mode 0: the whole walk; mode 1: only a segment's own contribution to the state
+// mode 0: the whole walk; mode 1: only a segment's own contribution to the state; (bf16) mode 2: the backward's, sum of scale exp(b) q dout^T from the
+// segment's end, with q in the place of k and dout in that of v
 template <int DK, int C, int MODE, typename IO>
 __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     constexpr int PK = DK + 4, PV = 64 + 4, PP = C + 4, KT = DK / 16, CT = C / 16;
@@ -96,15 +97,15 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
         load_tile<C, DK, PK, NT>(Ks, K + r0 * p.kl, p.kl, nr, p.dk, p.vec);
         load_tile<C, 64, PV, NT>(Vs, V + r0 * p.vl, p.vl, nr, p.dv - 64 * vt, p.vec);
         const float gv = lane < nr ? limit_decay(g[(r0 + lane) * p.gl]) : 0.0f;
-        const double b = chunk_decay_scan(gv, lane), bend = __shfl(b, 63, 64);
+        const double b = chunk_decay_scan(gv), bend = lane63(b);
         total += bend;
-        const float eend = exp2f((float)bend);
+        const float eend = hw_exp2((float)bend);
         if (wave == 0) {
             const float hi = (float)b;
             bh[lane] = hi;
             bl[lane] = (float)(b - hi);
-            eb[lane] = exp2f(hi) * p.scale;
-            wt[lane] = exp2f((float)(bend - b));
+            eb[lane] = hw_exp2(hi) * p.scale;
+            wt[lane] = hw_exp2((float)(bend - b));
         }
         __syncthreads();
         if (MODE == 0) {
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = 16 * it + 4 * gq + r;
-                    Ps[i * PP + j] = j <= i ? acc[r] * p.scale * exp2f((bh[i] - hj) + (bl[i] - lj)) : 0.0f;
+                    Ps[i * PP + j] = j <= i ? acc[r] * p.scale * hw_exp2((bh[i] - hj) + (bl[i] - lj)) : 0.0f;
                 }
             }
             __syncthreads();
@@ -181,6 +182,212 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     }
 }
 
+// The same walk for bf16 tensors on the bf16 matrix instruction; a workgroup owns all of dv (a wave 16 columns: NW = 4 or 8 waves), the next chunk is in
+// flight in registers during the products.  Per chunk: P (two-term weights, to LDS), then for all rows i  O^T = S^T Q^T (S in two terms), scaled by
+// exp(b_i), plus V^T P^T, then S += K^T (exp(b_C - b_j) V) with the weighted V in three terms: the state keeps 24 bits.
+// LDS rows are an odd number of 32-byte pieces long: 16-byte direct reads (4 cycles) and transposed ones (2) are then free of bank conflicts (measured
+// over pitches of 128 ... 320 bytes); q and P lie in operand order, so a lane's eight values are one read.
+template <int DK, int NW, int MODE, bool VEC>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fwd_bf16_kernel(const FwdArgs a) {
+    constexpr int NT = 64 * NW, C = 64, DV = 16 * NW, KT = DK / 16, KS = DK / 32, QP = 2 * DK + 32, KP = 2 * DK + 32, VP = 2 * DV + 32, PP = 2 * C + 32;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[C * (KP + VP) + (MODE == 0 ? C * (QP + 2 * PP) : 0) + 10 * C * 4];
+    unsigned char *Ks = lds, *Vs = Ks + C * KP, *Qs = Vs + C * VP, *Ph = Qs + C * QP, *Pl = Ph + C * PP;
+    float *decays = reinterpret_cast<float *>(MODE == 0 ? Pl + C * PP : Qs);     // two chunks of: b (two terms), scale exp(b), exp(b_C - b), exp(b_C)
+    const Problem &p = a.p;
+    const int tid = threadIdx.x, lane0 = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int walks = p.N * p.H * p.nseg;
+    if ((int)blockIdx.x >= walks) {              // packed rows that belong to no sequence: their output is zero
+        if (MODE == 0) zero_gaps(p, static_cast<bf16 *>(a.o), (long long)p.H * p.dv, blockIdx.x - walks);
+        return;
+    }
+    int id = xcd_remap(blockIdx.x, walks);       // heads of a group run next to each other on one XCD: they read the same q and k
+    const int h = id % p.H; id /= p.H;
+    const int seg = id % p.nseg, n = id / p.nseg;
+    const Seq s = get_seq(p, n);
+    const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
+    const int c1 = segment_end(p, seg, nch);
+    const bool empty = s.len == 0;
+    if (c0 >= c1 && !(empty && seg == 0)) return;
+    if (MODE == 1 && c1 == nch && !empty && !a.last) return;     // nothing starts from the last segment's end
+    if (MODE == 2 && c0 == 0 && !a.last) return;                 // (here: the gradient in front of the first segment is not wanted)
+    const int hk = h / (p.H / p.G), first = MODE == 2 ? c1 - 1 : c0;
+    const bf16 *Q = static_cast<const bf16 *>(p.q) + s.row * p.qb + (s.start + (long long)c0 * C) * p.ql + hk * p.qh;
+    const bf16 *K = static_cast<const bf16 *>(p.k) + s.row * p.kb + (s.start + (long long)first * C) * p.kl + hk * p.kh;
+    const bf16 *V = static_cast<const bf16 *>(p.v) + s.row * p.vb + (s.start + (long long)first * C) * p.vl + h * p.vh;
+    const float *g = p.g + s.row * p.gb + s.start * p.gl + h * p.gh;
+    const long long ldo = (long long)p.H * p.dv, nh = (long long)n * p.H + h, sz = (long long)p.dk * p.dv;
+    bf16 *O = static_cast<bf16 *>(a.o) + ((s.row * p.tokens + s.start + (long long)c0 * C) * p.H + h) * (long long)p.dv;
+    const int col = 16 * wave + (lane0 & 15);
+    f4 S[KT];
+    const float *init = MODE >= 1 ? nullptr : p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int k = 16 * t + 4 * (lane0 >> 4) + r;
+            S[t][r] = init && col < p.dv && k < p.dk ? init[k * p.dv + col] : 0.0f;
+        }
+    double total = 0.0;
+    f4 *saved = MODE == 0 && a.chunk_states ? reinterpret_cast<f4 *>(a.chunk_states) + ((chunk_base(p, s, n, C) + c0) * p.H + h) * (DK * DV / 4) + wave * KT * 64 + lane0 : nullptr;
+    TileRegs<C, DK, NT, VEC> qr, kr;
+    TileRegs<C, DV, NT, VEC> vr;
+    qr.init(p.ql, p.dk);
+    kr.init(p.kl, p.dk);
+    vr.init(p.vl, p.dv);
+    auto rows_of = [&](int c) { const int left = s.len - c * C; return left < C ? left : C; };
+    auto fetch = [&](int c) {                    // chunk c, the tensors' pointers at chunk c
+        const int nr = rows_of(c);
+        if (MODE == 0) qr.load(Q, p.ql, nr);
+        kr.load(K, p.kl, nr);
+        vr.load(V, p.vl, nr);
+    };
+    float gr = 0.0f;                             // wave 0: decays, a chunk ahead of the tiles
+    auto fetch_g = [&](int c) {
+        if (wave == 0 && c >= c0 && c < c1) gr = lane0 < rows_of(c) ? limit_decay(g[((long long)c * C + lane0) * p.gl]) : 0.0f;
+    };
+    auto scan = [&](int c) {
+        if (wave == 0 && c >= c0 && c < c1) {
+            float *d = decays + (c & 1) * 5 * C;
+            const double b = chunk_decay_scan(gr), bend = lane63(b);
+            const float hi = (float)b;
+            if (MODE >= 1) total += bend;
+            d[lane0] = hi;
+            d[C + lane0] = (float)(b - hi);
+            d[2 * C + lane0] = hw_exp2(hi) * p.scale;
+            d[3 * C + lane0] = hw_exp2((float)(bend - b));
+            if (lane0 == 63) d[4 * C] = hw_exp2((float)bend);
+        }
+    };
+    constexpr int STEP = MODE == 2 ? -1 : 1;
+    fetch_g(first);
+    scan(first);
+    fetch_g(first + STEP);
+    if (c0 < c1) fetch(first);
+#pragma unroll 1
+    for (int c = first; c >= c0 && c < c1; c += STEP) {
+        const int nr = rows_of(c);
+        if (MODE == 0 && saved) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) saved[64 * t] = S[t];
+            saved += (long long)p.H * (DK * DV / 4);
+        }
+        __syncthreads();
+        if (MODE == 0) qr.template put<true>(Qs, QP, Q, p.ql, nr, p.dk);
+        kr.put(Ks, KP, K, p.kl, nr, p.dk);
+        vr.put(Vs, VP, V, p.vl, nr, p.dv);
+        Q += C * p.ql; K += STEP * C * p.kl; V += STEP * C * p.vl;
+        if (MODE >= 1 && c + STEP >= c0 && c + STEP < c1) fetch(c + STEP);
+        const float *bh = decays + (c & 1) * 5 * C, *bl = bh + C, *eb = bl + C, *wt = eb + C, *tail = wt + C;
+        __syncthreads();
+        if (MODE == 0) {
+            // P[i][j] = scale exp(b_i - b_j) q_i . k_j, j <= i: four waves take a row tile each; eight take the even and the odd column tiles of one.  The
+            // tile behind the diagonal of an even row tile is zero: P is read 32 columns at a time
+            const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
+            const int it = NW == 8 ? wave >> 1 : wave, i = 16 * it + l16;
+            bf16x8 qf[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) qf[ks] = frag_p(Qs, QP, i, ks, gq);
+            const float hi = bh[i], li = bl[i];
+#pragma unroll 1
+            for (int jt = NW == 8 ? wave & 1 : 0; jt <= (it | 1); jt += NW == 8 ? 2 : 1) {
+                f4 acc = f4{0, 0, 0, 0};
+                if (jt <= it) {
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) acc = mfma8(frag(Ks, KP, 16 * jt + l16, ks, gq), qf[ks], acc);
+                    const f4 h4 = *reinterpret_cast<const f4 *>(bh + 16 * jt + 4 * gq), l4 = *reinterpret_cast<const f4 *>(bl + 16 * jt + 4 * gq);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        acc[r] = 16 * jt + 4 * gq + r <= i ? acc[r] * p.scale * hw_exp2((hi - h4[r]) + (li - l4[r])) : 0.0f;
+                }
+                const bf16x4 x = round4(acc);
+                const int at = i * PP + 2 * operand_pos(16 * jt + 4 * gq);
+                *reinterpret_cast<bf16x4 *>(Ph + at) = x;
+                *reinterpret_cast<bf16x4 *>(Pl + at) = round4(rest4(acc, x));
+            }
+            __syncthreads();
+        }
+        const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
+        bf16x8 vf[2];
+#pragma unroll
+        for (int js = 0; js < 2; ++js) vf[js] = frag_t(Vs, VP, wave, js, lane);
+        if (MODE == 0) {
+            f4 acc[4];
+#pragma unroll
+            for (int it = 0; it < 4; ++it) acc[it] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                bf16x8 sf[2];
+                split8<2>(S[2 * ks], S[2 * ks + 1], sf);
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const bf16x8 q = frag_p(Qs, QP, 16 * it + l16, ks, gq);
+                    acc[it] = mfma8(sf[0], q, acc[it]);
+                    acc[it] = mfma8(sf[1], q, acc[it]);
+                }
+                if (NW == 8) __builtin_amdgcn_sched_barrier(0);
+            }
+            const int oc = 16 * wave + 4 * gq;
+            bf16 *o = O + l16 * ldo + oc;
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                acc[it] *= eb[16 * it + l16];
+#pragma unroll
+                for (int js = 0; js <= it / 2; ++js) {
+                    acc[it] = mfma8(vf[js], frag_p(Ph, PP, 16 * it + l16, js, gq), acc[it]);
+                    acc[it] = mfma8(vf[js], frag_p(Pl, PP, 16 * it + l16, js, gq), acc[it]);
+                }
+                if (16 * it + l16 < nr) {
+                    if (VEC) {
+                        if (oc < p.dv) st4(o, acc[it]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (oc + r < p.dv) st1(o + r, acc[it][r]);
+                    }
+                }
+                o += 16 * ldo;
+            }
+            O += C * ldo;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (MODE == 0 && c + 1 < c1) fetch(c + 1);   // in flight during the state's products; earlier, its registers would cost a workgroup a CU
+        scan(c + STEP);
+        fetch_g(c + 2 * STEP);
+        const float eend = tail[0];
+        bf16x8 vw[2][3];
+#pragma unroll
+        for (int js = 0; js < 2; ++js) {
+            const float *w = MODE == 2 ? eb : wt;
+            const f4 w0 = *reinterpret_cast<const f4 *>(w + 32 * js + 4 * gq), w1 = *reinterpret_cast<const f4 *>(w + 32 * js + 16 + 4 * gq);
+            f4 x, y;
+            widen8(vf[js], x, y);
+            split8<3>(x * w0, y * w1, vw[js]);
+        }
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            S[t] *= eend;
+#pragma unroll
+            for (int js = 0; js < 2; ++js) {
+                const bf16x8 k = frag_t(Ks, KP, t, js, lane);
+#pragma unroll
+                for (int u = 0; u < 3; ++u) S[t] = mfma8(k, vw[js][u], S[t]);
+            }
+        }
+    }
+    float *dst = MODE >= 1 ? a.seg_states + (nh * p.nseg + seg) * sz : (a.last && p.nseg == 1) ? a.last + nh * sz : nullptr;
+    if (dst) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = 16 * t + 4 * (lane0 >> 4) + r;
+                if (col < p.dv && k < p.dk) dst[k * p.dv + col] = S[t][r];
+            }
+        if (MODE >= 1 && tid == 0) a.seg_decay[nh * p.nseg + seg] = total;
+    }
+}
+
 // joins the segments of a (sequence, head): seg_states[s] = state in front of segment s; one thread per state element
 __global__ __launch_bounds__(NT) void la_join_fwd_kernel(const FwdArgs a, int C) {
     const Problem &p = a.p;
@@ -191,12 +398,23 @@ __global__ __launch_bounds__(NT) void la_join_fwd_kernel(const FwdArgs a, int C)
     const Seq s = get_seq(p, (int)(nh / p.H));
     const int nch = (s.len + C - 1) / C, ns = segments_of(p, nch);
     float v = a.s0 ? a.s0[nh * sz + e] : 0.0f;
-    for (int i = 0; i < ns; ++i) {
-        float *u = a.seg_states + (nh * p.nseg + i) * sz + e;
-        if (i + 1 == ns && !a.last) { *u = v; break; }
-        const float own = *u;
-        *u = v;
-        v = v * exp2f((float)a.seg_decay[nh * p.nseg + i]) + own;
+    float *u = a.seg_states + nh * p.nseg * sz + e;
+    const double *d = a.seg_decay + nh * p.nseg;
+    for (int i = 0; i < ns; i += 8) {                       // eight segments' loads are in flight at once
+        float own[8], f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = i + j < ns ? i + j : ns - 1;      // (without `last` the last segment's contribution is not there, and not used)
+            own[j] = u[k * sz];
+            f[j] = hw_exp2((float)d[k]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (i + j < ns) {
+                u[(i + j) * sz] = v;
+                v = v * f[j] + own[j];
+            }
+        }
     }
     if (a.last) a.last[nh * sz + e] = v;
 }
@@ -213,20 +431,68 @@ void launch_fwd(const FwdArgs &a, unsigned gaps, hipStream_t s) {
     ss2d_launch((la_fwd_kernel<DK, C, 0, IO>), dim3(grid + gaps), dim3(NT), 0, s, a);
 }
 
-template <typename IO>
-void dispatch_fwd(const FwdArgs &a, unsigned gaps, hipStream_t s) {
+void dispatch_fwd_f32(const FwdArgs &a, unsigned gaps, hipStream_t s) {
     const int dk = a.p.dk;
-    const bool c64 = linattn_chunk(a.p.dk, a.p.dv) == 64;
-    if (dk <= 16) c64 ? launch_fwd<16, 64, IO>(a, gaps, s) : launch_fwd<16, 32, IO>(a, gaps, s);
-    else if (dk <= 64) c64 ? launch_fwd<64, 64, IO>(a, gaps, s) : launch_fwd<64, 32, IO>(a, gaps, s);
-    else launch_fwd<128, 32, IO>(a, gaps, s);
+    const bool c64 = linattn_chunk(SS2D_DTYPE_F32, a.p.dk, a.p.dv) == 64;
+    if (dk <= 16) c64 ? launch_fwd<16, 64, float>(a, gaps, s) : launch_fwd<16, 32, float>(a, gaps, s);
+    else if (dk <= 64) c64 ? launch_fwd<64, 64, float>(a, gaps, s) : launch_fwd<64, 32, float>(a, gaps, s);
+    else launch_fwd<128, 32, float>(a, gaps, s);
+}
+
+template <int DK, int NW, bool VEC>
+void launch_fwd_bf16(const FwdArgs &a, unsigned gaps, hipStream_t s) {
+    const Problem &p = a.p;
+    const unsigned walks = (unsigned)((long long)p.N * p.H * p.nseg);
+    if (p.nseg > 1) {
+        linattn_segment_pass_bf16(p, a.seg_states, a.seg_decay, a.last, false, s);
+        const long long sz = (long long)p.dk * p.dv;
+        ss2d_launch(la_join_fwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(p.N * p.H)), dim3(NT), 0, s, a, 64);
+    }
+    ss2d_launch((la_fwd_bf16_kernel<DK, NW, 0, VEC>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
+}
+template <bool VEC>
+void dispatch_fwd_bf16(const FwdArgs &a, unsigned gaps, hipStream_t s) {
+    const int dk = a.p.dk;
+    if (a.p.dv <= 64) {
+        if (dk <= 32) launch_fwd_bf16<32, 4, VEC>(a, gaps, s);
+        else if (dk <= 64) launch_fwd_bf16<64, 4, VEC>(a, gaps, s);
+        else launch_fwd_bf16<128, 4, VEC>(a, gaps, s);
+    } else {
+        if (dk <= 32) launch_fwd_bf16<32, 8, VEC>(a, gaps, s);
+        else if (dk <= 64) launch_fwd_bf16<64, 8, VEC>(a, gaps, s);
+        else launch_fwd_bf16<128, 8, VEC>(a, gaps, s);
+    }
+}
+
+template <int MODE, bool VEC>
+void segment_pass(const FwdArgs &a, hipStream_t s) {
+    const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg);
+    const int dk = a.p.dk;
+    if (a.p.dv <= 64) {
+        if (dk <= 32) ss2d_launch((la_fwd_bf16_kernel<32, 4, MODE, VEC>), dim3(walks), dim3(256), 0, s, a);
+        else if (dk <= 64) ss2d_launch((la_fwd_bf16_kernel<64, 4, MODE, VEC>), dim3(walks), dim3(256), 0, s, a);
+        else ss2d_launch((la_fwd_bf16_kernel<128, 4, MODE, VEC>), dim3(walks), dim3(256), 0, s, a);
+    } else {
+        if (dk <= 32) ss2d_launch((la_fwd_bf16_kernel<32, 8, MODE, VEC>), dim3(walks), dim3(512), 0, s, a);
+        else if (dk <= 64) ss2d_launch((la_fwd_bf16_kernel<64, 8, MODE, VEC>), dim3(walks), dim3(512), 0, s, a);
+        else ss2d_launch((la_fwd_bf16_kernel<128, 8, MODE, VEC>), dim3(walks), dim3(512), 0, s, a);
+    }
 }
 
 }  // namespace
 
-extern "C" int ss2d_linattn_chunk(int dk, int dv) { return linattn_chunk(dk, dv); }
-extern "C" int ss2d_linattn_segment_chunks(int N, long long max_len, int H, int dk, int dv, int backward) {
-    return N > 0 && max_len >= 0 && H > 0 ? linattn_segment_chunks(N, max_len, H, dk, dv, backward) : 1;
+void linattn_segment_pass_bf16(const linattn::Problem &p, float *seg_states, double *seg_decay, const float *want_end, bool reverse, hipStream_t s) {
+    FwdArgs a{};
+    a.p = p; a.seg_states = seg_states; a.seg_decay = seg_decay;
+    a.last = const_cast<float *>(want_end);      // only asked for being there
+    if (reverse) p.vec ? segment_pass<2, true>(a, s) : segment_pass<2, false>(a, s);
+    else p.vec ? segment_pass<1, true>(a, s) : segment_pass<1, false>(a, s);
+}
+
+extern "C" int ss2d_linattn_chunk(int dtype, int dk, int dv) { return linattn_chunk(dtype, dk, dv); }
+extern "C" long long ss2d_linattn_state_floats(int dtype, int dk, int dv) { return linattn_state_floats(dtype, dk, dv); }
+extern "C" int ss2d_linattn_segment_chunks(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
+    return all_tokens >= 0 && max_len >= 0 && H > 0 ? linattn_segment_chunks(dtype, all_tokens, max_len, H, dk, dv, backward) : 1;
 }
 
 extern "C" int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const void *v, const float *g, const long long *strides,
@@ -240,7 +506,9 @@ extern "C" int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const v
     if (nseg > 1 && (!seg_states || !seg_decay)) { ss2d_set_error("linattn_fwd: segments without a workspace"); return -2; }
     a.o = out; a.s0 = s0; a.last = last; a.chunk_states = chunk_states; a.seg_states = seg_states; a.seg_decay = seg_decay;
     const unsigned gaps = cu_seqlens ? GAP_WGS : 0;
-    if (dtype == SS2D_DTYPE_BF16) dispatch_fwd<bf16>(a, gaps, (hipStream_t)stream); else dispatch_fwd<float>(a, gaps, (hipStream_t)stream);
+    if (dtype == SS2D_DTYPE_F32) dispatch_fwd_f32(a, gaps, (hipStream_t)stream);
+    else if (a.p.vec) dispatch_fwd_bf16<true>(a, gaps, (hipStream_t)stream);
+    else dispatch_fwd_bf16<false>(a, gaps, (hipStream_t)stream);
     rc = ss2d_take_launch_rc();
     if (rc) ss2d_set_error("linattn_fwd: launch failed: %s", hipGetErrorString((hipError_t)rc));
     return rc;

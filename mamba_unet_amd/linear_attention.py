@@ -67,10 +67,10 @@ def _strides(q, k, v, g):
     return (ctypes.c_longlong * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *gs)
 
 
-def _segments(lib, dev, N, H, longest, dk, dv, backward):
+def _segments(lib, dev, code, N, tokens, H, longest, dk, dv, backward):
     """(segments, chunks a segment, state scratch, decay scratch)"""
-    C = lib.ss2d_linattn_chunk(dk, dv)
-    segc = lib.ss2d_linattn_segment_chunks(N, longest, H, dk, dv, backward)
+    C = lib.ss2d_linattn_chunk(code, dk, dv)
+    segc = lib.ss2d_linattn_segment_chunks(code, tokens, longest, H, dk, dv, backward)
     nseg = max(1, -(-(-(-longest // C)) // segc))
     if nseg == 1:
         return 1, segc, None, None
@@ -89,15 +89,16 @@ def _forward(q, k, v, g, s0, cu, scale, dims, longest, want_last, want_chunks):
             last.zero_() if s0 is None else last.copy_(s0)
         return out, last, None
     lib = _lib.load()
+    code = _BF16 if io == torch.bfloat16 else _F32
     chunks = None
     if want_chunks:
-        C = lib.ss2d_linattn_chunk(dk, dv)
+        C = lib.ss2d_linattn_chunk(code, dk, dv)
         slots = N * -(-L // C) if cu is None else L // C + N
-        chunks = torch.empty((slots, H, dk, dv), device=dev, dtype=torch.float32)
-    nseg, segc, ws, wd = _segments(lib, dev, N, H, longest, dk, dv, 0)
+        chunks = torch.empty((slots, H, lib.ss2d_linattn_state_floats(code, dk, dv)), device=dev, dtype=torch.float32)
+    nseg, segc, ws, wd = _segments(lib, dev, code, N, B * L, H, longest, dk, dv, 0)
     p = _lib.ptr
     with _lib.on_device(dev):
-        rc = lib.ss2d_linattn_fwd(_BF16 if io == torch.bfloat16 else _F32, p(q), p(k), p(v), p(g), _strides(q, k, v, g), p(cu), p(s0), p(out), p(last),
+        rc = lib.ss2d_linattn_fwd(code, p(q), p(k), p(v), p(g), _strides(q, k, v, g), p(cu), p(s0), p(out), p(last),
                                   p(chunks), p(ws), p(wd), N, L, H, G, dk, dv, scale, nseg, segc, _lib.stream())
     _lib.check(rc, "ss2d_linattn_fwd")
     return out, last, chunks
@@ -139,10 +140,11 @@ class LinearAttentionFn(torch.autograd.Function):
         ds0 = torch.empty((N, H, dk, dv), device=dev, dtype=torch.float32) if want_s0 else None
         heads = [torch.empty((B, L, H, dk), device=dev, dtype=torch.float32) for _ in range(2)] if H > G else (None, None)
         lib = _lib.load()
-        nseg, segc, ws, wd = _segments(lib, dev, N, H, longest, dk, dv, 1)
+        code = _BF16 if io == torch.bfloat16 else _F32
+        nseg, segc, ws, wd = _segments(lib, dev, code, N, B * L, H, longest, dk, dv, 1)
         p = _lib.ptr
         with _lib.on_device(dev):
-            rc = lib.ss2d_linattn_bwd(_BF16 if io == torch.bfloat16 else _F32, p(q), p(k), p(v), p(g), _strides(q, k, v, g), p(cu), p(go), p(gl), p(chunks),
+            rc = lib.ss2d_linattn_bwd(code, p(q), p(k), p(v), p(g), _strides(q, k, v, g), p(cu), p(go), p(gl), p(chunks),
                                       p(dq), p(dk_), p(dv_), p(dg), p(ds0), p(heads[0]), p(heads[1]), p(ws), p(wd), N, L, H, G, dk, dv, scale, nseg,
                                       segc, _lib.stream())
         _lib.check(rc, "ss2d_linattn_bwd")

@@ -403,21 +403,21 @@ __global__ __launch_bounds__(NT) void la_bwd_kernel(const BwdArgs a) {
     }
 }
 
-// The same walk for bf16 tensors on the bf16 matrix instruction: eight waves a workgroup, chunks of 64.  LDS holds the four tiles, X and Y (two terms
+// The same walk for bf16 tensors on the bf16 matrix instruction: chunks of 64, 16 waves a workgroup (dk <= 32: 8).  LDS holds the four tiles, X and Y (two terms
 // each) and the terms of ONE state at a time, transposed (dv x dk): first S (for dq), then D (for dk and dv); with NB = 1 (128 x 128) one
 // term at a time.  States enter with three terms where dg is taken from the product (q . S do, k . D v), with two in dv.
 // Orders: k, v, dout and the columns j of X and Y lie in operand order (one 16-byte read an operand); what is read transposed from such a
 // tile comes in that order too, so the rows of dq and dv and the columns of dk, dv and D are named by operand_index.
-template <int DK, int DV, bool VEC, typename QT>
-__global__ __launch_bounds__(512, 2) void la_bwd_bf16_kernel(const BwdArgs a) {
-    constexpr int NT = 512, C = 64, KT = DK / 16, KS = DK / 32, VT = DV / 16, VS = DV / 32;
+template <int DK, int DV, int NW, bool VEC, typename QT>
+__global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdArgs a) {
+    constexpr int NT = 64 * NW, C = 64, KT = DK / 16, KS = DK / 32, VT = DV / 16, VS = DV / 32;
     constexpr int QP = 2 * DK + 32, VP = 2 * DV + 32, PP = 2 * C + 32, SP = 2 * DK + 16;      // bytes a row
     constexpr int NB = DK == 128 && DV == 128 ? 1 : 3;                                        // terms of a state in LDS at once
-    constexpr int NI = KT / 2, NJ = VT / 2, TW = KT * VT / 8;                                 // tiles of a wave: rows of dq / dk, rows of dv, D
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * C * PP + NB * DV * SP + (10 * C + 8 * C + 8) * 4];
+    constexpr int NI = 4 * KT / NW, NJ = 4 * VT / NW, TW = KT * VT / NW;                               // tiles of a wave: rows of dq / dk, rows of dv, D
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * C * PP + NB * DV * SP + (10 * C + NW * C + NW) * 4];
     unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + C * PP, *Yh = Xl + C * PP,
                   *Yl = Yh + C * PP, *St = Yl + C * PP;
-    float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + 8 * C;
+    float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + NW * C;
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -452,7 +452,7 @@ __global__ __launch_bounds__(512, 2) void la_bwd_bf16_kernel(const BwdArgs a) {
     bf16 *DVp = static_cast<bf16 *>(a.dv_) + ((t0 + e0) * p.H + h) * (long long)p.dv;
     float *DG = a.dg + t0 * p.H + h;
     const int kt = wave % KT, i0 = wave / KT * NI;                   // dq / dk: column tile, first row tile
-    const int vt = wave % VT, j0 = wave / VT * NJ, kd = VT == 8 ? 0 : wave / VT * TW;           // dv: column tile, first row tile; D: first row tile
+    const int vt = wave % VT, j0 = wave / VT * NJ, kd = wave / VT * TW;           // dv: column tile, first row tile; D: first row tile
     f4 D[TW];
     {
         const int col = operand_index(16 * vt + (lane0 & 15));
@@ -505,7 +505,7 @@ __global__ __launch_bounds__(512, 2) void la_bwd_bf16_kernel(const BwdArgs a) {
         if (wave == 1) {
             double x = 0.0, e = 0.0;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) { x += (double)parts[w * C + lane0]; e += (double)corners[w]; }
+            for (int w = 0; w < NW; ++w) { x += (double)parts[w * C + lane0]; e += (double)corners[w]; }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_down(x, d, 64);
@@ -550,9 +550,9 @@ __global__ __launch_bounds__(512, 2) void la_bwd_bf16_kernel(const BwdArgs a) {
         put_terms(sr, 0, true);
         __syncthreads();
         parts[wave * C + lane0] = 0.0f;
-        {   // X, Y and the sums of M below the diagonal (the even and the odd column tiles of a row tile are two waves')
+        {   // X, Y and the sums of M below the diagonal (the column tiles of a row tile are dealt to NW / 4 waves)
             const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
-            const int it = wave >> 1, i = 16 * it + l16;
+            const int it = wave / (NW / 4), i = 16 * it + l16;
             bf16x8 qf[KS], of[VS];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) qf[ks] = frag(Qs, QP, i, ks, gq);
@@ -561,7 +561,7 @@ __global__ __launch_bounds__(512, 2) void la_bwd_bf16_kernel(const BwdArgs a) {
             const float hi = bh[i], li = bl[i];
             float rowsum = 0.0f;
 #pragma unroll 1
-            for (int jt = wave & 1; jt <= (it | 1); jt += 2) {
+            for (int jt = wave % (NW / 4); jt <= (it | 1); jt += NW / 4) {
                 f4 x = f4{0, 0, 0, 0}, y = f4{0, 0, 0, 0};
                 if (jt <= it) {
 #pragma unroll
@@ -804,16 +804,31 @@ __global__ __launch_bounds__(512, 2) void la_bwd_bf16_kernel(const BwdArgs a) {
     }
 }
 
-// dq / dk of the value heads that share a key head, summed: (rows, G, rep, dk) fp32 -> (rows, G, dk)
-template <typename IO>
+// dq / dk of the value heads that share a key head, summed in order: (rows, G, rep, dk) fp32 -> (rows, G, dk).  W columns a thread
+template <int W, typename IO>
 __global__ __launch_bounds__(NT) void la_head_sum_kernel(const float *a, const float *b, IO *oa, IO *ob, long long total, int rep, int dk) {
-    const long long e = (long long)blockIdx.x * NT + threadIdx.x;
+    const long long e = ((long long)blockIdx.x * NT + threadIdx.x) * W;
     if (e >= total) return;
     const long long rg = e / dk;
     const float *src = (blockIdx.y ? b : a) + rg * rep * dk + (e - rg * dk);
-    float v = src[0];
-    for (int i = 1; i < rep; ++i) v += src[(long long)i * dk];
-    st1((blockIdx.y ? ob : oa) + e, v);
+    IO *dst = (blockIdx.y ? ob : oa) + e;
+    if (W == 4) {
+        f4 v = ld4(src);
+#pragma unroll 4
+        for (int i = 1; i < rep; ++i) v += ld4(src + (long long)i * dk);
+        st4(dst, v);
+    } else {
+        float v = src[0];
+        for (int i = 1; i < rep; ++i) v += src[(long long)i * dk];
+        st1(dst, v);
+    }
+}
+template <typename IO>
+void launch_head_sum(const float *a, const float *b, void *oa, void *ob, long long total, int rep, int dk, hipStream_t s) {
+    const int w = dk % 4 == 0 ? 4 : 1;
+    const dim3 grid((unsigned)((total / w + NT - 1) / NT), 2);
+    if (w == 4) ss2d_launch((la_head_sum_kernel<4, IO>), grid, dim3(NT), 0, s, a, b, static_cast<IO *>(oa), static_cast<IO *>(ob), total, rep, dk);
+    else ss2d_launch((la_head_sum_kernel<1, IO>), grid, dim3(NT), 0, s, a, b, static_cast<IO *>(oa), static_cast<IO *>(ob), total, rep, dk);
 }
 
 template <int DK, int DV, int C, typename IO>
@@ -845,8 +860,9 @@ void dispatch_bwd_f32(const BwdArgs &a, unsigned gaps, hipStream_t s) {
 template <int DK, int DV, bool VEC>
 void launch_bwd_bf16(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg);
-    if (a.p.H > a.p.G) ss2d_launch((la_bwd_bf16_kernel<DK, DV, VEC, float>), dim3(walks + gaps), dim3(512), 0, s, a);
-    else ss2d_launch((la_bwd_bf16_kernel<DK, DV, VEC, bf16>), dim3(walks + gaps), dim3(512), 0, s, a);
+    constexpr int NW = DK <= 32 ? 8 : 16;
+    if (a.p.H > a.p.G) ss2d_launch((la_bwd_bf16_kernel<DK, DV, NW, VEC, float>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
+    else ss2d_launch((la_bwd_bf16_kernel<DK, DV, NW, VEC, bf16>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
 }
 template <bool VEC>
 void dispatch_bwd_bf16(const BwdArgs &a, unsigned gaps, hipStream_t s) {
@@ -895,9 +911,8 @@ extern "C" int ss2d_linattn_bwd(int dtype, const void *q, const void *k, const v
     else dispatch_bwd_bf16<false>(a, gaps, s);
     if (H > G) {
         const long long rows = (cu_seqlens ? 1 : N) * tokens, total = rows * G * dk;
-        const dim3 grid((unsigned)((total + NT - 1) / NT), 2);
-        if (dtype == SS2D_DTYPE_BF16) ss2d_launch((la_head_sum_kernel<bf16>), grid, dim3(NT), 0, s, dq_heads, dk_heads, (bf16 *)dq, (bf16 *)dk_out, total, H / G, dk);
-        else ss2d_launch((la_head_sum_kernel<float>), grid, dim3(NT), 0, s, dq_heads, dk_heads, (float *)dq, (float *)dk_out, total, H / G, dk);
+        if (dtype == SS2D_DTYPE_BF16) launch_head_sum<bf16>(dq_heads, dk_heads, dq, dk_out, total, H / G, dk, s);
+        else launch_head_sum<float>(dq_heads, dk_heads, dq, dk_out, total, H / G, dk, s);
     }
     rc = ss2d_take_launch_rc();
     if (rc) ss2d_set_error("linattn_bwd: launch failed: %s", hipGetErrorString((hipError_t)rc));

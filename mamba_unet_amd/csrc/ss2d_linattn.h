@@ -219,6 +219,43 @@ struct TileRegs {
     }
 };
 
+// the same for fp32 tiles (C x DP, PITCH floats a row): groups of four columns, register-held or element by element
+template <int C, int DP, int PITCH, int NT, bool VEC>
+struct TileRegsF {
+    static constexpr int PR = DP / 4, N = (C * PR + NT - 1) / NT;
+    f4 v[N];
+    int voff;
+    __device__ __forceinline__ void init(long long ld, int D) {
+        const int r = threadIdx.x / PR, c = 4 * (threadIdx.x % PR);
+        voff = c < D && r < C ? (r * (int)ld + c) * 4 : SS2D_BUF_OOR;
+    }
+    __device__ __forceinline__ void load(const float *src, long long ld, int n, int D) {
+        if (VEC) {
+            const __amdgpu_buffer_rsrc_t rs = make_rsrc(src, (unsigned)(n * (int)ld * 4));
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rs, voff, j * (NT / PR) * (int)ld * 4, 0));
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int e = threadIdx.x + j * NT, r = e / PR, c = 4 * (e % PR);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool ok = r < n && r < C && c + i < D;
+                    const float x = src[ok ? (long long)r * ld + c + i : 0];
+                    v[j][i] = ok ? x : 0.0f;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put(float *tile) const {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int e = threadIdx.x + j * NT, r = e / PR, c = 4 * (e % PR);
+            if (C * PR % NT == 0 || r < C) *reinterpret_cast<f4 *>(tile + r * PITCH + c) = v[j];
+        }
+    }
+};
+
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // tokens of a chunk: the backward holds q, k, v, dout, a dk x dv state and two C x C matrices in 160 KB of LDS

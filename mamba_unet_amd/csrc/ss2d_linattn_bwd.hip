@@ -32,14 +32,6 @@ struct BwdArgs {
     double *seg_decay;
 };
 
-template <int TP, typename F>
-__device__ __forceinline__ void each_tile_element(F f) {      // (row, column) of this thread's elements of D: tile t, register r
-#pragma unroll
-    for (int t = 0; t < TP; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) f(t, r);
-}
-
 // sum over the 16 lanes of a DPP row, in every lane of it
 __device__ __forceinline__ float row16_sum(float v) {
     v += dpp_mov<DPP_ROW_ROR(8), 0xf, false>(0.0f, v);
@@ -49,8 +41,8 @@ __device__ __forceinline__ float row16_sum(float v) {
     return v;
 }
 
-// a segment's own contribution to D: sum over its tokens of scale exp(b) q do^T
-template <int DK, int C, typename IO>
+// (fp32) a segment's own contribution to D: sum over its tokens of scale exp(b) q do^T
+template <int DK, int C>
 __global__ __launch_bounds__(NT) void la_bwd_seg_kernel(const BwdArgs a) {
     constexpr int PK = DK + 4, PV = 64 + 4, KT = DK / 16, CT = C / 16;
     __shared__ __attribute__((aligned(16))) float lds[C * PK + C * PV + 64];
@@ -68,9 +60,9 @@ __global__ __launch_bounds__(NT) void la_bwd_seg_kernel(const BwdArgs a) {
     if (c0 >= c1) return;
     const int hk = h / (p.H / p.G), col = 64 * vt + 16 * wave + l16;
     const bool cok = col < p.dv;
-    const IO *Q = static_cast<const IO *>(p.q) + s.row * p.qb + s.start * p.ql + hk * p.qh;
+    const float *Q = static_cast<const float *>(p.q) + s.row * p.qb + s.start * p.ql + hk * p.qh;
     const long long ldo = (long long)p.H * p.dv, nh = (long long)n * p.H + h, sz = (long long)p.dk * p.dv;
-    const IO *DO = static_cast<const IO *>(a.dout) + ((s.row * p.tokens + s.start) * p.H + h) * (long long)p.dv + 64 * vt;
+    const float *DO = static_cast<const float *>(a.dout) + ((s.row * p.tokens + s.start) * p.H + h) * (long long)p.dv + 64 * vt;
     const float *g = p.g + s.row * p.gb + s.start * p.gl + h * p.gh;
     f4 D[KT];
 #pragma unroll
@@ -156,28 +148,33 @@ __device__ void zero_rows(const Problem &p, IO *o, long long row, int w, int nw)
 }
 constexpr int GAP_WGS = 16;
 
-// QT: storage type of dq / dk (fp32 per value head when heads share keys, then summed)
-template <int DK, int DV, int C, typename IO, typename QT>
-__global__ __launch_bounds__(NT) void la_bwd_kernel(const BwdArgs a) {
-    constexpr int PK = DK + 4, PV = DV + 4, PP = C + 4, KT = DK / 16, VT = DV / 16, CT = C / 16;
-    constexpr int VW = (VT + 3) / 4, KW = (KT + 3) / 4;              // tiles of dv / of dk that a wave owns: wave + 4 m
-    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * C * PP + 8 * 64 + 4];
-    float *Qs = lds, *Ks = Qs + C * PK, *Vs = Ks + C * PK, *Os = Vs + C * PV, *Ds = Os + C * PV, *Xs = Ds + DK * PV, *Ys = Xs + C * PP;
-    float *bh = Ys + C * PP, *bl = bh + 64, *eb = bl + 64, *wt = eb + 64, *parts = wt + 64, *corners = parts + 256;
+// fp32: 16 waves a workgroup, so that every result of a chunk -- dq, dk (C x dk) and dv (C x dv) -- is at most one 16 x 16 tile a wave on
+// v_mfma_f32_16x16x4_f32.  A lane holds row / column l16 of an operand and contracted indices 4 gq + r of a 16-block in step r: direct operands are
+// 16-byte LDS reads, transposed ones four 4-byte reads, both free of bank conflicts at a pitch of 4 mod 16 floats.  LDS holds the four tiles, X,
+// Y and one state at a time: S (for dq), then D (for dk, dv).  The next chunk is in flight in registers.
+template <int DK, int DV, int C, bool VEC>
+__global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
+    constexpr int NT = 1024, PK = DK + 4, PV = DV + 4, PP = C + 4, KT = DK / 16, VT = DV / 16, CT = C / 16;
+    constexpr int TW = (KT * VT + 15) / 16;                          // tiles of D a wave owns: wave + 16 m
+    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * C * PP + 10 * 64 + 16 * 64 + 16];
+    float *Qs = lds, *Ks = Qs + C * PK, *Vs = Ks + C * PK, *Os = Vs + C * PV, *St = Os + C * PV, *Xs = St + DK * PV, *Ys = Xs + C * PP;
+    float *decays = Ys + C * PP, *parts = decays + 10 * 64, *corners = parts + 16 * 64;
     const Problem &p = a.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, gq = lane >> 4;
-    int id = blockIdx.x;
-    const int main_wgs = p.N * p.H * p.nseg;
+    const int tid = threadIdx.x, lane0 = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int walks = p.N * p.H * p.nseg;
     const int hq = p.H > p.G ? p.H : p.G;                            // heads of dq / dk as written
-    if (id >= main_wgs) {                                            // packed rows that belong to no sequence
-        zero_rows(p, static_cast<QT *>(a.dq), (long long)hq * p.dk, id - main_wgs, GAP_WGS);
-        zero_rows(p, static_cast<QT *>(a.dk_), (long long)hq * p.dk, id - main_wgs, GAP_WGS);
-        zero_rows(p, static_cast<IO *>(a.dv_), (long long)p.H * p.dv, id - main_wgs, GAP_WGS);
-        zero_rows(p, a.dg, p.H, id - main_wgs, GAP_WGS);
+    if ((int)blockIdx.x >= walks) {                                  // packed rows that belong to no sequence
+        const int w = (int)blockIdx.x - walks;
+        zero_rows(p, static_cast<float *>(a.dq), (long long)hq * p.dk, w, GAP_WGS);
+        zero_rows(p, static_cast<float *>(a.dk_), (long long)hq * p.dk, w, GAP_WGS);
+        zero_rows(p, static_cast<float *>(a.dv_), (long long)p.H * p.dv, w, GAP_WGS);
+        zero_rows(p, a.dg, p.H, w, GAP_WGS);
         return;
     }
-    const int seg = id % p.nseg; id /= p.nseg;
-    const int h = id % p.H, n = id / p.H;
+    int id = xcd_remap(blockIdx.x, walks);
+    const int h = id % p.H; id /= p.H;
+    const int seg = id % p.nseg, n = id / p.nseg;
     const Seq s = get_seq(p, n);
     const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
     const int c1 = segment_end(p, seg, nch);
@@ -185,78 +182,146 @@ __global__ __launch_bounds__(NT) void la_bwd_kernel(const BwdArgs a) {
     if (c0 >= c1 && !(empty && seg == 0)) return;
     const int hk = h / (p.H / p.G);
     const long long ldv = (long long)p.H * p.dv, ldq = (long long)hq * p.dk, nh = (long long)n * p.H + h, sz = (long long)p.dk * p.dv;
-    const IO *Q = static_cast<const IO *>(p.q) + s.row * p.qb + s.start * p.ql + hk * p.qh;
-    const IO *K = static_cast<const IO *>(p.k) + s.row * p.kb + s.start * p.kl + hk * p.kh;
-    const IO *V = static_cast<const IO *>(p.v) + s.row * p.vb + s.start * p.vl + h * p.vh;
-    const long long t0 = s.row * p.tokens + s.start;
-    const IO *DO = static_cast<const IO *>(a.dout) + (t0 * p.H + h) * (long long)p.dv;
+    const long long t0 = s.row * p.tokens + s.start, e0 = (long long)(c1 - 1) * C;              // the tensors' pointers start at the last chunk
+    const float *Q = static_cast<const float *>(p.q) + s.row * p.qb + (s.start + e0) * p.ql + hk * p.qh;
+    const float *K = static_cast<const float *>(p.k) + s.row * p.kb + (s.start + e0) * p.kl + hk * p.kh;
+    const float *V = static_cast<const float *>(p.v) + s.row * p.vb + (s.start + e0) * p.vl + h * p.vh;
+    const float *DO = static_cast<const float *>(a.dout) + ((t0 + e0) * p.H + h) * (long long)p.dv;
     const float *g = p.g + s.row * p.gb + s.start * p.gl + h * p.gh;
-    QT *DQ = static_cast<QT *>(a.dq) + (t0 * hq + h) * (long long)p.dk;
-    QT *DKp = static_cast<QT *>(a.dk_) + (t0 * hq + h) * (long long)p.dk;
-    IO *DVp = static_cast<IO *>(a.dv_) + (t0 * p.H + h) * (long long)p.dv;
+    float *DQ = static_cast<float *>(a.dq) + ((t0 + e0) * hq + h) * (long long)p.dk;
+    float *DKp = static_cast<float *>(a.dk_) + ((t0 + e0) * hq + h) * (long long)p.dk;
+    float *DVp = static_cast<float *>(a.dv_) + ((t0 + e0) * p.H + h) * (long long)p.dv;
     float *DG = a.dg + t0 * p.H + h;
-    f4 D[VW][KT];
-    const float *init = p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
+    // one tile each; the last waves take dq and dk first, the first waves the scores
+    const int wq = 15 - wave, qk = wq % KT, qi = wq / KT, vt = wave % VT, vj = wave / VT;
+    const bool has_q = wq < KT * CT, has_v = wave < VT * CT;
+    auto state_at = [&](int m, int r, int ln) {                      // element (t, r) of this lane's part of a state: row k, column dv; -1: outside
+        const int t = wave + 16 * m, k = 16 * (t / VT) + 4 * (ln >> 4) + r, c = 16 * (t % VT) + (ln & 15);
+        return t < KT * VT && k < p.dk && c < p.dv ? k * p.dv + c : -1;
+    };
+    f4 D[TW], sr[TW];
+    {
+        const float *init = p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
 #pragma unroll
-    for (int m = 0; m < VW; ++m)
-        each_tile_element<KT>([&](int t, int r) {
-            const int k = 16 * t + 4 * gq + r, col = 16 * (wave + 4 * m) + l16;
-            D[m][t][r] = init && col < p.dv && k < p.dk ? init[(long long)k * p.dv + col] : 0.0f;
-        });
-    const long long cb = chunk_base(p, s, n, C);
-    for (int c = c1 - 1; c >= c0; --c) {
-        const long long r0 = (long long)c * C;
-        const int nr = s.len - r0 < C ? (int)(s.len - r0) : C;
-        __syncthreads();
-        load_tile<C, DK, PK, NT>(Qs, Q + r0 * p.ql, p.ql, nr, p.dk, p.vec);
-        load_tile<C, DK, PK, NT>(Ks, K + r0 * p.kl, p.kl, nr, p.dk, p.vec);
-        load_tile<C, DV, PV, NT>(Vs, V + r0 * p.vl, p.vl, nr, p.dv, p.vec);
-        load_tile<C, DV, PV, NT>(Os, DO + r0 * ldv, ldv, nr, p.dv, p.vec);
+        for (int m = 0; m < TW; ++m)
 #pragma unroll
-        for (int m = 0; m < VW; ++m)
-            if (wave + 4 * m < VT)
-                each_tile_element<KT>([&](int t, int r) { Ds[(16 * t + 4 * gq + r) * PV + 16 * (wave + 4 * m) + l16] = D[m][t][r]; });
-        const float gv = lane < nr ? limit_decay(g[(r0 + lane) * p.gl]) : 0.0f;
-        const double b = chunk_decay_scan(gv), bend = lane63(b);
-        const float eend = hw_exp2((float)bend);
-        if (wave == 0) {
+            for (int r = 0; r < 4; ++r) {
+                const int o = state_at(m, r, lane0);
+                D[m][r] = init && o >= 0 ? init[o] : 0.0f;
+            }
+    }
+    TileRegsF<C, DK, PK, NT, VEC> qr, kr;
+    TileRegsF<C, DV, PV, NT, VEC> vr, orr;
+    qr.init(p.ql, p.dk);
+    kr.init(p.kl, p.dk);
+    vr.init(p.vl, p.dv);
+    orr.init(ldv, p.dv);
+    const float *saved = a.chunk_states + ((chunk_base(p, s, n, C) + c1 - 1) * p.H + h) * sz;
+    auto rows_of = [&](int c) { const int left = s.len - c * C; return left < C ? left : C; };
+    auto fetch = [&](int c) {
+        const int nr = rows_of(c), ln = fresh(lane0);
+        qr.load(Q, p.ql, nr, p.dk);
+        kr.load(K, p.kl, nr, p.dk);
+        vr.load(V, p.vl, nr, p.dv);
+        orr.load(DO, ldv, nr, p.dv);
+#pragma unroll
+        for (int m = 0; m < TW; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int o = state_at(m, r, ln);
+                const float x = saved[o >= 0 ? o : 0];
+                sr[m][r] = o >= 0 ? x : 0.0f;
+            }
+    };
+    float gr = 0.0f;
+    auto fetch_g = [&](int c) {
+        if (wave == 0 && c >= c0) gr = lane0 < rows_of(c) ? limit_decay(g[((long long)c * C + lane0) * p.gl]) : 0.0f;
+    };
+    auto scan = [&](int c) {                                         // two chunks of: b (two terms), scale exp(b), exp(b_C - b), exp(b_C)
+        if (wave == 0 && c >= c0) {
+            float *d = decays + (c & 1) * 5 * 64;
+            const double b = chunk_decay_scan(gr), bend = lane63(b);
             const float hi = (float)b;
-            bh[lane] = hi;
-            bl[lane] = (float)(b - hi);
-            eb[lane] = hw_exp2(hi) * p.scale;
-            wt[lane] = hw_exp2((float)(bend - b));
+            d[lane0] = hi;
+            d[64 + lane0] = (float)(b - hi);
+            d[128 + lane0] = hw_exp2(hi) * p.scale;
+            d[192 + lane0] = hw_exp2((float)(bend - b));
+            if (lane0 == 63) d[256] = hw_exp2((float)bend);
         }
-        parts[wave * 64 + lane] = 0.0f;                                  // gradient of b_i, a partial sum of every wave
+    };
+    auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: gradients of b inside the chunk, summed from its end
+        if (wave == 1) {
+            double x = 0.0, e = 0.0;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) { x += (double)parts[w * 64 + lane0]; e += (double)corners[w]; }
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const double o = __shfl_down(x, d, 64);
+                if (lane0 + d < 64) x += o;
+            }
+            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(x + e);
+        }
+    };
+    auto put_state = [&](const f4 (&x)[TW]) {
+        const int ln = fresh(lane0);
+#pragma unroll
+        for (int m = 0; m < TW; ++m) {
+            const int t = wave + 16 * m;
+            if (t < KT * VT) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) St[(16 * (t / VT) + 4 * (ln >> 4) + r) * PV + 16 * (t % VT) + (ln & 15)] = x[m][r];
+            }
+        }
+    };
+    auto dot4 = [&](const f4 &x, const f4 &y, f4 acc) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc = mfma4(x[r], y[r], acc);
+        return acc;
+    };
+    fetch_g(c1 - 1);
+    scan(c1 - 1);
+    fetch_g(c1 - 2);
+    if (c0 < c1) fetch(c1 - 1);
+#pragma unroll 1
+    for (int c = c1 - 1; c >= c0; --c) {
+        const int nr = rows_of(c);
+        const float *bh = decays + (c & 1) * 5 * 64, *bl = bh + 64, *eb = bl + 64, *wt = eb + 64, *tail = wt + 64;
         __syncthreads();
+        if (c + 1 < c1) finish_dg(c + 1);
+        qr.put(Qs);
+        kr.put(Ks);
+        vr.put(Vs);
+        orr.put(Os);
+        put_state(sr);
+        float corner = 0.0f;                                         // <D, S>
+#pragma unroll
+        for (int m = 0; m < TW; ++m) corner += (sr[m].x * D[m].x + sr[m].y * D[m].y) + (sr[m].z * D[m].z + sr[m].w * D[m].w);
+        Q -= C * p.ql; K -= C * p.kl; V -= C * p.vl; DO -= C * ldv; saved -= p.H * sz;
+        if (c > c0) fetch(c - 1);
+        __syncthreads();
+        const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
+        parts[wave * 64 + lane] = 0.0f;
         // X, Y and the sums of M below the diagonal
-        for (int t = wave; t < CT * CT; t += 4) {
-            const int it = t / CT, jt = t % CT;
-            if (jt > it) continue;
+#pragma unroll 1
+        for (int t = wave; t < CT * (CT + 1) / 2; t += 16) {
+            const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
             f4 x = f4{0, 0, 0, 0}, y = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                const f4 u = *reinterpret_cast<const f4 *>(Qs + (16 * it + l16) * PK + 16 * kt + 4 * gq);
-                const f4 w = *reinterpret_cast<const f4 *>(Ks + (16 * jt + l16) * PK + 16 * kt + 4 * gq);
+            for (int kt = 0; kt < KT; ++kt)
+                x = dot4(*reinterpret_cast<const f4 *>(Qs + (16 * it + l16) * PK + 16 * kt + 4 * gq), *reinterpret_cast<const f4 *>(Ks + (16 * jt + l16) * PK + 16 * kt + 4 * gq), x);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x = mfma4(u[r], w[r], x);
-            }
-#pragma unroll
-            for (int vt = 0; vt < VT; ++vt) {
-                const f4 u = *reinterpret_cast<const f4 *>(Os + (16 * it + l16) * PV + 16 * vt + 4 * gq);
-                const f4 w = *reinterpret_cast<const f4 *>(Vs + (16 * jt + l16) * PV + 16 * vt + 4 * gq);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y = mfma4(u[r], w[r], y);
-            }
+            for (int v = 0; v < VT; ++v)
+                y = dot4(*reinterpret_cast<const f4 *>(Os + (16 * it + l16) * PV + 16 * v + 4 * gq), *reinterpret_cast<const f4 *>(Vs + (16 * jt + l16) * PV + 16 * v + 4 * gq), y);
             const int j = 16 * jt + l16;
             const float hj = bh[j], lj = bl[j];
+            const f4 hi = *reinterpret_cast<const f4 *>(bh + 16 * it + 4 * gq), li = *reinterpret_cast<const f4 *>(bl + 16 * it + 4 * gq);
             float colsum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * it + 4 * gq + r;
-                const float w = j <= i ? p.scale * hw_exp2((bh[i] - hj) + (bl[i] - lj)) : 0.0f;
-                const float yw = j <= i ? y[r] * w : 0.0f, xw = j <= i ? x[r] * w : 0.0f;
-                const float m = j < i ? x[r] * yw : 0.0f;
-                Xs[i * PP + j] = xw;
+                const float w = p.scale * hw_exp2((hi[r] - hj) + (li[r] - lj));
+                const float yw = j <= i ? y[r] * w : 0.0f, m = j < i ? x[r] * yw : 0.0f;
+                Xs[i * PP + j] = j <= i ? x[r] * w : 0.0f;
                 Ys[i * PP + j] = yw;
                 colsum += m;
                 const float rs = row16_sum(m);
@@ -266,140 +331,126 @@ __global__ __launch_bounds__(NT) void la_bwd_kernel(const BwdArgs a) {
             colsum += __shfl_xor(colsum, 32, 64);
             if (gq == 0) parts[wave * 64 + j] -= colsum;
         }
-        __syncthreads();
-        // dq and dk: a wave owns 16-column slices of dk.  The corner <D, S_end> = exp(b_C) <D, S> + sum_j k_j . exp(b_C - b_j) D v_j.
-        const float *Sc = a.chunk_states + ((cb + c) * p.H + h) * sz;
-        float corner_s = 0.0f, corner_k = 0.0f;
-#pragma unroll 1
-        for (int m = 0; m < KW; ++m) {
-            const int kt = wave + 4 * m;
-            if (kt >= KT) break;
-            const int k = 16 * kt + l16;                              // this lane's column
-            const bool kok = k < p.dk;
-            f4 sf[VT], df[VT];
+        const int k = 16 * qk + l16;
+        f4 dq = f4{0, 0, 0, 0};
+        if (has_q) {
 #pragma unroll
-            for (int vt = 0; vt < VT; ++vt) {
-                const int v0 = 16 * vt + 4 * gq;
-                sf[vt] = f4{0, 0, 0, 0};
-                if (kok) {
-                    if (p.vec) {
-                        if (v0 < p.dv) sf[vt] = ld4(Sc + (long long)k * p.dv + v0);
-                    } else {
+            for (int v = 0; v < VT; ++v)
+                dq = dot4(*reinterpret_cast<const f4 *>(Os + (16 * qi + l16) * PV + 16 * v + 4 * gq), *reinterpret_cast<const f4 *>(St + k * PV + 16 * v + 4 * gq), dq);
+            dq *= *reinterpret_cast<const f4 *>(eb + 16 * qi + 4 * gq);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (v0 + r < p.dv) sf[vt][r] = Sc[(long long)k * p.dv + v0 + r];
-                    }
-                }
-                df[vt] = *reinterpret_cast<const f4 *>(Ds + k * PV + v0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) corner_s += sf[vt][r] * df[vt][r];
-            }
-#pragma unroll 1
-            for (int it = 0; it < CT; ++it) {
-                f4 dq = f4{0, 0, 0, 0}, dk = f4{0, 0, 0, 0};
-#pragma unroll
-                for (int vt = 0; vt < VT; ++vt) {
-                    const f4 u = *reinterpret_cast<const f4 *>(Os + (16 * it + l16) * PV + 16 * vt + 4 * gq);
-                    const f4 w = *reinterpret_cast<const f4 *>(Vs + (16 * it + l16) * PV + 16 * vt + 4 * gq);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) { dq = mfma4(u[r], sf[vt][r], dq); dk = mfma4(w[r], df[vt][r], dk); }
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * it + 4 * gq + r;
-                    dq[r] *= eb[i];
-                    dk[r] *= wt[i];
-                    const float qq = dq[r] * Qs[i * PK + k], kk = dk[r] * Ks[i * PK + k];
-                    corner_k += kk;
-                    const float rs = row16_sum(qq - kk);
-                    if (l16 == 0) parts[wave * 64 + i] += rs;
-                }
-                for (int jt = 0; jt <= it; ++jt) {
-                    const f4 u = *reinterpret_cast<const f4 *>(Ys + (16 * it + l16) * PP + 16 * jt + 4 * gq);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) dq = mfma4(u[r], Ks[(16 * jt + 4 * gq + r) * PK + k], dq);
-                }
-                for (int jt = it; jt < CT; ++jt)                      // rows of tile `it` of dk: sums over the later tokens
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        dk = mfma4(Ys[(16 * jt + 4 * gq + r) * PP + 16 * it + l16], Qs[(16 * jt + 4 * gq + r) * PK + k], dk);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * it + 4 * gq + r;
-                    if (i < nr && kok) {
-                        st1(DQ + (r0 + i) * ldq + k, dq[r]);
-                        st1(DKp + (r0 + i) * ldq + k, dk[r]);
-                    }
-                }
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * qi + 4 * gq + r;
+                const float rs = row16_sum(dq[r] * Qs[i * PK + k]);
+                if (l16 == 0) parts[wave * 64 + i] += rs;
             }
         }
-        const float corner = lanes_sum<64>(corner_s) * eend + lanes_sum<64>(corner_k);
+        __syncthreads();                                              // X, Y are there; S is done with
+        put_state(D);
+        if (has_q) {
+            for (int jt = 0; jt <= qi; ++jt) {
+                f4 y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = Ks[(16 * jt + 4 * gq + r) * PK + k];
+                dq = dot4(*reinterpret_cast<const f4 *>(Ys + (16 * qi + l16) * PP + 16 * jt + 4 * gq), y, dq);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * qi + 4 * gq + r;
+                if (i < nr && k < p.dk) DQ[i * ldq + k] = dq[r];
+            }
+        }
+        __syncthreads();                                              // D is there
+        const float eend = tail[0];
+        corner *= eend;
+        if (has_q) {
+            f4 dk = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int v = 0; v < VT; ++v)
+                dk = dot4(*reinterpret_cast<const f4 *>(Vs + (16 * qi + l16) * PV + 16 * v + 4 * gq), *reinterpret_cast<const f4 *>(St + k * PV + 16 * v + 4 * gq), dk);
+            dk *= *reinterpret_cast<const f4 *>(wt + 16 * qi + 4 * gq);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * qi + 4 * gq + r;
+                const float kk = dk[r] * Ks[j * PK + k];
+                corner += kk;
+                const float cs = row16_sum(kk);
+                if (l16 == 0) parts[wave * 64 + j] -= cs;
+            }
+            for (int it = qi; it < CT; ++it) {
+                f4 x, y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = Ys[(16 * it + 4 * gq + r) * PP + 16 * qi + l16];
+                    y[r] = Qs[(16 * it + 4 * gq + r) * PK + k];
+                }
+                dk = dot4(x, y, dk);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * qi + 4 * gq + r;
+                if (j < nr && k < p.dk) DKp[j * ldq + k] = dk[r];
+            }
+        }
+        corner = lanes_sum<64>(corner);
         if (lane == 0) corners[wave] = corner;
-        // dv and the state: a wave owns 16-column slices of dv
+        if (has_v) {
+            const int col = 16 * vt + l16;
+            f4 dv = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int m = 0; m < VW; ++m) {
-            if (wave + 4 * m >= VT) break;
-            const int col = 16 * (wave + 4 * m) + l16;
-            const bool cok = col < p.dv;
-#pragma unroll 1
-            for (int jt = 0; jt < CT; ++jt) {
-                f4 acc = f4{0, 0, 0, 0};
+            for (int kt = 0; kt < KT; ++kt) {
+                f4 y;
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const f4 u = *reinterpret_cast<const f4 *>(Ks + (16 * jt + l16) * PK + 16 * kt + 4 * gq);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc = mfma4(u[r], D[m][kt][r], acc);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[r] *= wt[16 * jt + 4 * gq + r];
-                for (int it = jt; it < CT; ++it)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc = mfma4(Xs[(16 * it + 4 * gq + r) * PP + 16 * jt + l16], Os[(16 * it + 4 * gq + r) * PV + col], acc);
+                for (int r = 0; r < 4; ++r) y[r] = St[(16 * kt + 4 * gq + r) * PV + col];
+                dv = dot4(*reinterpret_cast<const f4 *>(Ks + (16 * vj + l16) * PK + 16 * kt + 4 * gq), y, dv);
+            }
+            dv *= *reinterpret_cast<const f4 *>(wt + 16 * vj + 4 * gq);
+            for (int it = vj; it < CT; ++it) {
+                f4 x, y;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * jt + 4 * gq + r;
-                    if (j < nr && cok) st1(DVp + (r0 + j) * ldv + col, acc[r]);
+                    x[r] = Xs[(16 * it + 4 * gq + r) * PP + 16 * vj + l16];
+                    y[r] = Os[(16 * it + 4 * gq + r) * PV + col];
                 }
+                dv = dot4(x, y, dv);
             }
 #pragma unroll
-            for (int t = 0; t < KT; ++t) D[m][t] *= eend;
-#pragma unroll
-            for (int it = 0; it < CT; ++it) {
-                float y[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * it + 4 * gq + r;
-                    y[r] = Os[i * PV + col] * eb[i];
-                }
-#pragma unroll
-                for (int t = 0; t < KT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) D[m][t] = mfma4(Qs[(16 * it + 4 * gq + r) * PK + 16 * t + l16], y[r], D[m][t]);
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * vj + 4 * gq + r;
+                if (j < nr && col < p.dv) DVp[j * ldv + col] = dv[r];
             }
         }
-        __syncthreads();
-        if (wave == 0) {
-            double x = 0.0;                                           // gradient of b_lane inside the chunk, then its sums from the end
+        DQ -= C * ldq; DKp -= C * ldq; DVp -= C * ldv;
+        scan(c - 1);
+        fetch_g(c - 2);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) x += (double)parts[w * 64 + lane];
+        for (int m = 0; m < TW; ++m) {
+            const int t = wave + 16 * m;
+            if (t >= KT * VT) break;
+            D[m] *= eend;
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double o = __shfl_down(x, d, 64);
-                if (lane + d < 64) x += o;
+            for (int it = 0; it < CT; ++it) {
+                f4 x, y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = Qs[(16 * it + 4 * gq + r) * PK + 16 * (t / VT) + l16];
+                    y[r] = Os[(16 * it + 4 * gq + r) * PV + 16 * (t % VT) + l16];
+                }
+                D[m] = dot4(x, y * *reinterpret_cast<const f4 *>(eb + 16 * it + 4 * gq), D[m]);
             }
-            const float e = (corners[0] + corners[1]) + (corners[2] + corners[3]);
-            if (lane < nr) DG[(r0 + lane) * p.H] = (float)(x + (double)e);
         }
     }
+    __syncthreads();
+    if (c0 < c1) finish_dg(c0);
     if (a.ds0 && p.nseg == 1) {
         float *d = a.ds0 + nh * sz;
 #pragma unroll
-        for (int m = 0; m < VW; ++m)
-            each_tile_element<KT>([&](int t, int r) {
-                const int k = 16 * t + 4 * gq + r, col = 16 * (wave + 4 * m) + l16;
-                if (col < p.dv && k < p.dk) d[(long long)k * p.dv + col] = D[m][t][r];
-            });
+        for (int m = 0; m < TW; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int o = state_at(m, r, lane0);
+                if (o >= 0) d[o] = D[m][r];
+            }
     }
 }
 
@@ -831,29 +882,28 @@ void launch_head_sum(const float *a, const float *b, void *oa, void *ob, long lo
     else ss2d_launch((la_head_sum_kernel<1, IO>), grid, dim3(NT), 0, s, a, b, static_cast<IO *>(oa), static_cast<IO *>(ob), total, rep, dk);
 }
 
-template <int DK, int DV, int C, typename IO>
+template <int DK, int DV, int C>
 void launch_bwd(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     const Problem &p = a.p;
     const unsigned walks = (unsigned)((long long)p.N * p.H * p.nseg);
     if (p.nseg > 1) {
-        ss2d_launch((la_bwd_seg_kernel<DK, C, IO>), dim3(walks * ((p.dv + 63) / 64)), dim3(NT), 0, s, a);
+        ss2d_launch((la_bwd_seg_kernel<DK, C>), dim3(walks * ((p.dv + 63) / 64)), dim3(NT), 0, s, a);
         const long long sz = (long long)p.dk * p.dv;
         ss2d_launch(la_join_bwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(p.N * p.H)), dim3(NT), 0, s, a, C);
     }
-    if (p.H > p.G) ss2d_launch((la_bwd_kernel<DK, DV, C, IO, float>), dim3(walks + gaps), dim3(NT), 0, s, a);
-    else ss2d_launch((la_bwd_kernel<DK, DV, C, IO, IO>), dim3(walks + gaps), dim3(NT), 0, s, a);
+    if (p.vec) ss2d_launch((la_bwd_kernel<DK, DV, C, true>), dim3(walks + gaps), dim3(1024), 0, s, a);
+    else ss2d_launch((la_bwd_kernel<DK, DV, C, false>), dim3(walks + gaps), dim3(1024), 0, s, a);
 }
-
 void dispatch_bwd_f32(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     const int dk = a.p.dk, dv = a.p.dv;
     if (dv <= 64) {
-        if (dk <= 16) launch_bwd<16, 64, 64, float>(a, gaps, s);
-        else if (dk <= 64) launch_bwd<64, 64, 64, float>(a, gaps, s);
-        else launch_bwd<128, 64, 32, float>(a, gaps, s);
+        if (dk <= 16) launch_bwd<16, 64, 64>(a, gaps, s);
+        else if (dk <= 64) launch_bwd<64, 64, 64>(a, gaps, s);
+        else launch_bwd<128, 64, 32>(a, gaps, s);
     } else {
-        if (dk <= 16) launch_bwd<16, 128, 32, float>(a, gaps, s);
-        else if (dk <= 64) launch_bwd<64, 128, 32, float>(a, gaps, s);
-        else launch_bwd<128, 128, 32, float>(a, gaps, s);
+        if (dk <= 16) launch_bwd<16, 128, 32>(a, gaps, s);
+        else if (dk <= 64) launch_bwd<64, 128, 32>(a, gaps, s);
+        else launch_bwd<128, 128, 32>(a, gaps, s);
     }
 }
 

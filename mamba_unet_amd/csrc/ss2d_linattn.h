@@ -93,28 +93,6 @@ __device__ __forceinline__ double lane63(double b) {
 // a value that the compiler takes as new: addresses made from it are computed where they are used instead of living across a loop
 __device__ __forceinline__ int fresh(int v) { asm volatile("" : "+v"(v)); return v; }
 
-// rows [0, C) of `src` (row stride ld, D columns, rows >= n read as zero) -> fp32 tile in LDS, PITCH floats a row, columns
-// D .. DP-1 zero
-template <int C, int DP, int PITCH, int NT, typename IO>
-__device__ __forceinline__ void load_tile(float *dst, const IO *src, long long ld, int n, int D, bool vec) {
-    constexpr int Q = DP / 4;
-    for (int e = threadIdx.x; e < C * Q; e += NT) {
-        const int r = e / Q, c = 4 * (e % Q);
-        f4 v = f4{0, 0, 0, 0};
-        if (r < n) {
-            const IO *s = src + (long long)r * ld + c;
-            if (vec) {
-                if (c < D) v = ld4(s);
-            } else {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    if (c + t < D) v[t] = ld1(s + t);
-            }
-        }
-        *reinterpret_cast<f4 *>(dst + r * PITCH + c) = v;
-    }
-}
-
 // ---- bf16 operands on v_mfma_f32_16x16x32_bf16.  A lane (l16 = lane & 15, gq = lane >> 4) holds row / column l16 of an operand and eight of the 32
 // contracted indices.  Here they are 4 gq + {0..3} and 16 + 4 gq + {0..3} for every operand: the two halves are then exactly the rows that
 // the lane holds of two neighbouring 16 x 16 results, so a state in accumulators is an operand without moving data.
@@ -181,7 +159,7 @@ struct TileRegs {
         const int r = threadIdx.x / PR, c = 8 * (threadIdx.x % PR);
         voff = c < D && r < C ? (r * (int)ld + c) * 2 : SS2D_BUF_OOR;
     }
-    // a descriptor of n rows: later rows read as zero.  ld < 2^23 elements (host)
+    // a descriptor of n rows: later rows read as zero.  ld < 2^22 elements (host)
     __device__ __forceinline__ void load(const bf16 *src, long long ld, int n) {
         if (!VEC) return;
         const __amdgpu_buffer_rsrc_t rs = make_rsrc(src, (unsigned)(n * (int)ld * 2));
@@ -293,12 +271,13 @@ inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, 
     bool vec = dk % m == 0 && dv % m == 0 && ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0;
     for (int i = 0; i < 9; ++i) vec = vec && st[i] % m == 0;
     // 16-byte pieces come through descriptors of a chunk's rows: dense enough not to overlap, and short of 2^31 bytes
-    vec = vec && st[1] >= dk && st[4] >= dk && st[7] >= dv && st[1] < (1 << 23) && st[4] < (1 << 23) && st[7] < (1 << 23);
+    vec = vec && st[1] >= dk && st[4] >= dk && st[7] >= dv && st[1] < (1 << 22) && st[4] < (1 << 22) && st[7] < (1 << 22);
     p.vec = vec;
     return 0;
 }
 
 }  // namespace linattn
 
-// the pass over bf16 segments that leaves their own contributions (forward: k v^T; reverse: q dout^T), defined beside the forward
-void linattn_segment_pass_bf16(const linattn::Problem &p, float *seg_states, double *seg_decay, const float *want_end, bool reverse, hipStream_t s);
+// the pass over segments that leaves their own contributions (forward: k v^T; reverse: q dout^T, with q in the place of k and dout in that of v),
+// defined beside the forward
+void linattn_segment_pass(int dtype, const linattn::Problem &p, float *seg_states, double *seg_decay, const float *want_end, bool reverse, hipStream_t s);

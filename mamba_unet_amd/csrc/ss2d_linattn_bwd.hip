@@ -41,72 +41,6 @@ __device__ __forceinline__ float row16_sum(float v) {
     return v;
 }
 
-// (fp32) a segment's own contribution to D: sum over its tokens of scale exp(b) q do^T
-template <int DK, int C>
-__global__ __launch_bounds__(NT) void la_bwd_seg_kernel(const BwdArgs a) {
-    constexpr int PK = DK + 4, PV = 64 + 4, KT = DK / 16, CT = C / 16;
-    __shared__ __attribute__((aligned(16))) float lds[C * PK + C * PV + 64];
-    float *Qs = lds, *Os = Qs + C * PK, *eb = Os + C * PV;
-    const Problem &p = a.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, gq = lane >> 4;
-    const int dvt = (p.dv + 63) / 64;
-    int id = blockIdx.x;
-    const int vt = id % dvt; id /= dvt;
-    const int seg = id % p.nseg; id /= p.nseg;
-    const int h = id % p.H, n = id / p.H;
-    const Seq s = get_seq(p, n);
-    const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
-    const int c1 = segment_end(p, seg, nch);
-    if (c0 >= c1) return;
-    const int hk = h / (p.H / p.G), col = 64 * vt + 16 * wave + l16;
-    const bool cok = col < p.dv;
-    const float *Q = static_cast<const float *>(p.q) + s.row * p.qb + s.start * p.ql + hk * p.qh;
-    const long long ldo = (long long)p.H * p.dv, nh = (long long)n * p.H + h, sz = (long long)p.dk * p.dv;
-    const float *DO = static_cast<const float *>(a.dout) + ((s.row * p.tokens + s.start) * p.H + h) * (long long)p.dv + 64 * vt;
-    const float *g = p.g + s.row * p.gb + s.start * p.gl + h * p.gh;
-    f4 D[KT];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) D[t] = f4{0, 0, 0, 0};
-    double total = 0.0;
-    for (int c = c1 - 1; c >= c0; --c) {
-        const long long r0 = (long long)c * C;
-        const int nr = s.len - r0 < C ? (int)(s.len - r0) : C;
-        __syncthreads();
-        load_tile<C, DK, PK, NT>(Qs, Q + r0 * p.ql, p.ql, nr, p.dk, p.vec);
-        load_tile<C, 64, PV, NT>(Os, DO + r0 * ldo, ldo, nr, p.dv - 64 * vt, p.vec);
-        const float gv = lane < nr ? limit_decay(g[(r0 + lane) * p.gl]) : 0.0f;
-        const double b = chunk_decay_scan(gv), bend = lane63(b);
-        total += bend;
-        const float eend = hw_exp2((float)bend);
-        if (wave == 0) eb[lane] = hw_exp2((float)b) * p.scale;
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < KT; ++t) D[t] *= eend;
-#pragma unroll
-        for (int it = 0; it < CT; ++it) {
-            float y[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * it + 4 * gq + r;
-                y[r] = Os[i * PV + 16 * wave + l16] * eb[i];
-            }
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) D[t] = mfma4(Qs[(16 * it + 4 * gq + r) * PK + 16 * t + l16], y[r], D[t]);
-        }
-    }
-    float *dst = a.seg_states + (nh * p.nseg + seg) * sz;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int k = 16 * t + 4 * gq + r;
-            if (cok && k < p.dk) dst[(long long)k * p.dv + col] = D[t][r];
-        }
-    if (tid == 0 && vt == 0) a.seg_decay[nh * p.nseg + seg] = total;
-}
-
 // seg_states[s] = D behind segment s
 __global__ __launch_bounds__(NT) void la_join_bwd_kernel(const BwdArgs a, int C) {
     const Problem &p = a.p;
@@ -884,14 +818,8 @@ void launch_head_sum(const float *a, const float *b, void *oa, void *ob, long lo
 
 template <int DK, int DV, int C>
 void launch_bwd(const BwdArgs &a, unsigned gaps, hipStream_t s) {
-    const Problem &p = a.p;
-    const unsigned walks = (unsigned)((long long)p.N * p.H * p.nseg);
-    if (p.nseg > 1) {
-        ss2d_launch((la_bwd_seg_kernel<DK, C>), dim3(walks * ((p.dv + 63) / 64)), dim3(NT), 0, s, a);
-        const long long sz = (long long)p.dk * p.dv;
-        ss2d_launch(la_join_bwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(p.N * p.H)), dim3(NT), 0, s, a, C);
-    }
-    if (p.vec) ss2d_launch((la_bwd_kernel<DK, DV, C, true>), dim3(walks + gaps), dim3(1024), 0, s, a);
+    const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg);
+    if (a.p.vec) ss2d_launch((la_bwd_kernel<DK, DV, C, true>), dim3(walks + gaps), dim3(1024), 0, s, a);
     else ss2d_launch((la_bwd_kernel<DK, DV, C, false>), dim3(walks + gaps), dim3(1024), 0, s, a);
 }
 void dispatch_bwd_f32(const BwdArgs &a, unsigned gaps, hipStream_t s) {
@@ -917,14 +845,6 @@ void launch_bwd_bf16(const BwdArgs &a, unsigned gaps, hipStream_t s) {
 template <bool VEC>
 void dispatch_bwd_bf16(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     const Problem &p = a.p;
-    if (p.nseg > 1) {
-        Problem r = p;                            // q in the place of k, dout in that of v
-        r.k = p.q; r.kb = p.qb; r.kl = p.ql; r.kh = p.qh;
-        r.v = a.dout; r.vb = p.tokens * p.H * p.dv; r.vl = (long long)p.H * p.dv; r.vh = p.dv;
-        linattn_segment_pass_bf16(r, a.seg_states, a.seg_decay, a.ds0, true, s);
-        const long long sz = (long long)p.dk * p.dv;
-        ss2d_launch(la_join_bwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(p.N * p.H)), dim3(NT), 0, s, a, 64);
-    }
     const int dk = p.dk;
     if (p.dv <= 64) {
         if (dk <= 32) launch_bwd_bf16<32, 64, VEC>(a, gaps, s);
@@ -955,7 +875,15 @@ extern "C" int ss2d_linattn_bwd(int dtype, const void *q, const void *k, const v
     a.p.vec = a.p.vec && (uintptr_t)dout % 16 == 0;
     const unsigned gaps = cu_seqlens ? GAP_WGS : 0;
     hipStream_t s = (hipStream_t)stream;
-    a.p.vec = a.p.vec && (long long)H * dv < (1 << 23);
+    a.p.vec = a.p.vec && (long long)H * dv < (1 << 22);
+    if (nseg > 1) {
+        Problem r = a.p;                          // q in the place of k, dout in that of v
+        r.k = q; r.kb = r.qb; r.kl = r.ql; r.kh = r.qh;
+        r.v = dout; r.vb = tokens * H * dv; r.vl = (long long)H * dv; r.vh = dv;
+        linattn_segment_pass(dtype, r, seg_states, seg_decay, ds0, true, s);
+        const long long sz = (long long)dk * dv;
+        ss2d_launch(la_join_bwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(N * H)), dim3(NT), 0, s, a, linattn_chunk(dtype, dk, dv));
+    }
     if (dtype == SS2D_DTYPE_F32) dispatch_bwd_f32(a, gaps, s);
     else if (a.p.vec) dispatch_bwd_bf16<true>(a, gaps, s);
     else dispatch_bwd_bf16<false>(a, gaps, s);

@@ -6,7 +6,6 @@
 // columns of dv.  A sequence is cut into segments when there are too few (sequence, head) pairs to fill the card: a first pass
 // leaves every segment's own contribution, a small pass joins them in order, and the main pass starts each segment from its
 // true state.
-#include <type_traits>
 #include "ss2d_linattn.h"
 #include "../../include/ss2d.h"
 
@@ -36,83 +35,119 @@ __device__ void zero_gaps(const Problem &p, IO *o, long long row, int w) {
     for (long long e = hi * row + (long long)w * NT + threadIdx.x; e < p.tokens * row; e += step) st1(o + e, 0.0f);
 }
 
-// mode 0: the whole walk; mode 1: only a segment's own contribution to the state; (bf16) mode 2: the backward's, sum of scale exp(b) q dout^T from the
+// mode 0: the whole walk; mode 1: only a segment's own contribution to the state; mode 2: the backward's, sum of scale exp(b) q dout^T from the
 // segment's end, with q in the place of k and dout in that of v
-template <int DK, int C, int MODE, typename IO>
+// fp32 on v_mfma_f32_16x16x4_f32, 64 columns of dv a workgroup: a lane holds row / column l16 of an operand and contracted indices 4 gq + r of a
+// 16-block in step r, so a state tile in accumulators is an operand; direct operands are 16-byte LDS reads, transposed ones 4-byte reads, both free of
+// bank conflicts at a pitch of 4 mod 16 floats.  The next chunk is in flight in registers.
+template <int DK, int C, int MODE, bool VEC>
 __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     constexpr int PK = DK + 4, PV = 64 + 4, PP = C + 4, KT = DK / 16, CT = C / 16;
-    __shared__ __attribute__((aligned(16))) float lds[C * PK + C * PV + 256 + (MODE == 0 ? C * PK + C * PP : 0)];
-    float *Ks = lds, *Vs = Ks + C * PK, *bh = Vs + C * PV, *bl = bh + 64, *eb = bl + 64, *wt = eb + 64, *Qs = wt + 64, *Ps = Qs + C * PK;
+    __shared__ __attribute__((aligned(16))) float lds[C * PK + C * PV + 640 + (MODE == 0 ? C * PK + C * PP : 0)];
+    float *Ks = lds, *Vs = Ks + C * PK, *decays = Vs + C * PV, *Qs = decays + 640, *Ps = Qs + C * PK;
     const Problem &p = a.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, gq = lane >> 4;
-    const int dvt = (p.dv + 63) / 64;
-    int id = blockIdx.x;
-    if (id >= p.N * p.H * p.nseg * dvt) {        // packed rows that belong to no sequence: their output is zero
-        if (MODE == 0) zero_gaps(p, static_cast<IO *>(a.o), (long long)p.H * p.dv, id - p.N * p.H * p.nseg * dvt);
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, gq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int dvt = (p.dv + 63) / 64, walks = p.N * p.H * p.nseg * dvt;
+    if ((int)blockIdx.x >= walks) {              // packed rows that belong to no sequence: their output is zero
+        if (MODE == 0) zero_gaps(p, static_cast<float *>(a.o), (long long)p.H * p.dv, blockIdx.x - walks);
         return;
     }
+    int id = xcd_remap(blockIdx.x, walks);
     const int vt = id % dvt; id /= dvt;
-    const int seg = id % p.nseg; id /= p.nseg;
-    const int h = id % p.H, n = id / p.H;
+    const int h = id % p.H; id /= p.H;
+    const int seg = id % p.nseg, n = id / p.nseg;
     const Seq s = get_seq(p, n);
     const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
     const int c1 = segment_end(p, seg, nch);
     const bool empty = s.len == 0;
     if (c0 >= c1 && !(empty && seg == 0)) return;
     if (MODE == 1 && c1 == nch && !empty && !a.last) return;     // nothing starts from the last segment's end
-    const int hk = h / (p.H / p.G), col = 64 * vt + 16 * wave + l16;
+    if (MODE == 2 && c0 == 0 && !a.last) return;                 // (here: the gradient in front of the first segment is not wanted)
+    const int hk = h / (p.H / p.G), col = 64 * vt + 16 * wave + l16, first = MODE == 2 ? c1 - 1 : c0, dvc = p.dv - 64 * vt;
     const bool cok = col < p.dv;
-    const IO *Q = static_cast<const IO *>(p.q) + s.row * p.qb + s.start * p.ql + hk * p.qh;
-    const IO *K = static_cast<const IO *>(p.k) + s.row * p.kb + s.start * p.kl + hk * p.kh;
-    const IO *V = static_cast<const IO *>(p.v) + s.row * p.vb + s.start * p.vl + h * p.vh + 64 * vt;
+    const float *Q = static_cast<const float *>(p.q) + s.row * p.qb + (s.start + (long long)c0 * C) * p.ql + hk * p.qh;
+    const float *K = static_cast<const float *>(p.k) + s.row * p.kb + (s.start + (long long)first * C) * p.kl + hk * p.kh;
+    const float *V = static_cast<const float *>(p.v) + s.row * p.vb + (s.start + (long long)first * C) * p.vl + h * p.vh + 64 * vt;
     const float *g = p.g + s.row * p.gb + s.start * p.gl + h * p.gh;
-    IO *O = static_cast<IO *>(a.o) + ((s.row * p.tokens + s.start) * p.H + h) * (long long)p.dv;
     const long long ldo = (long long)p.H * p.dv, nh = (long long)n * p.H + h, sz = (long long)p.dk * p.dv;
+    float *O = static_cast<float *>(a.o) + ((s.row * p.tokens + s.start + (long long)c0 * C) * p.H + h) * (long long)p.dv + col;
     f4 S[KT];
-    const float *init = MODE == 1 ? nullptr : p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
+    const float *init = MODE >= 1 ? nullptr : p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int k = 16 * t + 4 * gq + r;
-            S[t][r] = init && cok && k < p.dk ? init[(long long)k * p.dv + col] : 0.0f;
+            S[t][r] = init && cok && k < p.dk ? init[k * p.dv + col] : 0.0f;
         }
     double total = 0.0;
-    const long long cb = chunk_base(p, s, n, C);
-    for (int c = c0; c < c1; ++c) {
-        const long long r0 = (long long)c * C;
-        const int nr = s.len - r0 < C ? (int)(s.len - r0) : C;
-        if (MODE == 0 && a.chunk_states) {
-            float *d = a.chunk_states + ((cb + c) * p.H + h) * sz;
+    float *saved = MODE == 0 && a.chunk_states ? a.chunk_states + ((chunk_base(p, s, n, C) + c0) * p.H + h) * sz : nullptr;
+    TileRegsF<C, DK, PK, NT, VEC> qr, kr;
+    TileRegsF<C, 64, PV, NT, VEC> vr;
+    qr.init(p.ql, p.dk);
+    kr.init(p.kl, p.dk);
+    vr.init(p.vl, dvc);
+    auto rows_of = [&](int c) { const int left = s.len - c * C; return left < C ? left : C; };
+    constexpr int STEP = MODE == 2 ? -1 : 1;
+    auto fetch = [&](int c) {                    // chunk c, the tensors' pointers at chunk c
+        const int nr = rows_of(c);
+        if (MODE == 0) qr.load(Q, p.ql, nr, p.dk);
+        kr.load(K, p.kl, nr, p.dk);
+        vr.load(V, p.vl, nr, dvc);
+        Q += C * p.ql; K += STEP * C * p.kl; V += STEP * C * p.vl;
+    };
+    float gr = 0.0f;                             // wave 0: decays, a chunk ahead of the tiles
+    auto fetch_g = [&](int c) {
+        if (wave == 0 && c >= c0 && c < c1) gr = lane < rows_of(c) ? limit_decay(g[((long long)c * C + lane) * p.gl]) : 0.0f;
+    };
+    auto scan = [&](int c) {                     // two chunks of: b (two terms), scale exp(b), exp(b_C - b), exp(b_C)
+        if (wave == 0 && c >= c0 && c < c1) {
+            float *d = decays + (c & 1) * 320;
+            const double b = chunk_decay_scan(gr), bend = lane63(b);
+            const float hi = (float)b;
+            if (MODE >= 1) total += bend;
+            d[lane] = hi;
+            d[64 + lane] = (float)(b - hi);
+            d[128 + lane] = hw_exp2(hi) * p.scale;
+            d[192 + lane] = hw_exp2((float)(bend - b));
+            if (lane == 63) d[256] = hw_exp2((float)bend);
+        }
+    };
+    fetch_g(first);
+    scan(first);
+    fetch_g(first + STEP);
+    if (c0 < c1) fetch(first);
+#pragma unroll 1
+    for (int c = first; c >= c0 && c < c1; c += STEP) {
+        const int nr = rows_of(c);
+        if (MODE == 0 && saved) {
+            float *d = saved + (4 * gq) * p.dv + col;
+            int step = p.dv;
+            asm volatile("" : "+s"(step));       // (else the offsets of all rows live in registers across the loop)
 #pragma unroll
-            for (int t = 0; t < KT; ++t)
+            for (int t = 0; t < KT; ++t) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int k = 16 * t + 4 * gq + r;
-                    if (cok && k < p.dk) d[(long long)k * p.dv + col] = S[t][r];
+                    if (cok && 16 * t + 4 * gq + r < p.dk) *d = S[t][r];
+                    d += step;
                 }
+                d += 12 * step;
+            }
+            saved += p.H * sz;
         }
         __syncthreads();
-        if (MODE == 0) load_tile<C, DK, PK, NT>(Qs, Q + r0 * p.ql, p.ql, nr, p.dk, p.vec);
-        load_tile<C, DK, PK, NT>(Ks, K + r0 * p.kl, p.kl, nr, p.dk, p.vec);
-        load_tile<C, 64, PV, NT>(Vs, V + r0 * p.vl, p.vl, nr, p.dv - 64 * vt, p.vec);
-        const float gv = lane < nr ? limit_decay(g[(r0 + lane) * p.gl]) : 0.0f;
-        const double b = chunk_decay_scan(gv), bend = lane63(b);
-        total += bend;
-        const float eend = hw_exp2((float)bend);
-        if (wave == 0) {
-            const float hi = (float)b;
-            bh[lane] = hi;
-            bl[lane] = (float)(b - hi);
-            eb[lane] = hw_exp2(hi) * p.scale;
-            wt[lane] = hw_exp2((float)(bend - b));
-        }
+        if (MODE == 0) qr.put(Qs);
+        kr.put(Ks);
+        vr.put(Vs);
+        if (c + STEP >= c0 && c + STEP < c1) fetch(c + STEP);
         __syncthreads();
+        const float *bh = decays + (c & 1) * 320, *bl = bh + 64, *eb = bl + 64, *wt = eb + 64, *tail = wt + 64;
         if (MODE == 0) {
             // P[i][j] = scale exp(b_i - b_j) q_i . k_j, j <= i: tiles (it, jt) dealt to the waves
-            for (int t = wave; t < CT * CT; t += 4) {
-                const int it = t / CT, jt = t % CT;
-                if (jt > it) continue;
+#pragma unroll 1
+            for (int t = wave; t < CT * (CT + 1) / 2; t += 4) {
+                const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
                 f4 acc = f4{0, 0, 0, 0};
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
@@ -123,62 +158,75 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
                 }
                 const int j = 16 * jt + l16;
                 const float hj = bh[j], lj = bl[j];
+                const f4 hi = *reinterpret_cast<const f4 *>(bh + 16 * it + 4 * gq), li = *reinterpret_cast<const f4 *>(bl + 16 * it + 4 * gq);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = 16 * it + 4 * gq + r;
-                    Ps[i * PP + j] = j <= i ? acc[r] * p.scale * hw_exp2((bh[i] - hj) + (bl[i] - lj)) : 0.0f;
+                    Ps[i * PP + j] = j <= i ? acc[r] * p.scale * hw_exp2((hi[r] - hj) + (li[r] - lj)) : 0.0f;
                 }
             }
             __syncthreads();
+        }
+        float vv[CT][4];                         // this wave's columns of v: rows 16 jt + 4 gq + r
 #pragma unroll
-            for (int it = 0; it < CT; ++it) {
-                f4 acc = f4{0, 0, 0, 0};
+        for (int jt = 0; jt < CT; ++jt)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
+            for (int r = 0; r < 4; ++r) vv[jt][r] = Vs[(16 * jt + 4 * gq + r) * PV + 16 * wave + l16];
+        if (MODE == 0) {
+            f4 acc[CT];
+#pragma unroll
+            for (int it = 0; it < CT; ++it) acc[it] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int it = 0; it < CT; ++it) {
                     const f4 x = *reinterpret_cast<const f4 *>(Qs + (16 * it + l16) * PK + 16 * kt + 4 * gq);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc = mfma4(x[r], S[kt][r], acc);
+                    for (int r = 0; r < 4; ++r) acc[it] = mfma4(x[r], S[kt][r], acc[it]);
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[r] *= eb[16 * it + 4 * gq + r];
+            for (int it = 0; it < CT; ++it) {
+                acc[it] *= *reinterpret_cast<const f4 *>(eb + 16 * it + 4 * gq);
+#pragma unroll
                 for (int jt = 0; jt <= it; ++jt) {
                     const f4 x = *reinterpret_cast<const f4 *>(Ps + (16 * it + l16) * PP + 16 * jt + 4 * gq);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc = mfma4(x[r], Vs[(16 * jt + 4 * gq + r) * PV + 16 * wave + l16], acc);
+                    for (int r = 0; r < 4; ++r) acc[it] = mfma4(x[r], vv[jt][r], acc[it]);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = 16 * it + 4 * gq + r;
-                    if (i < nr && cok) st1(O + (r0 + i) * ldo + col, acc[r]);
+                    if (i < nr && cok) O[i * ldo] = acc[it][r];
                 }
             }
+            O += C * ldo;
         }
+        scan(c + STEP);
+        fetch_g(c + 2 * STEP);
+        const float eend = tail[0];
 #pragma unroll
         for (int t = 0; t < KT; ++t) S[t] *= eend;
 #pragma unroll
         for (int jt = 0; jt < CT; ++jt) {
-            float y[4];
+            const f4 w = *reinterpret_cast<const f4 *>((MODE == 2 ? eb : wt) + 16 * jt + 4 * gq);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = 16 * jt + 4 * gq + r;
-                y[r] = Vs[j * PV + 16 * wave + l16] * wt[j];
-            }
+            for (int r = 0; r < 4; ++r) vv[jt][r] *= w[r];
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[t] = mfma4(Ks[(16 * jt + 4 * gq + r) * PK + 16 * t + l16], y[r], S[t]);
+                for (int r = 0; r < 4; ++r) S[t] = mfma4(Ks[(16 * jt + 4 * gq + r) * PK + 16 * t + l16], vv[jt][r], S[t]);
         }
     }
-    float *dst = MODE == 1 ? a.seg_states + (nh * p.nseg + seg) * sz : (a.last && p.nseg == 1) ? a.last + nh * sz : nullptr;
+    float *dst = MODE >= 1 ? a.seg_states + (nh * p.nseg + seg) * sz : (a.last && p.nseg == 1) ? a.last + nh * sz : nullptr;
     if (dst) {
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int k = 16 * t + 4 * gq + r;
-                if (cok && k < p.dk) dst[(long long)k * p.dv + col] = S[t][r];
+                if (cok && k < p.dk) dst[k * p.dv + col] = S[t][r];
             }
-        if (MODE == 1 && tid == 0 && vt == 0) a.seg_decay[nh * p.nseg + seg] = total;
+        if (MODE >= 1 && tid == 0 && vt == 0) a.seg_decay[nh * p.nseg + seg] = total;
     }
 }
 
@@ -419,74 +467,49 @@ __global__ __launch_bounds__(NT) void la_join_fwd_kernel(const FwdArgs a, int C)
     if (a.last) a.last[nh * sz + e] = v;
 }
 
-template <int DK, int C, typename IO>
-void launch_fwd(const FwdArgs &a, unsigned gaps, hipStream_t s) {
-    const Problem &p = a.p;
-    const unsigned grid = (unsigned)((long long)p.N * p.H * p.nseg * ((p.dv + 63) / 64));
-    if (p.nseg > 1) {
-        ss2d_launch((la_fwd_kernel<DK, C, 1, IO>), dim3(grid), dim3(NT), 0, s, a);
-        const long long sz = (long long)p.dk * p.dv;
-        ss2d_launch(la_join_fwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(p.N * p.H)), dim3(NT), 0, s, a, C);
-    }
-    ss2d_launch((la_fwd_kernel<DK, C, 0, IO>), dim3(grid + gaps), dim3(NT), 0, s, a);
+template <int MODE, bool VEC, int DK, int C>
+void launch_f32(const FwdArgs &a, unsigned gaps, hipStream_t s) {
+    const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg * ((a.p.dv + 63) / 64));
+    ss2d_launch((la_fwd_kernel<DK, C, MODE, VEC>), dim3(walks + gaps), dim3(NT), 0, s, a);
 }
-
-void dispatch_fwd_f32(const FwdArgs &a, unsigned gaps, hipStream_t s) {
+template <int MODE, bool VEC>
+void dispatch_f32(const FwdArgs &a, unsigned gaps, hipStream_t s) {
     const int dk = a.p.dk;
     const bool c64 = linattn_chunk(SS2D_DTYPE_F32, a.p.dk, a.p.dv) == 64;
-    if (dk <= 16) c64 ? launch_fwd<16, 64, float>(a, gaps, s) : launch_fwd<16, 32, float>(a, gaps, s);
-    else if (dk <= 64) c64 ? launch_fwd<64, 64, float>(a, gaps, s) : launch_fwd<64, 32, float>(a, gaps, s);
-    else launch_fwd<128, 32, float>(a, gaps, s);
+    if (dk <= 16) c64 ? launch_f32<MODE, VEC, 16, 64>(a, gaps, s) : launch_f32<MODE, VEC, 16, 32>(a, gaps, s);
+    else if (dk <= 64) c64 ? launch_f32<MODE, VEC, 64, 64>(a, gaps, s) : launch_f32<MODE, VEC, 64, 32>(a, gaps, s);
+    else launch_f32<MODE, VEC, 128, 32>(a, gaps, s);
 }
-
-template <int DK, int NW, bool VEC>
-void launch_fwd_bf16(const FwdArgs &a, unsigned gaps, hipStream_t s) {
-    const Problem &p = a.p;
-    const unsigned walks = (unsigned)((long long)p.N * p.H * p.nseg);
-    if (p.nseg > 1) {
-        linattn_segment_pass_bf16(p, a.seg_states, a.seg_decay, a.last, false, s);
-        const long long sz = (long long)p.dk * p.dv;
-        ss2d_launch(la_join_fwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(p.N * p.H)), dim3(NT), 0, s, a, 64);
-    }
-    ss2d_launch((la_fwd_bf16_kernel<DK, NW, 0, VEC>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
+template <int MODE, bool VEC, int DK, int NW>
+void launch_bf16(const FwdArgs &a, unsigned gaps, hipStream_t s) {
+    ss2d_launch((la_fwd_bf16_kernel<DK, NW, MODE, VEC>), dim3((unsigned)((long long)a.p.N * a.p.H * a.p.nseg) + gaps), dim3(64 * NW), 0, s, a);
 }
-template <bool VEC>
-void dispatch_fwd_bf16(const FwdArgs &a, unsigned gaps, hipStream_t s) {
-    const int dk = a.p.dk;
-    if (a.p.dv <= 64) {
-        if (dk <= 32) launch_fwd_bf16<32, 4, VEC>(a, gaps, s);
-        else if (dk <= 64) launch_fwd_bf16<64, 4, VEC>(a, gaps, s);
-        else launch_fwd_bf16<128, 4, VEC>(a, gaps, s);
-    } else {
-        if (dk <= 32) launch_fwd_bf16<32, 8, VEC>(a, gaps, s);
-        else if (dk <= 64) launch_fwd_bf16<64, 8, VEC>(a, gaps, s);
-        else launch_fwd_bf16<128, 8, VEC>(a, gaps, s);
-    }
-}
-
 template <int MODE, bool VEC>
-void segment_pass(const FwdArgs &a, hipStream_t s) {
-    const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg);
+void dispatch_bf16(const FwdArgs &a, unsigned gaps, hipStream_t s) {
     const int dk = a.p.dk;
     if (a.p.dv <= 64) {
-        if (dk <= 32) ss2d_launch((la_fwd_bf16_kernel<32, 4, MODE, VEC>), dim3(walks), dim3(256), 0, s, a);
-        else if (dk <= 64) ss2d_launch((la_fwd_bf16_kernel<64, 4, MODE, VEC>), dim3(walks), dim3(256), 0, s, a);
-        else ss2d_launch((la_fwd_bf16_kernel<128, 4, MODE, VEC>), dim3(walks), dim3(256), 0, s, a);
+        if (dk <= 32) launch_bf16<MODE, VEC, 32, 4>(a, gaps, s);
+        else if (dk <= 64) launch_bf16<MODE, VEC, 64, 4>(a, gaps, s);
+        else launch_bf16<MODE, VEC, 128, 4>(a, gaps, s);
     } else {
-        if (dk <= 32) ss2d_launch((la_fwd_bf16_kernel<32, 8, MODE, VEC>), dim3(walks), dim3(512), 0, s, a);
-        else if (dk <= 64) ss2d_launch((la_fwd_bf16_kernel<64, 8, MODE, VEC>), dim3(walks), dim3(512), 0, s, a);
-        else ss2d_launch((la_fwd_bf16_kernel<128, 8, MODE, VEC>), dim3(walks), dim3(512), 0, s, a);
+        if (dk <= 32) launch_bf16<MODE, VEC, 32, 8>(a, gaps, s);
+        else if (dk <= 64) launch_bf16<MODE, VEC, 64, 8>(a, gaps, s);
+        else launch_bf16<MODE, VEC, 128, 8>(a, gaps, s);
     }
+}
+template <int MODE>
+void dispatch(int dtype, const FwdArgs &a, unsigned gaps, hipStream_t s) {
+    if (dtype == SS2D_DTYPE_F32) a.p.vec ? dispatch_f32<MODE, true>(a, gaps, s) : dispatch_f32<MODE, false>(a, gaps, s);
+    else a.p.vec ? dispatch_bf16<MODE, true>(a, gaps, s) : dispatch_bf16<MODE, false>(a, gaps, s);
 }
 
 }  // namespace
 
-void linattn_segment_pass_bf16(const linattn::Problem &p, float *seg_states, double *seg_decay, const float *want_end, bool reverse, hipStream_t s) {
+void linattn_segment_pass(int dtype, const linattn::Problem &p, float *seg_states, double *seg_decay, const float *want_end, bool reverse, hipStream_t s) {
     FwdArgs a{};
     a.p = p; a.seg_states = seg_states; a.seg_decay = seg_decay;
     a.last = const_cast<float *>(want_end);      // only asked for being there
-    if (reverse) p.vec ? segment_pass<2, true>(a, s) : segment_pass<2, false>(a, s);
-    else p.vec ? segment_pass<1, true>(a, s) : segment_pass<1, false>(a, s);
+    reverse ? dispatch<2>(dtype, a, 0, s) : dispatch<1>(dtype, a, 0, s);
 }
 
 extern "C" int ss2d_linattn_chunk(int dtype, int dk, int dv) { return linattn_chunk(dtype, dk, dv); }
@@ -506,9 +529,13 @@ extern "C" int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const v
     if (nseg > 1 && (!seg_states || !seg_decay)) { ss2d_set_error("linattn_fwd: segments without a workspace"); return -2; }
     a.o = out; a.s0 = s0; a.last = last; a.chunk_states = chunk_states; a.seg_states = seg_states; a.seg_decay = seg_decay;
     const unsigned gaps = cu_seqlens ? GAP_WGS : 0;
-    if (dtype == SS2D_DTYPE_F32) dispatch_fwd_f32(a, gaps, (hipStream_t)stream);
-    else if (a.p.vec) dispatch_fwd_bf16<true>(a, gaps, (hipStream_t)stream);
-    else dispatch_fwd_bf16<false>(a, gaps, (hipStream_t)stream);
+    hipStream_t s = (hipStream_t)stream;
+    if (nseg > 1) {
+        linattn_segment_pass(dtype, a.p, seg_states, seg_decay, last, false, s);
+        const long long sz = (long long)dk * dv;
+        ss2d_launch(la_join_fwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(N * H)), dim3(NT), 0, s, a, linattn_chunk(dtype, dk, dv));
+    }
+    dispatch<0>(dtype, a, gaps, s);
     rc = ss2d_take_launch_rc();
     if (rc) ss2d_set_error("linattn_fwd: launch failed: %s", hipGetErrorString((hipError_t)rc));
     return rc;

@@ -411,13 +411,13 @@ int ss2d_seg_loss_bwd(int dtype, const void *logits, const void *labels, int lab
  * cu_seqlens null: N sequences of `tokens` tokens, rows = N.  Else N + 1 non-decreasing row offsets (device memory, clamped to [0, tokens]) of
  * sequences packed into rows = 1 row; rows outside every sequence get zero outputs and gradients.  Sequences may be empty.
  * A decay below -150 (exp underflows in fp32; -inf: a reset) counts as -150.
- * Segments: a sequence is walked in nseg pieces of seg_chunks chunks (ss2d_linattn_segment_chunks, from the tokens of all sequences; nseg from the
- * longest one; the last piece takes the rest); nseg > 1 needs seg_states (N * H * nseg * dk * dv floats) and seg_decay (N * H * nseg doubles) as scratch memory.
+ * Segments: a sequence is walked in nseg pieces of seg_chunks chunks (ss2d_linattn_segments, from the tokens of all sequences and the longest one:
+ * nseg << 32 | seg_chunks; the last piece takes the rest); nseg > 1 needs seg_states (N * H * nseg * dk * dv floats) and seg_decay (N * H * nseg doubles) as scratch memory.
  * chunk_states (null: none): the forward leaves the state in front of every chunk of ss2d_linattn_chunk(dtype, dk, dv) tokens there for the backward:
  * slots * H * ss2d_linattn_state_floats(dtype, dk, dv) floats with slots = N * ceil(tokens / chunk), packed: tokens / chunk + N. */
 long long ss2d_linattn_state_floats(int dtype, int dk, int dv);
 int ss2d_linattn_chunk(int dtype, int dk, int dv);
-int ss2d_linattn_segment_chunks(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward);
+long long ss2d_linattn_segments(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward);
 int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const void *v, const float *g, const long long *strides, const int *cu_seqlens,
                      const float *s0 /* (N, H, dk, dv) or null: 0 */, void *out /* (rows, tokens, H, dv) */, float *last /* (N, H, dk, dv) or null */,
                      float *chunk_states, float *seg_states, double *seg_decay, int N, long long tokens, int H, int G, int dk, int dv, float scale,

@@ -74,7 +74,7 @@ _SIGNATURES = {
     "ss2d_layernorm_merge_bwd": (_i, [_i, _i] + [_vp] * 8 + [ctypes.c_longlong, _i, _i, _i, _vp]),
     "ss2d_linattn_chunk": (_i, [_i, _i, _i]),
     "ss2d_linattn_state_floats": (ctypes.c_longlong, [_i, _i, _i]),
-    "ss2d_linattn_segment_chunks": (_i, [_i, ctypes.c_longlong, ctypes.c_longlong, _i, _i, _i, _i]),
+    "ss2d_linattn_segments": (ctypes.c_longlong, [_i, ctypes.c_longlong, ctypes.c_longlong, _i, _i, _i, _i]),
     "ss2d_linattn_fwd": (_i, [_i] + [_vp] * 12 + [_i, ctypes.c_longlong, _i, _i, _i, _i, ctypes.c_float, _i, _i, _vp]),
     "ss2d_linattn_bwd": (_i, [_i] + [_vp] * 18 + [_i, ctypes.c_longlong, _i, _i, _i, _i, ctypes.c_float, _i, _i, _vp]),
     "ss2d_linattn_step": (_i, [_i] + [_vp] * 7 + [_i, _vp, ctypes.c_longlong, ctypes.c_longlong] + [_i] * 5 + [ctypes.c_float, _vp]),
@@ -146,6 +146,13 @@ def on_device(dev):
     if idx is None or idx == torch.cuda.current_device():
         return _NO_CTX
     return torch.cuda.device(dev)
+
+
+def stream_of(index):
+    """Raw handle of torch's current stream on device `index` when that is the current device, else None (the caller then enters
+    torch.cuda.device(index)).  For operators whose time is the host's: no context manager, no Stream object."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index) if torch._C._cuda_getDevice() == index else None
 
 
 def stream():

@@ -239,16 +239,18 @@ __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_a
 // tokens of a chunk: the backward holds q, k, v, dout, a dk x dv state and two C x C matrices in 160 KB of LDS
 inline int linattn_chunk(int dtype, int dk, int dv) { return dtype || (dk <= 64 && dv <= 64) ? 64 : 32; }
 
-// Chunks a segment.  One workgroup walks a segment; with fewer workgroups than the card holds at once (two or three a CU) it idles, and a segment
+// Segments.  One workgroup walks a segment; with fewer workgroups than the card holds at once (two or three a CU) it idles, and a segment
 // costs a second pass over k and v (q and dout in the backward) and a state's round trip: so all tokens of all sequences and
 // heads are dealt to that many workgroups, at least four chunks each.
-inline int linattn_segment_chunks(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
+// Returns the segments of the longest sequence in the upper and the chunks a segment in the lower 32 bits.
+inline long long linattn_segments(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
     const int C = linattn_chunk(dtype, dk, dv);
     const long long nch = (max_len + C - 1) / C, all = (all_tokens + C - 1) / C * H * (backward || dtype ? 1 : (dv + 63) / 64);
     const long long wgs = dtype && !backward && dv <= 64 ? 768 : 512;
     long long segc = (all + wgs - 1) / wgs;
     if (segc < 4) segc = 4;
-    return (int)(segc < nch ? segc : nch > 0 ? nch : 1);
+    if (segc >= nch) return (1LL << 32) | (nch > 0 ? nch : 1);
+    return (nch + segc - 1) / segc << 32 | segc;
 }
 
 // floats of one chunk's saved state.  bf16 kernels: accumulator order, padded to whole tiles (16-byte pieces of a wave side by side)

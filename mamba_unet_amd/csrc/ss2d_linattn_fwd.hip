@@ -514,8 +514,8 @@ void linattn_segment_pass(int dtype, const linattn::Problem &p, float *seg_state
 
 extern "C" int ss2d_linattn_chunk(int dtype, int dk, int dv) { return linattn_chunk(dtype, dk, dv); }
 extern "C" long long ss2d_linattn_state_floats(int dtype, int dk, int dv) { return linattn_state_floats(dtype, dk, dv); }
-extern "C" int ss2d_linattn_segment_chunks(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
-    return all_tokens >= 0 && max_len >= 0 && H > 0 ? linattn_segment_chunks(dtype, all_tokens, max_len, H, dk, dv, backward) : 1;
+extern "C" long long ss2d_linattn_segments(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
+    return all_tokens >= 0 && max_len >= 0 && H > 0 ? linattn_segments(dtype, all_tokens, max_len, H, dk, dv, backward) : 1LL << 32 | 1;
 }
 
 extern "C" int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const void *v, const float *g, const long long *strides,

@@ -6,7 +6,7 @@
 many requests whose states lie in a pool.  Both run on the HIP kernels of libss2d_hip.so; CPU tensors are rejected."""
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
@@ -20,25 +20,44 @@ _MAX_DIM = 128
 def _operand(t, io):
     """t in the storage type, its last axis dense and, where the head size allows 16-byte accesses, everything aligned for them
     (a slice of a fused projection is used in place; a view at an odd offset is copied)."""
-    if t.dtype != io:
+    if t.dtype is not io:
         t = t.to(io)
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    n, s = t.shape[-1], t.stride()
+    if n > 1 and s[3] != 1:
         return t.contiguous()
-    if t.shape[-1] % 8 == 0 and (t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1])):
-        return t.contiguous() if not t.is_contiguous() else t.clone()
+    if n % 8 == 0 and (t.data_ptr() % 16 or (s[0] | s[1] | s[2]) % 8):
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
+def _storage(q, k, v):
+    return torch.bfloat16 if q.dtype is torch.bfloat16 and k.dtype is torch.bfloat16 and v.dtype is torch.bfloat16 else torch.float32
+
+
+def _fp32(t):
+    return t if t is None or t.dtype is torch.float32 else t.float()
+
+
+def _check_devices(name, **tensors):
+    """Raises for the first tensor that is not on the GPU, or on another one than the first."""
+    first = None
+    for n, t in tensors.items():
+        if t is not None:
+            if not t.is_cuda:
+                raise RuntimeError(f"{name}: `{n}` must be a GPU tensor (no CPU path in mamba_unet_amd)")
+            first = first or (n, t.device)
+            if t.device != first[1]:
+                raise ValueError(f"{name}: `{n}` is on {t.device}, {first[0]} on {first[1]}")
+
+
 def _check(q, k, v, log_decay, initial_state, cu_seqlens):
-    for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("initial_state", initial_state), ("cu_seqlens", cu_seqlens)):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"linear_attention_fn: `{name}` must be a GPU tensor (no CPU path in mamba_unet_amd)")
-        if t.device != q.device:
-            raise ValueError(f"linear_attention_fn: `{name}` is on {t.device}, q on {q.device}")
-        if name != "cu_seqlens" and not t.is_floating_point():
-            raise ValueError(f"linear_attention_fn: `{name}` must be a floating-point tensor, got {t.dtype}")
+    d = q.get_device()
+    if d < 0 or k.get_device() != d or v.get_device() != d or log_decay.get_device() != d or (initial_state is not None and initial_state.get_device() != d) \
+            or (cu_seqlens is not None and cu_seqlens.get_device() != d):
+        _check_devices("linear_attention_fn", q=q, k=k, v=v, log_decay=log_decay, initial_state=initial_state, cu_seqlens=cu_seqlens)
+    if not (q.is_floating_point() and k.is_floating_point() and v.is_floating_point() and log_decay.is_floating_point()) \
+            or (initial_state is not None and not initial_state.is_floating_point()):
+        raise ValueError("linear_attention_fn: q, k, v, log_decay and initial_state must be floating-point tensors")
     if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2]:
         raise ValueError(f"q/k must be (batch, L, groups, dk) and equal, v (batch, L, heads, dv): {tuple(q.shape)} / {tuple(k.shape)} / {tuple(v.shape)}")
     B, L, G, dk = q.shape
@@ -61,21 +80,27 @@ def _check(q, k, v, log_decay, initial_state, cu_seqlens):
     return B, L, G, dk, H, dv, N
 
 
+_TWELVE, _EIGHT = struct.Struct("12q").pack, struct.Struct("8q").pack
+
+
 def _strides(q, k, v, g):
     """The host array of twelve strides (batch, token, head of q, k, v, g); a decay for each head only has stride 0 over tokens."""
     gs = (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
-    return (ctypes.c_longlong * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *gs)
+    return _TWELVE(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *gs)
 
 
 def _segments(lib, dev, code, N, tokens, H, longest, dk, dv, backward):
     """(segments, chunks a segment, state scratch, decay scratch)"""
-    C = lib.ss2d_linattn_chunk(code, dk, dv)
-    segc = lib.ss2d_linattn_segment_chunks(code, tokens, longest, H, dk, dv, backward)
-    nseg = max(1, -(-(-(-longest // C)) // segc))
+    plan = lib.ss2d_linattn_segments(code, tokens, longest, H, dk, dv, backward)
+    nseg, segc = plan >> 32, plan & 0xffffffff
     if nseg == 1:
         return 1, segc, None, None
     return (nseg, segc, torch.empty((N, H, nseg, dk, dv), device=dev, dtype=torch.float32),
             torch.empty((N, H, nseg), device=dev, dtype=torch.float64))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _forward(q, k, v, g, s0, cu, scale, dims, longest, want_last, want_chunks):
@@ -89,26 +114,31 @@ def _forward(q, k, v, g, s0, cu, scale, dims, longest, want_last, want_chunks):
             last.zero_() if s0 is None else last.copy_(s0)
         return out, last, None
     lib = _lib.load()
-    code = _BF16 if io == torch.bfloat16 else _F32
+    code = _BF16 if io is torch.bfloat16 else _F32
     chunks = None
     if want_chunks:
         C = lib.ss2d_linattn_chunk(code, dk, dv)
         slots = N * -(-L // C) if cu is None else L // C + N
         chunks = torch.empty((slots, H, lib.ss2d_linattn_state_floats(code, dk, dv)), device=dev, dtype=torch.float32)
     nseg, segc, ws, wd = _segments(lib, dev, code, N, B * L, H, longest, dk, dv, 0)
-    p = _lib.ptr
-    with _lib.on_device(dev):
-        rc = lib.ss2d_linattn_fwd(code, p(q), p(k), p(v), p(g), _strides(q, k, v, g), p(cu), p(s0), p(out), p(last),
-                                  p(chunks), p(ws), p(wd), N, L, H, G, dk, dv, scale, nseg, segc, _lib.stream())
-    _lib.check(rc, "ss2d_linattn_fwd")
+    args = (code, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), _strides(q, k, v, g), _ptr(cu), _ptr(s0), out.data_ptr(), _ptr(last), _ptr(chunks),
+            _ptr(ws), _ptr(wd), N, L, H, G, dk, dv, scale, nseg, segc)
+    stream = _lib.stream_of(dev.index)
+    if stream is None:
+        with torch.cuda.device(dev):
+            rc = lib.ss2d_linattn_fwd(*args, _lib.stream())
+    else:
+        rc = lib.ss2d_linattn_fwd(*args, stream)
+    if rc:
+        _lib.check(rc, "ss2d_linattn_fwd")
     return out, last, chunks
 
 
 class LinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial_state, cu_seqlens, scale, dims, longest, want_last):
-        io = torch.bfloat16 if q.dtype == k.dtype == v.dtype == torch.bfloat16 else torch.float32
-        q_, k_, v_, g_ = _operand(q, io), _operand(k, io), _operand(v, io), log_decay.float()
+        io = _storage(q, k, v)
+        q_, k_, v_, g_ = _operand(q, io), _operand(k, io), _operand(v, io), _fp32(log_decay)
         s0 = None if initial_state is None else initial_state.float().contiguous()
         ctx.set_materialize_grads(False)
         out, last, chunks = _forward(q_, k_, v_, g_, s0, cu_seqlens, scale, dims, longest, want_last, True)
@@ -169,14 +199,16 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, cu_s
     longest = L if cu_seqlens is None or max_seqlen is None else min(L, max(1, int(max_seqlen)))
     if N == 0:
         raise ValueError("linear_attention_fn: empty batch")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, initial_state)):
-        return LinearAttentionFn.apply(q, k, v, log_decay, initial_state, cu_seqlens, scale, dims, longest, bool(return_last_state))
-    io = torch.bfloat16 if q.dtype == k.dtype == v.dtype == torch.bfloat16 else torch.float32
-    s0 = None if initial_state is None else initial_state.float().contiguous()
-    out, last, _ = _forward(_operand(q, io), _operand(k, io), _operand(v, io), log_decay.float(), s0, cu_seqlens, scale, dims, longest,
-                            bool(return_last_state), False)
-    out = out.to(v.dtype)
-    return (out, last) if return_last_state else out
+    want_last = bool(return_last_state)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or (initial_state is not None and initial_state.requires_grad)):
+        return LinearAttentionFn.apply(q, k, v, log_decay, initial_state, cu_seqlens, scale, dims, longest, want_last)
+    io = _storage(q, k, v)
+    s0 = None if initial_state is None else _fp32(initial_state).contiguous()
+    out, last, _ = _forward(_operand(q, io), _operand(k, io), _operand(v, io), _fp32(log_decay), s0, cu_seqlens, scale, dims, longest, want_last, False)
+    if out.dtype is not v.dtype:
+        out = out.to(v.dtype)
+    return (out, last) if want_last else out
 
 
 def linear_attention_step(state, q, k, v, log_decay, scale=None, state_indices=None):
@@ -186,49 +218,64 @@ def linear_attention_step(state, q, k, v, log_decay, scale=None, state_indices=N
     (b, h); scale defaults to dk ** -0.5.  state_indices (b,) int32 or int64: the slot of each request (default: slot = request).  An index outside the
     pool, -1 for instance, marks a padded request: it gives zeros and changes no state.  Requests that name the same slot are applied in
     their order.  States as linear_attention_fn returns them.  For serving: no gradients."""
-    for name, t in (("state", state), ("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("state_indices", state_indices)):
-        if t is not None:
-            if not t.is_cuda:
-                raise RuntimeError(f"linear_attention_step: `{name}` must be a GPU tensor (no CPU path in mamba_unet_amd)")
-            if t.device != state.device:
-                raise ValueError(f"linear_attention_step: `{name}` is on {t.device}, state on {state.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (state, q, k, v, log_decay)):
+    d = state.get_device()
+    if d < 0 or q.get_device() != d or k.get_device() != d or v.get_device() != d or log_decay.get_device() != d \
+            or (state_indices is not None and state_indices.get_device() != d):
+        _check_devices("linear_attention_step", state=state, q=q, k=k, v=v, log_decay=log_decay, state_indices=state_indices)
+    if torch.is_grad_enabled() and (state.requires_grad or q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad):
         raise RuntimeError("linear_attention_step updates its state in place and has no gradient: call it under torch.no_grad(), or linear_attention_fn")
-    if q.dim() != 3 or k.shape != q.shape or v.dim() != 3 or v.shape[0] != q.shape[0]:
-        raise ValueError(f"q/k must be (b, groups, dk) and equal, v (b, heads, dv): {tuple(q.shape)} / {tuple(k.shape)} / {tuple(v.shape)}")
-    B, G, dk = q.shape
-    H, dv = v.shape[1:]
+    qs, vs, ss = q.shape, v.shape, state.shape
+    if len(qs) != 3 or k.shape != qs or len(vs) != 3 or vs[0] != qs[0]:
+        raise ValueError(f"q/k must be (b, groups, dk) and equal, v (b, heads, dv): {tuple(qs)} / {tuple(k.shape)} / {tuple(vs)}")
+    B, G, dk = qs
+    _, H, dv = vs
     if G == 0 or H == 0 or H % G:
         raise ValueError(f"{H} heads are not a multiple of {G} key heads")
     if not (1 <= dk <= _MAX_DIM and 1 <= dv <= _MAX_DIM):
         raise ValueError(f"dk {dk} and dv {dv} must lie in 1 ... {_MAX_DIM}")
-    if state.dtype != torch.float32 or state.dim() != 4 or state.shape[1:] != (H, dk, dv):
-        raise ValueError(f"state must be fp32 (slots, {H}, {dk}, {dv}), got {state.dtype} {tuple(state.shape)}")
-    pool = state.shape[0]
-    n = H * dk * dv
-    if pool and not (state[0].is_contiguous() and (pool == 1 or state.stride(0) >= n)):
+    if state.dtype is not torch.float32 or len(ss) != 4 or ss[1] != H or ss[2] != dk or ss[3] != dv:
+        raise ValueError(f"state must be fp32 (slots, {H}, {dk}, {dv}), got {state.dtype} {tuple(ss)}")
+    pool, n = ss[0], H * dk * dv
+    pitch, *inner = state.stride()
+    if pool and (inner != [dk * dv, dv, 1] and not state[0].is_contiguous() or pool > 1 and pitch < n):
         raise ValueError("the slots of state must be dense and must not overlap: it is updated in place")
-    if log_decay.shape not in ((H,), (B, H)):
-        raise ValueError(f"log_decay must be ({H},) or {(B, H)}, got {tuple(log_decay.shape)}")
+    gs = log_decay.shape
+    if gs != (H,) and gs != (B, H):
+        raise ValueError(f"log_decay must be ({H},) or {(B, H)}, got {tuple(gs)}")
+    slots, wide = None, 0
     if state_indices is None:
         if pool != B:
             raise ValueError(f"{B} requests and {pool} states: give state_indices")
-    elif state_indices.shape != (B,) or state_indices.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"state_indices must be ({B},) int32 or int64, got {state_indices.dtype} {tuple(state_indices.shape)}")
-    io = torch.bfloat16 if q.dtype == k.dtype == v.dtype == torch.bfloat16 else torch.float32
-    dense = lambda t: t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()  # noqa: E731
-    q_, k_, v_, g_ = dense(q.to(io)), dense(k.to(io)), dense(v.to(io)), log_decay.float()
-    out = torch.empty((B, H, dv), device=state.device, dtype=io)
+    else:
+        wide = int(state_indices.dtype is torch.int64)
+        if state_indices.shape != (B,) or not (wide or state_indices.dtype is torch.int32):
+            raise ValueError(f"state_indices must be ({B},) int32 or int64, got {state_indices.dtype} {tuple(state_indices.shape)}")
+        slots = state_indices.contiguous()
+    io = _storage(q, k, v)
+    q_, k_, v_, g_ = _token(q, io), _token(k, io), _token(v, io), _fp32(log_decay)
+    dev = state.device
+    out = torch.empty((B, H, dv), device=dev, dtype=io)
     if B == 0 or pool == 0:
         return out.zero_().to(v.dtype)
-    idx = None if state_indices is None else state_indices.contiguous()
-    strides = (ctypes.c_longlong * 8)(q_.stride(0), q_.stride(1), k_.stride(0), k_.stride(1), v_.stride(0), v_.stride(1),
-                                      *((0, g_.stride(0)) if g_.dim() == 1 else g_.stride()))
-    lib, p = _lib.load(), _lib.ptr
-    with _lib.on_device(state.device):
-        rc = lib.ss2d_linattn_step(_BF16 if io == torch.bfloat16 else _F32, p(state), p(q_), p(k_), p(v_), p(g_), strides, p(idx),
-                                   int(idx is not None and idx.dtype == torch.int64), p(out), pool, max(n, state.stride(0)), B, H, G, dk, dv,
-                                   float(dk ** -0.5 if scale is None else scale), _lib.stream())
-    _lib.check(rc, "ss2d_linattn_step")
-    torch.autograd.graph.increment_version(state)
-    return out if out.dtype == v.dtype else out.to(v.dtype)
+    strides = _EIGHT(*q_.stride()[:2], *k_.stride()[:2], *v_.stride()[:2], *((0, g_.stride(0)) if len(gs) == 1 else g_.stride()))
+    lib = _lib.load()
+    args = (_BF16 if io is torch.bfloat16 else _F32, state.data_ptr(), q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), g_.data_ptr(), strides, _ptr(slots), wide,
+            out.data_ptr(), pool, max(n, pitch), B, H, G, dk, dv, float(dk ** -0.5 if scale is None else scale))
+    stream = _lib.stream_of(d)
+    if stream is None:
+        with torch.cuda.device(dev):
+            rc = lib.ss2d_linattn_step(*args, _lib.stream())
+    else:
+        rc = lib.ss2d_linattn_step(*args, stream)
+    if rc:
+        _lib.check(rc, "ss2d_linattn_step")
+    if not state.is_inference():                # (tensors made under inference_mode have no version)
+        torch._C._increment_version((state,))
+    return out if io is v.dtype else out.to(v.dtype)
+
+
+def _token(t, io):
+    """t in the storage type with a dense last axis"""
+    if t.dtype is not io:
+        t = t.to(io)
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()

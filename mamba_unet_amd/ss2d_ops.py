@@ -781,30 +781,48 @@ def _norm_rows(t, io, D):
     return t, ld
 
 
+def _fp32_param(t):
+    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
+
+
+def _norm_gate_residual(x, y, z, w1, b1, a, w2, b2, drop, eps, rms, want_stats):
+    """One forward pass: (x', h) in the storage types, the statistics (or None) and what the backward needs."""
+    D = x.shape[-1]
+    rows = x.numel() // D
+    (rt, rcode), (io, code) = _io(x), _io(y)
+    (x_, ldx), (y_, ldy) = _norm_rows(x, rt, D), _norm_rows(y, io, D)
+    z_, ldz = (None, D) if z is None else _norm_rows(z, io, D)
+    w1_, b1_, a_, w2_, b2_, drop_ = _fp32_param(w1), _fp32_param(b1), _fp32_param(a), _fp32_param(w2), _fp32_param(b2), _fp32_param(drop)
+    dev = x.device
+    x_out, h = torch.empty(x.shape, device=dev, dtype=rt), torch.empty(x.shape, device=dev, dtype=io)
+    stats = torch.empty((rows, 4), device=dev, dtype=torch.float32) if want_stats else None
+    rps = rows // drop.numel() if drop is not None and drop.numel() else 0
+    if rows:
+        p = _data_ptr
+        args = (rcode, code, x_.data_ptr(), y_.data_ptr(), p(z_), w1_.data_ptr(), p(b1_), w2_.data_ptr(), p(b2_), p(a_), p(drop_), rps, x_out.data_ptr(),
+                h.data_ptr(), p(stats), rows, D, ldx, ldy, ldz, eps, rms)
+        stream = _lib.stream_of(dev.index)
+        if stream is None:
+            with torch.cuda.device(dev):
+                rc = _lib.load().ss2d_block_norm_fwd(*args, _stream())
+        else:
+            rc = _lib.load().ss2d_block_norm_fwd(*args, stream)
+        if rc:
+            _lib.check(rc, "ss2d_block_norm_fwd")
+    return x_out, h, stats, (x_, y_, z_, w1_, b1_, a_, w2_, drop_), (rcode, code, D, ldx, ldy, ldz, rps, rms, rows)
+
+
+def _data_ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 class _NormGateResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, z, w1, b1, a, w2, b2, drop, eps, rms):
         ctx.set_materialize_grads(False)
-        D = x.shape[-1]
-        rows = x.numel() // D
-        (rt, rcode), (io, code) = _io(x), _io(y)
-        (x_, ldx), (y_, ldy) = _norm_rows(x, rt, D), _norm_rows(y, io, D)
-        z_, ldz = (None, D) if z is None else _norm_rows(z, io, D)
-        f32 = lambda t: None if t is None else t.detach().float().contiguous()  # noqa: E731
-        w1_, b1_, a_, w2_, b2_, drop_ = f32(w1), f32(b1), f32(a), f32(w2), f32(b2), f32(drop)
-        x_out, h = torch.empty(x.shape, device=x.device, dtype=rt), torch.empty(x.shape, device=x.device, dtype=io)
-        stats = torch.empty((rows, 4), device=x.device, dtype=torch.float32) if any(ctx.needs_input_grad) else None
-        rps = rows // drop.numel() if drop is not None and drop.numel() else 0
-        ctx.rows = rows
-        if rows:
-            p = _lib.ptr
-            with _lib.on_device(x.device):
-                rc = _lib.load().ss2d_block_norm_fwd(rcode, code, p(x_), p(y_), p(z_), p(w1_), p(b1_), p(w2_), p(b2_), p(a_), p(drop_), rps, p(x_out), p(h),
-                                                     p(stats), rows, D, ldx, ldy, ldz, float(eps), int(rms), _stream())
-            _lib.check(rc, "ss2d_block_norm_fwd")
-        if stats is not None:
-            ctx.save_for_backward(x_, y_, z_, w1_, b1_, a_, w2_, drop_, stats)
-        ctx.meta = (rcode, code, D, ldx, ldy, ldz, rps, int(rms), x.shape, [None if t is None else t.dtype for t in (x, y, z, w1, b1, a, w2, b2)])
+        x_out, h, stats, saved, meta = _norm_gate_residual(x, y, z, w1, b1, a, w2, b2, drop, eps, rms, True)
+        ctx.save_for_backward(*saved, stats)
+        ctx.meta = meta + (x.shape, [None if t is None else t.dtype for t in (x, y, z, w1, b1, a, w2, b2)])
         return x_out.to(x.dtype), h.to(y.dtype)
 
     @staticmethod
@@ -813,8 +831,8 @@ class _NormGateResidual(torch.autograd.Function):
         if dx_out is None and dh is None:
             return (None,) * 11
         x, y, z, w1, b1, a, w2, drop, stats = ctx.saved_tensors
-        rcode, code, D, ldx, ldy, ldz, rps, rms, shape, dt = ctx.meta
-        dev, rows = x.device, ctx.rows
+        rcode, code, D, ldx, ldy, ldz, rps, rms, rows, shape, dt = ctx.meta
+        dev = x.device
         aligned = lambda t: t.clone() if t is not None and t.data_ptr() % 16 else t  # noqa: E731
         gx = aligned(None if dx_out is None else dx_out.to(x.dtype).contiguous())
         gh = aligned(None if dh is None else dh.to(y.dtype).contiguous())
@@ -844,22 +862,30 @@ def norm_gate_residual(x, y, post_weight, pre_weight, post_bias=None, pre_bias=N
     with `rms`; statistics in fp32, h from the unrounded x'.  z (y's shape; a channel slice of a wider tensor is read in place), the biases,
     res_scale (D,) and drop_scale (one factor per sample, not differentiated) are optional.  bf16 x and y / z stay bf16 in memory (x may be fp32 with a bf16
     branch); D <= 8192."""
-    for name, t in (("x", x), ("y", y), ("z", z), ("post_weight", post_weight), ("pre_weight", pre_weight), ("post_bias", post_bias), ("pre_bias", pre_bias),
-                    ("res_scale", res_scale), ("drop_scale", drop_scale)):
+    named = (("x", x), ("y", y), ("post_weight", post_weight), ("pre_weight", pre_weight), ("z", z), ("post_bias", post_bias), ("pre_bias", pre_bias),
+             ("res_scale", res_scale), ("drop_scale", drop_scale))
+    shape, dev, need = x.shape, x.get_device(), False
+    if not shape or not 1 <= shape[-1] <= 8192:
+        raise ValueError(f"norm_gate_residual: the last axis must hold 1 ... 8192 channels, got {tuple(shape)}")
+    vec = shape[-1:]
+    for name, t in named:
         if t is None:
             continue
-        _need_gpu(t, f"norm_gate_residual: `{name}`")
-        if t.device != x.device:
+        if t.get_device() != dev or dev < 0:
+            _need_gpu(t, f"norm_gate_residual: `{name}`")
+            _need_gpu(x, "norm_gate_residual: `x`")
             raise ValueError(f"norm_gate_residual: `{name}` is on {t.device}, x on {x.device}")
-        if name in ("y", "z") and t.shape != x.shape:
-            raise ValueError(f"norm_gate_residual: `{name}` must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
-        if name not in ("x", "y", "z", "drop_scale") and t.shape != x.shape[-1:]:
-            raise ValueError(f"norm_gate_residual: `{name}` must be ({x.shape[-1]},), got {tuple(t.shape)}")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
-        raise ValueError(f"norm_gate_residual: the last axis must hold 1 ... 8192 channels, got {tuple(x.shape)}")
-    if drop_scale is not None and (x.dim() < 2 or drop_scale.numel() != x.shape[0]):
+        if name == "drop_scale":
+            continue
+        if t.shape != (shape if name in ("x", "y", "z") else vec):
+            raise ValueError(f"norm_gate_residual: `{name}` must be {tuple(shape if name in ('x', 'y', 'z') else vec)}, got {tuple(t.shape)}")
+        need = need or t.requires_grad
+    if drop_scale is not None and (len(shape) < 2 or drop_scale.numel() != shape[0]):
         raise ValueError("norm_gate_residual: `drop_scale` must hold one factor per sample")
-    return _NormGateResidual.apply(x, y, z, post_weight, post_bias, res_scale, pre_weight, pre_bias, drop_scale, eps, bool(rms))
+    if need and torch.is_grad_enabled():
+        return _NormGateResidual.apply(x, y, z, post_weight, post_bias, res_scale, pre_weight, pre_bias, drop_scale, float(eps), int(bool(rms)))
+    x_out, h = _norm_gate_residual(x, y, z, post_weight, post_bias, res_scale, pre_weight, pre_bias, drop_scale, float(eps), int(bool(rms)), False)[:2]
+    return x_out if x_out.dtype is x.dtype else x_out.to(x.dtype), h if h.dtype is y.dtype else h.to(y.dtype)
 
 
 class _LayerNorm(torch.autograd.Function):

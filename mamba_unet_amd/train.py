@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import os as _os
 from array import array
+from operator import attrgetter
 
 import torch
 import torch.nn.functional as F
@@ -147,6 +148,9 @@ def set_lr(optimizer, lr: float):
             g["lr"] = lr
 
 
+_dtype_of = attrgetter("dtype")
+
+
 def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """Scales the gradients in place by min(1, max_norm / (norm + 1e-6)) with their global norm (2 or inf) and returns the norm, a 0-dim
     fp32 tensor: what torch.nn.utils.clip_grad_norm_ computes, without a host read of the norm (so it can be captured in a HIP graph) and in two
@@ -154,8 +158,10 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tens
     GPU, none sharing memory with another.  The norm is summed in 64 bits in a fixed order; one that is not a number makes every
     gradient not a number.  max_norm = inf only measures."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    grads = [g.grad if type(g) is torch.nn.Parameter else g for g in grads]
-    grads = [g for g in grads if g is not None]
+    kinds = set(map(type, grads))
+    if torch.nn.Parameter in kinds or type(None) in kinds:
+        grads = [g.grad if type(g) is torch.nn.Parameter else g for g in grads]
+        grads = [g for g in grads if g is not None]
     max_norm, norm_type = float(max_norm), float(norm_type)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm: max_norm must be >= 0, got {max_norm}")
@@ -163,13 +169,13 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tens
         raise ValueError(f"clip_grad_norm: norm_type must be 2 or inf, got {norm_type}")
     if not grads:
         return torch.tensor(0.0)
-    devs, types = set(map(torch.Tensor.get_device, grads)), [g.dtype for g in grads]
+    devs, types = set(map(torch.Tensor.get_device, grads)), set(map(_dtype_of, grads))
     if min(devs) < 0:
         raise RuntimeError("clip_grad_norm: GPU tensors required (no CPU path in mamba_unet_amd)")
     if len(devs) > 1:
         raise ValueError(f"clip_grad_norm: gradients on several devices: {sorted(devs)}")
-    if not set(types) <= {torch.float32, torch.bfloat16}:
-        raise ValueError(f"clip_grad_norm: fp32 or bf16 gradients required, got {set(types)}")
+    if not types <= {torch.float32, torch.bfloat16}:
+        raise ValueError(f"clip_grad_norm: fp32 or bf16 gradients required, got {types}")
     dev = grads[0].device
     work = grads
     if not all(map(torch.Tensor.is_contiguous, grads)):
@@ -179,21 +185,27 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tens
     lib = _lib.load()
     ptrs = array("Q", map(torch.Tensor.data_ptr, work))
     sizes = array("q", map(torch.Tensor.numel, work))
-    kinds = bytes([t is torch.bfloat16 for t in types])
+    is_bf16 = bytes([t.dtype is torch.bfloat16 for t in grads]) if len(types) > 1 else (b"\1" if torch.bfloat16 in types else b"\0") * n
     nbytes = lib.ss2d_grad_clip_workspace_bytes(n)
     norm = torch.empty((), device=dev, dtype=torch.float32)
     ws = torch.empty(nbytes // 8, device=dev, dtype=torch.float64)
-    with _lib.on_device(dev):
-        rc = lib.ss2d_grad_clip(kinds, ptrs.buffer_info()[0], sizes.buffer_info()[0], n, int(norm_type != 2.0), max_norm, int(max_norm != float("inf")),
-                                norm.data_ptr(), ws.data_ptr(), nbytes, _lib.stream())
-    _lib.check(rc, "ss2d_grad_clip")
+    args = (is_bf16, ptrs.buffer_info()[0], sizes.buffer_info()[0], n, int(norm_type != 2.0), max_norm, int(max_norm != float("inf")), norm.data_ptr(),
+            ws.data_ptr(), nbytes)
+    stream = _lib.stream_of(dev.index)
+    if stream is None:
+        with torch.cuda.device(dev):
+            rc = lib.ss2d_grad_clip(*args, _lib.stream())
+    else:
+        rc = lib.ss2d_grad_clip(*args, stream)
+    if rc:
+        _lib.check(rc, "ss2d_grad_clip")
     if max_norm != float("inf"):
         if work is not grads:
             with torch.no_grad():
                 for g, w in zip(grads, work):
                     if w.data_ptr() != g.data_ptr():
                         g.copy_(w)
-        torch.autograd.graph.increment_version(grads)
+        torch._C._increment_version([g for g in grads if not g.is_inference()] if grads[0].is_inference() else grads)
     return norm
 
 

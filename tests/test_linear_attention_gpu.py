@@ -374,6 +374,17 @@ def test_step_on_a_layer_of_a_pool_and_strided_inputs():
     assert torch.equal(layers[:, 0], keep[:, 0]) and torch.equal(layers[:, 2], keep[:, 2])
 
 
+def test_step_and_prompt_under_inference_mode():
+    t = step_inputs(3, 0, 4, 2, 64, 64, "token", torch.bfloat16)
+    d = {n: None if x is None else x.cuda() for n, x in t.items()}
+    want = d["state"].clone()
+    out = linear_attention_step(want, d["q"], d["k"], d["v"], d["g"])
+    with torch.inference_mode():
+        state = d["state"].clone()
+        assert torch.equal(linear_attention_step(state, d["q"], d["k"], d["v"], d["g"]), out) and torch.equal(state, want)
+        assert linear_attention_fn(d["q"][:, None], d["k"][:, None], d["v"][:, None], d["g"][:, None], initial_state=d["state"]).shape == (3, 1, 4, 64)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 def test_prompt_then_tokens_equals_the_whole_sequence(dtype):
     """As a server uses them: packed prompts through linear_attention_fn into a pool, then tokens one by one, in a captured graph."""

@@ -11,7 +11,7 @@ import struct
 import torch
 
 from . import _lib
-from .ss2d_ops import colsum
+from .ss2d_ops import _dense16, colsum
 
 _F32, _BF16 = 0, 1          # include/ss2d.h: SS2D_DTYPE_F32 / SS2D_DTYPE_BF16
 _MAX_DIM = 128
@@ -160,27 +160,29 @@ class LinearAttentionFn(torch.autograd.Function):
             z = lambda *sh, dt: torch.zeros(sh, device=dev, dtype=dt)  # noqa: E731
             ds0 = None if not want_s0 else (z(N, H, dk, dv, dt=s_dt) if dlast is None else dlast.to(s_dt))
             return z(B, L, G, dk, dt=q_dt), z(B, L, G, dk, dt=k_dt), z(B, L, H, dv, dt=v_dt), z(*g.shape, dt=g_dt), ds0, None, None, None, None, None
-        go = torch.zeros((B, L, H, dv), device=dev, dtype=io) if dout is None else dout.to(io).contiguous()
-        if go.data_ptr() % 16:
-            go = go.clone()
-        gl = None if dlast is None else dlast.float().contiguous()
+        go = torch.zeros((B, L, H, dv), device=dev, dtype=io) if dout is None else _dense16(dout, io)
+        gl = None if dlast is None else _dense16(dlast, torch.float32)
         dq, dk_ = torch.empty((B, L, G, dk), device=dev, dtype=io), torch.empty((B, L, G, dk), device=dev, dtype=io)
         dv_ = torch.empty((B, L, H, dv), device=dev, dtype=io)
         dg = torch.empty((B, L, H), device=dev, dtype=torch.float32)
         ds0 = torch.empty((N, H, dk, dv), device=dev, dtype=torch.float32) if want_s0 else None
-        heads = [torch.empty((B, L, H, dk), device=dev, dtype=torch.float32) for _ in range(2)] if H > G else (None, None)
+        hq, hk = [torch.empty((B, L, H, dk), device=dev, dtype=torch.float32) for _ in range(2)] if H > G else (None, None)
         lib = _lib.load()
-        code = _BF16 if io == torch.bfloat16 else _F32
+        code = _BF16 if io is torch.bfloat16 else _F32
         nseg, segc, ws, wd = _segments(lib, dev, code, N, B * L, H, longest, dk, dv, 1)
-        p = _lib.ptr
-        with _lib.on_device(dev):
-            rc = lib.ss2d_linattn_bwd(code, p(q), p(k), p(v), p(g), _strides(q, k, v, g), p(cu), p(go), p(gl), p(chunks),
-                                      p(dq), p(dk_), p(dv_), p(dg), p(ds0), p(heads[0]), p(heads[1]), p(ws), p(wd), N, L, H, G, dk, dv, scale, nseg,
-                                      segc, _lib.stream())
-        _lib.check(rc, "ss2d_linattn_bwd")
+        args = (code, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), _strides(q, k, v, g), _ptr(cu), go.data_ptr(), _ptr(gl), chunks.data_ptr(),
+                dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(), dg.data_ptr(), _ptr(ds0), _ptr(hq), _ptr(hk), _ptr(ws), _ptr(wd), N, L, H, G, dk, dv, scale, nseg, segc)
+        stream = _lib.stream_of(dev.index)
+        if stream is None:
+            with torch.cuda.device(dev):
+                rc = lib.ss2d_linattn_bwd(*args, _lib.stream())
+        else:
+            rc = lib.ss2d_linattn_bwd(*args, stream)
+        if rc:
+            _lib.check(rc, "ss2d_linattn_bwd")
         if g.dim() == 1:        # a decay for each head: the sum over all tokens (in a fixed order, and right in a replayed graph)
             dg = colsum(dg.view(B * L, H)) if ctx.needs_input_grad[3] else None
-        cast = lambda t, d: None if t is None else t.to(d)  # noqa: E731
+        cast = lambda t, d: t if t is None or t.dtype is d else t.to(d)  # noqa: E731
         return cast(dq, q_dt), cast(dk_, k_dt), cast(dv_, v_dt), cast(dg, g_dt), cast(ds0, s_dt), None, None, None, None, None
 
 

@@ -832,24 +832,35 @@ class _NormGateResidual(torch.autograd.Function):
             return (None,) * 11
         x, y, z, w1, b1, a, w2, drop, stats = ctx.saved_tensors
         rcode, code, D, ldx, ldy, ldz, rps, rms, rows, shape, dt = ctx.meta
-        dev = x.device
-        aligned = lambda t: t.clone() if t is not None and t.data_ptr() % 16 else t  # noqa: E731
-        gx = aligned(None if dx_out is None else dx_out.to(x.dtype).contiguous())
-        gh = aligned(None if dh is None else dh.to(y.dtype).contiguous())
+        dev, p = x.device, _data_ptr
+        gx, gh = _dense16(dx_out, x.dtype), _dense16(dh, y.dtype)
         dx, dy = torch.empty(shape, device=dev, dtype=x.dtype), torch.empty(shape, device=dev, dtype=y.dtype)
         dz = None if z is None else torch.empty(shape, device=dev, dtype=y.dtype)
         if rows:
-            lib, p = _lib.load(), _lib.ptr
-            dp = torch.empty((5, D), device=dev, dtype=torch.float32)
-            ws = torch.empty(int(lib.ss2d_block_norm_bwd_workspace_floats(rows, D)), device=dev, dtype=torch.float32)
-            with _lib.on_device(dev):
-                rc = lib.ss2d_block_norm_bwd(rcode, code, p(gx), p(gh), p(x), p(y), p(z), p(w1), p(b1), p(w2), p(a), p(drop), rps, p(stats), p(dx), p(dy),
-                                             p(dz), p(dp), p(ws), rows, D, ldx, ldy, ldz, rms, _stream())
-            _lib.check(rc, "ss2d_block_norm_bwd")
+            lib = _lib.load()
+            n = lib.ss2d_block_norm_bwd_workspace_floats(rows, D)
+            dp, ws = torch.empty(5 * D, device=dev, dtype=torch.float32), torch.empty(n, device=dev, dtype=torch.float32)
+            args = (rcode, code, p(gx), p(gh), x.data_ptr(), y.data_ptr(), p(z), w1.data_ptr(), p(b1), w2.data_ptr(), p(a), p(drop), rps, stats.data_ptr(),
+                    dx.data_ptr(), dy.data_ptr(), p(dz), dp.data_ptr(), ws.data_ptr(), rows, D, ldx, ldy, ldz, rms)
+            stream = _lib.stream_of(dev.index)
+            if stream is None:
+                with torch.cuda.device(dev):
+                    rc = lib.ss2d_block_norm_bwd(*args, _stream())
+            else:
+                rc = lib.ss2d_block_norm_bwd(*args, stream)
+            if rc:
+                _lib.check(rc, "ss2d_block_norm_bwd")
         else:
-            dp = torch.zeros((5, D), device=dev, dtype=torch.float32)
-        grads = (dx, dy, dz, dp[0], dp[1], dp[2], dp[3], dp[4])
-        return tuple(g.to(d) if d is not None and n else None for g, d, n in zip(grads, dt, ctx.needs_input_grad)) + (None, None, None)
+            dp = torch.zeros(5 * D, device=dev, dtype=torch.float32)
+        grads = (dx, dy, dz, *dp.split(D))
+        return (*(None if d is None or not n else g if g.dtype is d else g.to(d) for g, d, n in zip(grads, dt, ctx.needs_input_grad)), None, None, None)
+
+
+def _dense16(g, dtype):
+    """g dense, in `dtype`, on a 16-byte boundary"""
+    if g is None or (g.dtype is dtype and g.is_contiguous() and g.data_ptr() % 16 == 0):
+        return g
+    return g.to(dtype).clone(memory_format=torch.contiguous_format)
 
 
 def norm_gate_residual(x, y, post_weight, pre_weight, post_bias=None, pre_bias=None, z=None, res_scale=None, drop_scale=None, eps: float = 1e-5,

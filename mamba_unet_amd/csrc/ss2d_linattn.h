@@ -234,6 +234,44 @@ struct TileRegsF {
     }
 };
 
+// Results of a chunk leave through a descriptor of its rows: rows past the last token and columns past D fall outside and are dropped, without a branch
+// that would split the products around it into pieces waiting for LDS one by one.
+struct RowsOut {
+    __amdgpu_buffer_rsrc_t rs;
+    template <typename T>
+    __device__ __forceinline__ RowsOut(T *base, int n, long long ld) : rs(make_rsrc(base, (unsigned)(n * (int)ld * (int)sizeof(T)))) {}
+    // four columns c .. c + 3 of row r (VEC: all four or none inside)
+    template <bool VEC>
+    __device__ __forceinline__ void put4(bf16 *, int r, int c, long long ld, int D, f4 v) const {
+        const u32x2 w = __builtin_bit_cast(u32x2, round4(v));
+        const int off = (r * (int)ld + c) * 2;
+        if (VEC) {
+            __builtin_amdgcn_raw_buffer_store_b64(w, rs, c < D ? off : SS2D_BUF_OOR, 0, 0);
+        } else {
+            const unsigned a = w.x, b = w.y;
+            const unsigned short h[4] = {(unsigned short)a, (unsigned short)(a >> 16), (unsigned short)b, (unsigned short)(b >> 16)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) __builtin_amdgcn_raw_buffer_store_b16(h[e], rs, c + e < D ? off + 2 * e : SS2D_BUF_OOR, 0, 0);
+        }
+    }
+    template <bool VEC>
+    __device__ __forceinline__ void put4(float *, int r, int c, long long ld, int D, f4 v) const {
+        const int off = (r * (int)ld + c) * 4;
+        if (VEC) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, c < D ? off : SS2D_BUF_OOR, 0, 0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = v[e];
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), rs, c + e < D ? off + 4 * e : SS2D_BUF_OOR, 0, 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void put1(float v, int r, int c, long long ld, int D) const {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rs, c < D ? (r * (int)ld + c) * 4 : SS2D_BUF_OOR, 0, 0);
+    }
+};
+
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // tokens of a chunk: the backward holds q, k, v, dout, a dk x dv state and two C x C matrices in 160 KB of LDS
@@ -265,6 +303,7 @@ inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, 
     if (N <= 0 || tokens <= 0 || tokens > 0x7fffff00LL || H <= 0 || G <= 0 || nseg <= 0 || segc <= 0) { ss2d_set_error("%s: size out of range", name); return -3; }
     if (H % G) { ss2d_set_error("%s: %d heads are not a multiple of %d key heads", name, H, G); return -4; }
     if (dk < 1 || dk > 128 || dv < 1 || dv > 128) { ss2d_set_error("%s: dk %d and dv %d must be 1 ... 128", name, dk, dv); return -5; }
+    if ((long long)H * dk >= (1 << 22) || (long long)H * dv >= (1 << 22)) { ss2d_set_error("%s: %d heads are too many", name, H); return -6; }
     if ((long long)N * H * nseg * 2 > 0x7ffffff0LL || (long long)N * H > 65535LL * 32) { ss2d_set_error("%s: too many sequences and heads", name); return -6; }
     p.q = q; p.k = k; p.v = v; p.g = g; p.cu = cu; p.tokens = tokens; p.N = N; p.H = H; p.G = G; p.dk = dk; p.dv = dv; p.scale = scale; p.nseg = nseg; p.segc = segc;
     p.qb = st[0]; p.ql = st[1]; p.qh = st[2]; p.kb = st[3]; p.kl = st[4]; p.kh = st[5];

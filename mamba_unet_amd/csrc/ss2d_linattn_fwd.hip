@@ -268,16 +268,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
     bf16 *O = static_cast<bf16 *>(a.o) + ((s.row * p.tokens + s.start + (long long)c0 * C) * p.H + h) * (long long)p.dv;
     const int col = 16 * wave + (lane0 & 15);
     f4 S[KT];
-    const float *init = MODE >= 1 ? nullptr : p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int k = 16 * t + 4 * (lane0 >> 4) + r;
-            S[t][r] = init && col < p.dv && k < p.dk ? init[k * p.dv + col] : 0.0f;
-        }
-    double total = 0.0;
-    f4 *saved = MODE == 0 && a.chunk_states ? reinterpret_cast<f4 *>(a.chunk_states) + ((chunk_base(p, s, n, C) + c0) * p.H + h) * (DK * DV / 4) + wave * KT * 64 + lane0 : nullptr;
     TileRegs<C, DK, NT, VEC> qr, kr;
     TileRegs<C, DV, NT, VEC> vr;
     qr.init(p.ql, p.dk);
@@ -294,6 +284,18 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
     auto fetch_g = [&](int c) {
         if (wave == 0 && c >= c0 && c < c1) gr = lane0 < rows_of(c) ? limit_decay(g[((long long)c * C + lane0) * p.gl]) : 0.0f;
     };
+    fetch_g(first);
+    if (c0 < c1) fetch(first);
+    const float *init = MODE >= 1 ? nullptr : p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int k = 16 * t + 4 * (lane0 >> 4) + r;
+            S[t][r] = init && col < p.dv && k < p.dk ? init[k * p.dv + col] : 0.0f;
+        }
+    double total = 0.0;
+    f4 *saved = MODE == 0 && a.chunk_states ? reinterpret_cast<f4 *>(a.chunk_states) + ((chunk_base(p, s, n, C) + c0) * p.H + h) * (DK * DV / 4) + wave * KT * 64 + lane0 : nullptr;
     auto scan = [&](int c) {
         if (wave == 0 && c >= c0 && c < c1) {
             float *d = decays + (c & 1) * 5 * C;
@@ -308,10 +310,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
         }
     };
     constexpr int STEP = MODE == 2 ? -1 : 1;
-    fetch_g(first);
     scan(first);
     fetch_g(first + STEP);
-    if (c0 < c1) fetch(first);
+    if (MODE == 0 && tid < 128) {                // the tiles of P behind the diagonal that are read with it (32 columns at a time): zero for good
+        const int i = 32 * (tid >> 6) + (tid & 15), at = i * PP + 2 * operand_pos(32 * (tid >> 6) + 16 + 4 * ((tid >> 4) & 3));
+        *reinterpret_cast<u32x2 *>(Ph + at) = u32x2{0, 0};
+        *reinterpret_cast<u32x2 *>(Pl + at) = u32x2{0, 0};
+    }
 #pragma unroll 1
     for (int c = first; c >= c0 && c < c1; c += STEP) {
         const int nr = rows_of(c);
@@ -329,29 +334,30 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
         const float *bh = decays + (c & 1) * 5 * C, *bl = bh + C, *eb = bl + C, *wt = eb + C, *tail = wt + C;
         __syncthreads();
         if (MODE == 0) {
-            // P[i][j] = scale exp(b_i - b_j) q_i . k_j, j <= i: four waves take a row tile each; eight take the even and the odd column tiles of one.  The
-            // tile behind the diagonal of an even row tile is zero: P is read 32 columns at a time
+            // P[i][j] = scale exp(b_i - b_j) q_i . k_j, j <= i: the ten 16 x 16 tiles are dealt to the waves and worked on side by side (a wave with one
+            // less repeats the last one: the same values)
             const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
-            const int it = NW == 8 ? wave >> 1 : wave, i = 16 * it + l16;
-            bf16x8 qf[KS];
+            constexpr int NTL = (10 + NW - 1) / NW;
+            f4 acc[NTL];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) qf[ks] = frag_p(Qs, QP, i, ks, gq);
-            const float hi = bh[i], li = bl[i];
-#pragma unroll 1
-            for (int jt = NW == 8 ? wave & 1 : 0; jt <= (it | 1); jt += NW == 8 ? 2 : 1) {
-                f4 acc = f4{0, 0, 0, 0};
-                if (jt <= it) {
+            for (int n = 0; n < NTL; ++n) {
+                const int t = wave + n * NW < 10 ? wave + n * NW : 9, it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
+                acc[n] = f4{0, 0, 0, 0};
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) acc = mfma8(frag(Ks, KP, 16 * jt + l16, ks, gq), qf[ks], acc);
-                    const f4 h4 = *reinterpret_cast<const f4 *>(bh + 16 * jt + 4 * gq), l4 = *reinterpret_cast<const f4 *>(bl + 16 * jt + 4 * gq);
+                for (int ks = 0; ks < KS; ++ks) acc[n] = mfma8(frag(Ks, KP, 16 * jt + l16, ks, gq), frag_p(Qs, QP, 16 * it + l16, ks, gq), acc[n]);
+            }
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[r] = 16 * jt + 4 * gq + r <= i ? acc[r] * p.scale * hw_exp2((hi - h4[r]) + (li - l4[r])) : 0.0f;
-                }
-                const bf16x4 x = round4(acc);
-                const int at = i * PP + 2 * operand_pos(16 * jt + 4 * gq);
+            for (int n = 0; n < NTL; ++n) {
+                const int t = wave + n * NW < 10 ? wave + n * NW : 9, it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
+                const int i = 16 * it + l16, j = 16 * jt + 4 * gq;
+                const float hi = bh[i], li = bl[i];
+                const f4 h4 = *reinterpret_cast<const f4 *>(bh + j), l4 = *reinterpret_cast<const f4 *>(bl + j);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[n][r] = j + r <= i ? acc[n][r] * p.scale * hw_exp2((hi - h4[r]) + (li - l4[r])) : 0.0f;
+                const bf16x4 x = round4(acc[n]);
+                const int at = i * PP + 2 * operand_pos(j);
                 *reinterpret_cast<bf16x4 *>(Ph + at) = x;
-                *reinterpret_cast<bf16x4 *>(Pl + at) = round4(rest4(acc, x));
+                *reinterpret_cast<bf16x4 *>(Pl + at) = round4(rest4(acc[n], x));
             }
             __syncthreads();
         }
@@ -375,8 +381,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
                 }
                 if (NW == 8) __builtin_amdgcn_sched_barrier(0);
             }
-            const int oc = 16 * wave + 4 * gq;
-            bf16 *o = O + l16 * ldo + oc;
+            const RowsOut out(O, nr, ldo);
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
                 acc[it] *= eb[16 * it + l16];
@@ -385,17 +390,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
                     acc[it] = mfma8(vf[js], frag_p(Ph, PP, 16 * it + l16, js, gq), acc[it]);
                     acc[it] = mfma8(vf[js], frag_p(Pl, PP, 16 * it + l16, js, gq), acc[it]);
                 }
-                if (16 * it + l16 < nr) {
-                    if (VEC) {
-                        if (oc < p.dv) st4(o, acc[it]);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (oc + r < p.dv) st1(o + r, acc[it][r]);
-                    }
-                }
-                o += 16 * ldo;
             }
+#pragma unroll
+            for (int it = 0; it < 4; ++it) out.template put4<VEC>(O, 16 * it + l16, 16 * wave + 4 * gq, ldo, p.dv, acc[it]);
             O += C * ldo;
         }
         __builtin_amdgcn_sched_barrier(0);

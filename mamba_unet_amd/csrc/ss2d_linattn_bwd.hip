@@ -288,11 +288,9 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
                 for (int r = 0; r < 4; ++r) y[r] = Ks[(16 * jt + 4 * gq + r) * PK + k];
                 dq = dot4(*reinterpret_cast<const f4 *>(Ys + (16 * qi + l16) * PP + 16 * jt + 4 * gq), y, dq);
             }
+            const RowsOut out(DQ, nr, ldq);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * qi + 4 * gq + r;
-                if (i < nr && k < p.dk) DQ[i * ldq + k] = dq[r];
-            }
+            for (int r = 0; r < 4; ++r) out.put1(dq[r], 16 * qi + 4 * gq + r, k, ldq, p.dk);
         }
         __syncthreads();                                              // D is there
         const float eend = tail[0];
@@ -320,11 +318,9 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
                 }
                 dk = dot4(x, y, dk);
             }
+            const RowsOut out(DKp, nr, ldq);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = 16 * qi + 4 * gq + r;
-                if (j < nr && k < p.dk) DKp[j * ldq + k] = dk[r];
-            }
+            for (int r = 0; r < 4; ++r) out.put1(dk[r], 16 * qi + 4 * gq + r, k, ldq, p.dk);
         }
         corner = lanes_sum<64>(corner);
         if (lane == 0) corners[wave] = corner;
@@ -348,11 +344,9 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
                 }
                 dv = dot4(x, y, dv);
             }
+            const RowsOut out(DVp, nr, ldv);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = 16 * vj + 4 * gq + r;
-                if (j < nr && col < p.dv) DVp[j * ldv + col] = dv[r];
-            }
+            for (int r = 0; r < 4; ++r) out.put1(dv[r], 16 * vj + 4 * gq + r, col, ldv, p.dv);
         }
         DQ -= C * ldq; DKp -= C * ldq; DVp -= C * ldv;
         scan(c - 1);
@@ -439,17 +433,6 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     const int kt = wave % KT, i0 = wave / KT * NI;                   // dq / dk: column tile, first row tile
     const int vt = wave % VT, j0 = wave / VT * NJ, kd = wave / VT * TW;           // dv: column tile, first row tile; D: first row tile
     f4 D[TW];
-    {
-        const int col = operand_index(16 * vt + (lane0 & 15));
-        const float *init = p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
-#pragma unroll
-        for (int t = 0; t < TW; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int k = 16 * (kd + t) + 4 * (lane0 >> 4) + r;
-                D[t][r] = init && col < p.dv && k < p.dk ? init[k * p.dv + col] : 0.0f;
-            }
-    }
     TileRegs<C, DK, NT, VEC> qr, kr;
     TileRegs<C, DV, NT, VEC> vr, orr;
     qr.init(p.ql, p.dk);
@@ -474,6 +457,19 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     auto fetch_g = [&](int c) {
         if (wave == 0 && c >= c0) gr = lane0 < rows_of(c) ? limit_decay(g[((long long)c * C + lane0) * p.gl]) : 0.0f;
     };
+    fetch_g(c1 - 1);
+    if (c0 < c1) fetch(c1 - 1);
+    {
+        const int col = operand_index(16 * vt + (lane0 & 15));
+        const float *init = p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
+#pragma unroll
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = 16 * (kd + t) + 4 * (lane0 >> 4) + r;
+                D[t][r] = init && col < p.dv && k < p.dk ? init[k * p.dv + col] : 0.0f;
+            }
+    }
     auto scan = [&](int c) {                                         // two chunks of: b (two terms), scale exp(b), exp(b_C - b), exp(b_C)
         if (wave == 0 && c >= c0) {
             float *d = decays + (c & 1) * 5 * C;
@@ -515,10 +511,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
             }
         }
     };
-    fetch_g(c1 - 1);
+    if (tid < 128) {                             // the tiles of X and Y behind the diagonal that are read with it (32 columns at a time): zero for good
+        const int i = 32 * (tid >> 6) + (tid & 15), at = i * PP + 2 * operand_pos(32 * (tid >> 6) + 16 + 4 * ((tid >> 4) & 3));
+        *reinterpret_cast<u32x2 *>(Xh + at) = u32x2{0, 0};
+        *reinterpret_cast<u32x2 *>(Xl + at) = u32x2{0, 0};
+        *reinterpret_cast<u32x2 *>(Yh + at) = u32x2{0, 0};
+        *reinterpret_cast<u32x2 *>(Yl + at) = u32x2{0, 0};
+    }
     scan(c1 - 1);
     fetch_g(c1 - 2);
-    if (c0 < c1) fetch(c1 - 1);
 #pragma unroll 1
     for (int c = c1 - 1; c >= c0; --c) {
         const int nr = rows_of(c);
@@ -535,46 +536,39 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
         put_terms(sr, 0, true);
         __syncthreads();
         parts[wave * C + lane0] = 0.0f;
-        {   // X, Y and the sums of M below the diagonal (the column tiles of a row tile are dealt to NW / 4 waves)
+        // X, Y and the sums of M below the diagonal: ten 16 x 16 tiles dealt to the waves
+#pragma unroll
+        for (int tn = 0; tn < (10 + NW - 1) / NW; ++tn) {
+            const int t = wave + tn * NW;
+            if (t >= 10) break;
             const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
-            const int it = wave / (NW / 4), i = 16 * it + l16;
-            bf16x8 qf[KS], of[VS];
+            const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2, i = 16 * it + l16, j = 16 * jt + 4 * gq;
+            f4 x = f4{0, 0, 0, 0}, y = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) qf[ks] = frag(Qs, QP, i, ks, gq);
+            for (int ks = 0; ks < KS; ++ks) x = mfma8(frag_p(Ks, QP, 16 * jt + l16, ks, gq), frag(Qs, QP, i, ks, gq), x);
 #pragma unroll
-            for (int vs = 0; vs < VS; ++vs) of[vs] = frag_p(Os, VP, i, vs, gq);
+            for (int vs = 0; vs < VS; ++vs) y = mfma8(frag_p(Vs, VP, 16 * jt + l16, vs, gq), frag_p(Os, VP, i, vs, gq), y);
             const float hi = bh[i], li = bl[i];
-            float rowsum = 0.0f;
-#pragma unroll 1
-            for (int jt = wave % (NW / 4); jt <= (it | 1); jt += NW / 4) {
-                f4 x = f4{0, 0, 0, 0}, y = f4{0, 0, 0, 0};
-                if (jt <= it) {
+            const f4 h4 = *reinterpret_cast<const f4 *>(bh + j), l4 = *reinterpret_cast<const f4 *>(bl + j);
+            f4 m;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) x = mfma8(frag_p(Ks, QP, 16 * jt + l16, ks, gq), qf[ks], x);
-#pragma unroll
-                    for (int vs = 0; vs < VS; ++vs) y = mfma8(frag_p(Vs, VP, 16 * jt + l16, vs, gq), of[vs], y);
-                    const f4 h4 = *reinterpret_cast<const f4 *>(bh + 16 * jt + 4 * gq), l4 = *reinterpret_cast<const f4 *>(bl + 16 * jt + 4 * gq);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = 16 * jt + 4 * gq + r;
-                        const float w = p.scale * hw_exp2((hi - h4[r]) + (li - l4[r]));
-                        const float yw = j <= i ? y[r] * w : 0.0f, m = j < i ? x[r] * yw : 0.0f;
-                        x[r] = j <= i ? x[r] * w : 0.0f;
-                        y[r] = yw;
-                        rowsum += m;
-                        const float cs = row16_sum(m);
-                        if (l16 == 0) parts[wave * C + j] -= cs;
-                    }
-                }
-                const int at = i * PP + 2 * operand_pos(16 * jt + 4 * gq);
-                const bf16x4 xh = round4(x), yh = round4(y);
-                *reinterpret_cast<bf16x4 *>(Xh + at) = xh;
-                *reinterpret_cast<bf16x4 *>(Xl + at) = round4(rest4(x, xh));
-                *reinterpret_cast<bf16x4 *>(Yh + at) = yh;
-                *reinterpret_cast<bf16x4 *>(Yl + at) = round4(rest4(y, yh));
+            for (int r = 0; r < 4; ++r) {
+                const float w = p.scale * hw_exp2((hi - h4[r]) + (li - l4[r]));
+                y[r] = j + r <= i ? y[r] * w : 0.0f;
+                m[r] = j + r < i ? x[r] * y[r] : 0.0f;
+                x[r] = j + r <= i ? x[r] * w : 0.0f;
             }
+            const int at = i * PP + 2 * operand_pos(j);
+            const bf16x4 xh = round4(x), yh = round4(y);
+            *reinterpret_cast<bf16x4 *>(Xh + at) = xh;
+            *reinterpret_cast<bf16x4 *>(Xl + at) = round4(rest4(x, xh));
+            *reinterpret_cast<bf16x4 *>(Yh + at) = yh;
+            *reinterpret_cast<bf16x4 *>(Yl + at) = round4(rest4(y, yh));
+            float rowsum = (m.x + m.y) + (m.z + m.w);
             rowsum += __shfl_xor(rowsum, 16, 64);
             rowsum += __shfl_xor(rowsum, 32, 64);
+            const f4 cs = f4{row16_sum(m.x), row16_sum(m.y), row16_sum(m.z), row16_sum(m.w)};
+            if (l16 == 0) *reinterpret_cast<f4 *>(parts + wave * C + j) -= cs;
             if (gq == 0) parts[wave * C + i] += rowsum;
         }
         {   // dq
@@ -626,20 +620,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                     acc[m] = mfma8(kf, frag_p(Yl, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
                 }
             }
+            const RowsOut out(DQ, nr, ldq);
 #pragma unroll
-            for (int m = 0; m < NI; ++m) {
-                const int i = 16 * (i0 + m) + l16;
-                if (i < nr) {
-                    QT *d = DQ + i * ldq + k;
-                    if (VEC) {
-                        if (k < p.dk) st4(d, acc[m]);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (k + r < p.dk) st1(d + r, acc[m][r]);
-                    }
-                }
-            }
+            for (int m = 0; m < NI; ++m) out.template put4<VEC>(DQ, 16 * (i0 + m) + l16, k, ldq, p.dk, acc[m]);
         }
         __syncthreads();                                              // D's terms are there
         const float eend = tail[0];
@@ -687,7 +670,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                     }
                 }
             }
-            corner = lanes_sum<64>(corner) * eend;
+            corner *= eend;
 #pragma unroll
             for (int m = 0; m < NI; ++m) {
                 const int j = operand_index(16 * (i0 + m) + l16);
@@ -695,11 +678,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                 const u32x2 w = *reinterpret_cast<const u32x2 *>(Ks + j * QP + 2 * operand_pos(16 * kt + 4 * gq));
                 const f2 k0 = bf16pair_to_f2(w.x), k1 = bf16pair_to_f2(w.y);
                 float d = (dk[m].x * k0.x + dk[m].y * k0.y) + (dk[m].z * k1.x + dk[m].w * k1.y);
-                corner += lanes_sum<64>(d);
+                corner += d;
                 d += __shfl_xor(d, 16, 64);
                 d += __shfl_xor(d, 32, 64);
                 if (gq == 0) parts[wave * C + j] -= d;
             }
+            corner = lanes_sum<64>(corner);
             if (lane == 0) corners[wave] = corner;
 #pragma unroll
             for (int m = 0; m < NJ; ++m) dv[m] *= wt[operand_index(16 * (j0 + m) + l16)];
@@ -720,34 +704,11 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                 }
             }
             const int k = 16 * kt + 4 * gq, v = operand_index(16 * vt + 4 * gq);
+            const RowsOut outk(DKp, nr, ldq), outv(DVp, nr, ldv);
 #pragma unroll
-            for (int m = 0; m < NI; ++m) {
-                const int j = operand_index(16 * (i0 + m) + l16);
-                if (j < nr) {
-                    QT *d = DKp + j * ldq + k;
-                    if (VEC) {
-                        if (k < p.dk) st4(d, dk[m]);
-                    } else {
+            for (int m = 0; m < NI; ++m) outk.template put4<VEC>(DKp, operand_index(16 * (i0 + m) + l16), k, ldq, p.dk, dk[m]);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (k + r < p.dk) st1(d + r, dk[m][r]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int m = 0; m < NJ; ++m) {
-                const int j = operand_index(16 * (j0 + m) + l16);
-                if (j < nr) {
-                    bf16 *d = DVp + j * ldv + v;
-                    if (VEC) {
-                        if (v < p.dv) st4(d, dv[m]);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (v + r < p.dv) st1(d + r, dv[m][r]);
-                    }
-                }
-            }
+            for (int m = 0; m < NJ; ++m) outv.template put4<VEC>(DVp, operand_index(16 * (j0 + m) + l16), v, ldv, p.dv, dv[m]);
         }
         DQ -= C * ldq; DKp -= C * ldq; DVp -= C * ldv;
         {   // D

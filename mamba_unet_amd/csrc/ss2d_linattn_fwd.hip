@@ -71,7 +71,7 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     const float *V = static_cast<const float *>(p.v) + s.row * p.vb + (s.start + (long long)first * C) * p.vl + h * p.vh + 64 * vt;
     const float *g = p.g + s.row * p.gb + s.start * p.gl + h * p.gh;
     const long long ldo = (long long)p.H * p.dv, nh = (long long)n * p.H + h, sz = (long long)p.dk * p.dv;
-    float *O = static_cast<float *>(a.o) + ((s.row * p.tokens + s.start + (long long)c0 * C) * p.H + h) * (long long)p.dv + col;
+    float *O = static_cast<float *>(a.o) + ((s.row * p.tokens + s.start + (long long)c0 * C) * p.H + h) * (long long)p.dv;
     f4 S[KT];
     const float *init = MODE >= 1 ? nullptr : p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
 #pragma unroll
@@ -193,12 +193,12 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[it] = mfma4(x[r], vv[jt][r], acc[it]);
                 }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * it + 4 * gq + r;
-                    if (i < nr && cok) O[i * ldo] = acc[it][r];
-                }
             }
+            const RowsOut out(O, nr, ldo);
+#pragma unroll
+            for (int it = 0; it < CT; ++it)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) out.put1(acc[it][r], 16 * it + 4 * gq + r, col, ldo, p.dv);
             O += C * ldo;
         }
         scan(c + STEP);

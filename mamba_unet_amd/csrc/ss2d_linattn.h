@@ -138,7 +138,6 @@ __device__ __forceinline__ bf16x8 frag_p(const unsigned char *tile, int pitch, i
     return *reinterpret_cast<const bf16x8 *>(tile + row * pitch + (32 * s + 8 * gq) * 2);
 }
 __device__ __forceinline__ int operand_pos(int c) { return (c & ~31) + 8 * ((c >> 2) & 3) + 4 * ((c >> 4) & 1); }      // of a group of four, c % 4 == 0
-__device__ __forceinline__ int operand_index(int pos) { return (pos & ~31) + 16 * ((pos >> 2) & 1) + 4 * ((pos >> 3) & 3) + (pos & 3); }   // its inverse
 // an operand from LDS, contracted index along the rows (rows 32 s + ...), columns 16 c .. 16 c + 15: ds_read_b64_tr_b16 hands every lane of 16 its
 // column of four rows; lane 4 a + b of the 16 addresses row a, columns 4 b .. 4 b + 3
 __device__ __forceinline__ bf16x8 frag_t(const unsigned char *tile, int pitch, int c, int s, int lane) {
@@ -146,6 +145,17 @@ __device__ __forceinline__ bf16x8 frag_t(const unsigned char *tile, int pitch, i
     const unsigned char *q = tile + (32 * s + 4 * (lane >> 4) + ((lane >> 2) & 3)) * pitch + (16 * c + 4 * (lane & 3)) * 2;
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 16 * pitch));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// the same with the contracted indices 8 gq + {0..7} of every 32, beside direct operands read as eight values in a row (frag_c)
+__device__ __forceinline__ bf16x8 frag_tc(const unsigned char *tile, int pitch, int c, int s, int lane) {
+    typedef s16x4 __attribute__((address_space(3))) *lp;
+    const unsigned char *q = tile + (32 * s + 8 * (lane >> 4) + ((lane >> 2) & 3)) * pitch + (16 * c + 4 * (lane & 3)) * 2;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)q), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 4 * pitch));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ bf16x8 frag_c(const unsigned char *tile, int pitch, int row, int s, int gq) {
+    return *reinterpret_cast<const bf16x8 *>(tile + row * pitch + (32 * s + 8 * gq) * 2);
 }
 
 // A C x DP tile of bf16 on its way from memory to LDS, 16-byte pieces; rows past n and columns past D are zero.  VEC: the pieces wait in registers, so

@@ -385,8 +385,8 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
 // The same walk for bf16 tensors on the bf16 matrix instruction: chunks of 64, 16 waves a workgroup (dk <= 32: 8).  LDS holds the four tiles, X and Y (two terms
 // each) and the terms of ONE state at a time, transposed (dv x dk): first S (for dq), then D (for dk and dv); with NB = 1 (128 x 128) one
 // term at a time.  States enter with three terms where dg is taken from the product (q . S do, k . D v), with two in dv.
-// Orders: k, v, dout and the columns j of X and Y lie in operand order (one 16-byte read an operand); what is read transposed from such a
-// tile comes in that order too, so the rows of dq and dv and the columns of dk, dv and D are named by operand_index.
+// Direct operands are eight values in a row (one 16-byte LDS read); what they are multiplied with, where it is read transposed, takes its contracted
+// rows in the same order (frag_tc).  Products of two transposed operands (over tokens) use frag_t for both.
 template <int DK, int DV, int NW, bool VEC, typename QT>
 __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdArgs a) {
     constexpr int NT = 64 * NW, C = 64, KT = DK / 16, KS = DK / 32, VT = DV / 16, VS = DV / 32;
@@ -448,8 +448,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
         kr.load(K, p.kl, nr);
         vr.load(V, p.vl, nr);
         orr.load(DO, ldv, nr);
-        const int ln = fresh(lane0), col = operand_index(16 * vt + (ln & 15));
-        const f4 *src = saved + (col >> 4) * KT * 64 + (ln >> 4) * 16 + (col & 15);
+        const int ln = fresh(lane0);
+        const f4 *src = saved + vt * KT * 64 + ln;
 #pragma unroll
         for (int t = 0; t < TW; ++t) sr[t] = src[64 * (kd + t)];
     };
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     fetch_g(c1 - 1);
     if (c0 < c1) fetch(c1 - 1);
     {
-        const int col = operand_index(16 * vt + (lane0 & 15));
+        const int col = 16 * vt + (lane0 & 15);
         const float *init = p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
@@ -495,13 +495,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
             if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(x + e);
         }
     };
-    auto put_terms = [&](const f4 (&x)[TW], int u0, bool ordered) {  // terms u0 ... u0 + NB - 1 of a state -> St, row dv, column k
-        const int ln = fresh(lane0), col = operand_index(16 * vt + (ln & 15));
+    auto put_terms = [&](const f4 (&x)[TW], int u0) {                // terms u0 ... u0 + NB - 1 of a state -> St, row dv, column k
+        const int ln = fresh(lane0), col = 16 * vt + (ln & 15);
 #pragma unroll
         for (int t = 0; t < TW; ++t) {
             const int k = 16 * (kd + t) + 4 * (ln >> 4);
             f4 v = x[t];
-            unsigned char *d = St + col * SP + 2 * (ordered ? operand_pos(k) : k);
+            unsigned char *d = St + col * SP + 2 * k;
 #pragma unroll
             for (int u = 0; u < 3; ++u) {
                 if (u >= u0 + NB) break;
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
         }
     };
     if (tid < 128) {                             // the tiles of X and Y behind the diagonal that are read with it (32 columns at a time): zero for good
-        const int i = 32 * (tid >> 6) + (tid & 15), at = i * PP + 2 * operand_pos(32 * (tid >> 6) + 16 + 4 * ((tid >> 4) & 3));
+        const int i = 32 * (tid >> 6) + (tid & 15), at = i * PP + 2 * (32 * (tid >> 6) + 16 + 4 * ((tid >> 4) & 3));
         *reinterpret_cast<u32x2 *>(Xh + at) = u32x2{0, 0};
         *reinterpret_cast<u32x2 *>(Xl + at) = u32x2{0, 0};
         *reinterpret_cast<u32x2 *>(Yh + at) = u32x2{0, 0};
@@ -527,13 +527,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
         __syncthreads();
         if (c + 1 < c1) finish_dg(c + 1);
         qr.put(Qs, QP, Q, p.ql, nr, p.dk);
-        kr.template put<true>(Ks, QP, K, p.kl, nr, p.dk);
-        vr.template put<true>(Vs, VP, V, p.vl, nr, p.dv);
-        orr.template put<true>(Os, VP, DO, ldv, nr, p.dv);
+        kr.put(Ks, QP, K, p.kl, nr, p.dk);
+        vr.put(Vs, VP, V, p.vl, nr, p.dv);
+        orr.put(Os, VP, DO, ldv, nr, p.dv);
         float corner = 0.0f;                                         // <D, S>
 #pragma unroll
         for (int t = 0; t < TW; ++t) corner += (sr[t].x * D[t].x + sr[t].y * D[t].y) + (sr[t].z * D[t].z + sr[t].w * D[t].w);
-        put_terms(sr, 0, true);
+        put_terms(sr, 0);
         __syncthreads();
         parts[wave * C + lane0] = 0.0f;
         // X, Y and the sums of M below the diagonal: ten 16 x 16 tiles dealt to the waves
@@ -545,9 +545,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
             const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2, i = 16 * it + l16, j = 16 * jt + 4 * gq;
             f4 x = f4{0, 0, 0, 0}, y = f4{0, 0, 0, 0};
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) x = mfma8(frag_p(Ks, QP, 16 * jt + l16, ks, gq), frag(Qs, QP, i, ks, gq), x);
+            for (int ks = 0; ks < KS; ++ks) x = mfma8(frag_c(Ks, QP, 16 * jt + l16, ks, gq), frag_c(Qs, QP, i, ks, gq), x);
 #pragma unroll
-            for (int vs = 0; vs < VS; ++vs) y = mfma8(frag_p(Vs, VP, 16 * jt + l16, vs, gq), frag_p(Os, VP, i, vs, gq), y);
+            for (int vs = 0; vs < VS; ++vs) y = mfma8(frag_c(Vs, VP, 16 * jt + l16, vs, gq), frag_c(Os, VP, i, vs, gq), y);
             const float hi = bh[i], li = bl[i];
             const f4 h4 = *reinterpret_cast<const f4 *>(bh + j), l4 = *reinterpret_cast<const f4 *>(bl + j);
             f4 m;
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                 m[r] = j + r < i ? x[r] * y[r] : 0.0f;
                 x[r] = j + r <= i ? x[r] * w : 0.0f;
             }
-            const int at = i * PP + 2 * operand_pos(j);
+            const int at = i * PP + 2 * j;
             const bf16x4 xh = round4(x), yh = round4(y);
             *reinterpret_cast<bf16x4 *>(Xh + at) = xh;
             *reinterpret_cast<bf16x4 *>(Xl + at) = round4(rest4(x, xh));
@@ -580,23 +580,23 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
             for (int u0 = 0; u0 < 3; u0 += NB) {
                 if (u0 > 0) {
                     __syncthreads();
-                    put_terms(sr, u0, true);
+                    put_terms(sr, u0);
                     __syncthreads();
                 }
 #pragma unroll
                 for (int vs = 0; vs < VS; ++vs) {
                     bf16x8 of[NI];
 #pragma unroll
-                    for (int m = 0; m < NI; ++m) of[m] = frag_p(Os, VP, 16 * (i0 + m) + l16, vs, gq);
+                    for (int m = 0; m < NI; ++m) of[m] = frag_c(Os, VP, 16 * (i0 + m) + l16, vs, gq);
 #pragma unroll
                     for (int u = 0; u < NB; ++u) {
-                        const bf16x8 sf = frag_t(St + u * DV * SP, SP, kt, vs, lane);
+                        const bf16x8 sf = frag_tc(St + u * DV * SP, SP, kt, vs, lane);
 #pragma unroll
                         for (int m = 0; m < NI; ++m) acc[m] = mfma8(sf, of[m], acc[m]);
                     }
                 }
             }
-            const int k = operand_index(16 * kt + 4 * gq);
+            const int k = 16 * kt + 4 * gq;
 #pragma unroll
             for (int m = 0; m < NI; ++m) {
                 const int i = 16 * (i0 + m) + l16;
@@ -609,15 +609,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                 if (gq == 0) parts[wave * C + i] += d;
             }
             __syncthreads();                                          // X, Y are there; S is done with
-            put_terms(D, 0, false);
+            put_terms(D, 0);
 #pragma unroll
             for (int js = 0; js < 2; ++js) {
-                const bf16x8 kf = frag_t(Ks, QP, kt, js, lane);
+                const bf16x8 kf = frag_tc(Ks, QP, kt, js, lane);
 #pragma unroll
                 for (int m = 0; m < NI; ++m) {
                     if (js > (i0 + m) / 2) continue;
-                    acc[m] = mfma8(kf, frag_p(Yh, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
-                    acc[m] = mfma8(kf, frag_p(Yl, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
+                    acc[m] = mfma8(kf, frag_c(Yh, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
+                    acc[m] = mfma8(kf, frag_c(Yl, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
                 }
             }
             const RowsOut out(DQ, nr, ldq);
@@ -635,22 +635,22 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
             for (int m = 0; m < NI; ++m) dk[m] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int m = 0; m < NJ; ++m) dv[m] = f4{0, 0, 0, 0};
-            const int vrow = operand_index(16 * vt + l16);
+            const int vrow = 16 * vt + l16;
 #pragma unroll 1
             for (int u0 = 0; u0 < 3; u0 += NB) {
                 if (u0 > 0) {
                     __syncthreads();
-                    put_terms(D, u0, false);
+                    put_terms(D, u0);
                     __syncthreads();
                 }
 #pragma unroll
                 for (int vs = 0; vs < VS; ++vs) {
                     bf16x8 vf[NI];
 #pragma unroll
-                    for (int m = 0; m < NI; ++m) vf[m] = frag_p(Vs, VP, operand_index(16 * (i0 + m) + l16), vs, gq);
+                    for (int m = 0; m < NI; ++m) vf[m] = frag_c(Vs, VP, 16 * (i0 + m) + l16, vs, gq);
 #pragma unroll
                     for (int u = 0; u < NB; ++u) {
-                        const bf16x8 df = frag_t(St + u * DV * SP, SP, kt, vs, lane);
+                        const bf16x8 df = frag_tc(St + u * DV * SP, SP, kt, vs, lane);
 #pragma unroll
                         for (int m = 0; m < NI; ++m) dk[m] = mfma8(df, vf[m], dk[m]);
                     }
@@ -660,10 +660,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                     for (int ks = 0; ks < KS; ++ks) {
                         bf16x8 kf[NJ];
 #pragma unroll
-                        for (int m = 0; m < NJ; ++m) kf[m] = frag_p(Ks, QP, operand_index(16 * (j0 + m) + l16), ks, gq);
+                        for (int m = 0; m < NJ; ++m) kf[m] = frag_c(Ks, QP, 16 * (j0 + m) + l16, ks, gq);
 #pragma unroll
                         for (int u = 0; u < (NB == 3 ? 2 : 1); ++u) {
-                            const bf16x8 df = frag(St + u * DV * SP, SP, vrow, ks, gq);
+                            const bf16x8 df = frag_c(St + u * DV * SP, SP, vrow, ks, gq);
 #pragma unroll
                             for (int m = 0; m < NJ; ++m) dv[m] = mfma8(df, kf[m], dv[m]);
                         }
@@ -673,9 +673,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
             corner *= eend;
 #pragma unroll
             for (int m = 0; m < NI; ++m) {
-                const int j = operand_index(16 * (i0 + m) + l16);
+                const int j = 16 * (i0 + m) + l16;
                 dk[m] *= wt[j];
-                const u32x2 w = *reinterpret_cast<const u32x2 *>(Ks + j * QP + 2 * operand_pos(16 * kt + 4 * gq));
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(Ks + j * QP + 2 * (16 * kt + 4 * gq));
                 const f2 k0 = bf16pair_to_f2(w.x), k1 = bf16pair_to_f2(w.y);
                 float d = (dk[m].x * k0.x + dk[m].y * k0.y) + (dk[m].z * k1.x + dk[m].w * k1.y);
                 corner += d;
@@ -686,7 +686,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
             corner = lanes_sum<64>(corner);
             if (lane == 0) corners[wave] = corner;
 #pragma unroll
-            for (int m = 0; m < NJ; ++m) dv[m] *= wt[operand_index(16 * (j0 + m) + l16)];
+            for (int m = 0; m < NJ; ++m) dv[m] *= wt[16 * (j0 + m) + l16];
 #pragma unroll
             for (int is = 0; is < 2; ++is) {
                 const bf16x8 qf = frag_t(Qs, QP, kt, is, lane), of = frag_t(Os, VP, vt, is, lane);
@@ -703,12 +703,12 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                     dv[m] = mfma8(of, frag_t(Xl, PP, j0 + m, is, lane), dv[m]);
                 }
             }
-            const int k = 16 * kt + 4 * gq, v = operand_index(16 * vt + 4 * gq);
+            const int k = 16 * kt + 4 * gq, v = 16 * vt + 4 * gq;
             const RowsOut outk(DKp, nr, ldq), outv(DVp, nr, ldv);
 #pragma unroll
-            for (int m = 0; m < NI; ++m) outk.template put4<VEC>(DKp, operand_index(16 * (i0 + m) + l16), k, ldq, p.dk, dk[m]);
+            for (int m = 0; m < NI; ++m) outk.template put4<VEC>(DKp, 16 * (i0 + m) + l16, k, ldq, p.dk, dk[m]);
 #pragma unroll
-            for (int m = 0; m < NJ; ++m) outv.template put4<VEC>(DVp, operand_index(16 * (j0 + m) + l16), v, ldv, p.dv, dv[m]);
+            for (int m = 0; m < NJ; ++m) outv.template put4<VEC>(DVp, 16 * (j0 + m) + l16, v, ldv, p.dv, dv[m]);
         }
         DQ -= C * ldq; DKp -= C * ldq; DVp -= C * ldv;
         {   // D
@@ -738,7 +738,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     __syncthreads();
     if (c0 < c1) finish_dg(c0);
     if (a.ds0 && p.nseg == 1) {
-        const int col = operand_index(16 * vt + (lane0 & 15));
+        const int col = 16 * vt + (lane0 & 15);
         float *d = a.ds0 + nh * sz;
 #pragma unroll
         for (int t = 0; t < TW; ++t)

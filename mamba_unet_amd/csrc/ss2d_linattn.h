@@ -21,7 +21,7 @@ struct Problem {
     int N, H, G, dk, dv;
     float scale;
     int nseg, segc;               // segments of a sequence, chunks a segment
-    int vec;                      // all rows start on 16-byte boundaries and dk, dv are multiples of 8
+    int vec;                      // rows are made of 16-byte pieces that begin on 32-bit words
 };
 
 // A workgroup's sequence: token rows [start, start + len) of batch row `row`.  The offsets of a packed batch come from device
@@ -158,59 +158,72 @@ __device__ __forceinline__ bf16x8 frag_c(const unsigned char *tile, int pitch, i
     return *reinterpret_cast<const bf16x8 *>(tile + row * pitch + (32 * s + 8 * gq) * 2);
 }
 
-// A C x DP tile of bf16 on its way from memory to LDS, 16-byte pieces; rows past n and columns past D are zero.  VEC: the pieces wait in registers, so
-// a chunk is in flight while the previous one is worked on; else (rows not made of 16-byte pieces) elements go straight to LDS.
+// A C x DP tile of bf16 on its way from memory to LDS, in 16-byte pieces of a row that wait in registers, so a chunk is in flight while the previous
+// one is worked on; rows past n and columns past D are zero.  VEC: rows are made of such pieces.  Else a piece may begin in the middle of a 32-bit
+// word: five words are read and shifted, and the last piece of a row is masked (4 x 4096 tokens, 16 heads of 100 x 96, forward and backward:
+// 595 us; element by element 1004).  Every row, head and batch starts on an even or odd element for good: C rows are an even number.
 template <int C, int DP, int NT, bool VEC>
 struct TileRegs {
-    static constexpr int PR = DP / 8, N = C * PR / NT > 0 ? C * PR / NT : 1;      // pieces a row, pieces a thread
-    u32x4 v[VEC ? N : 1];
-    int voff;                                                      // bytes from the chunk's first row; pieces past D lie outside every descriptor
-    __device__ __forceinline__ void init(long long ld, int D) {
-        const int r = threadIdx.x / PR, c = 8 * (threadIdx.x % PR);
-        voff = c < D && r < C ? (r * (int)ld + c) * 2 : SS2D_BUF_OOR;
+    static constexpr int PR = DP / 8, N = C * PR / NT > 0 ? C * PR / NT : 1, STEP = NT / PR;     // pieces a row, pieces a thread, rows from one to the next
+    static_assert(C % 2 == 0 && STEP % 2 == 0, "a thread's pieces begin alike");
+    u32x4 v[N];
+    unsigned last[VEC ? 1 : N];
+    int voff, shift;                                               // bytes from the chunk's first row; pieces past D lie outside every descriptor
+    __device__ __forceinline__ void init(const bf16 *src, long long ld, int D) {
+        const int r = threadIdx.x / PR, c = 8 * (threadIdx.x % PR), off = (r * (int)ld + c) * 2 + (VEC ? 0 : (int)((uintptr_t)src & 2));
+        voff = c < D && r < C ? off & ~3 : SS2D_BUF_OOR;
+        shift = (off & 2) * 8;
     }
-    // a descriptor of n rows: later rows read as zero.  ld < 2^22 elements (host)
-    __device__ __forceinline__ void load(const bf16 *src, long long ld, int n) {
-        if (!VEC) return;
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(src, (unsigned)(n * (int)ld * 2));
+    // a descriptor of n rows: later rows read as zero.  D <= ld < 2^22 elements (host)
+    __device__ __forceinline__ void load(const bf16 *src, long long ld, int n, int D) {
+        if (VEC) {
+            const __amdgpu_buffer_rsrc_t rs = make_rsrc(src, (unsigned)(n * (int)ld * 2));
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[VEC ? j : 0] = __builtin_amdgcn_raw_buffer_load_b128(rs, voff, j * (NT / PR) * (int)ld * 2, 0);
+            for (int j = 0; j < N; ++j) v[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, voff, j * STEP * (int)ld * 2, 0);
+        } else {
+            const int lead = (int)((uintptr_t)src & 2);            // whole words, the first and last of which may be half outside
+            const __amdgpu_buffer_rsrc_t rs = make_rsrc(reinterpret_cast<const char *>(src) - lead, n > 0 ? (unsigned)(lead + ((n - 1) * (int)ld + D) * 2 + 3) & ~3u : 0u);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int at = (int)threadIdx.x / PR + j * STEP < n ? voff : SS2D_BUF_OOR;
+                v[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, at, j * STEP * (int)ld * 2, 0);
+                last[VEC ? 0 : j] = __builtin_amdgcn_raw_buffer_load_b32(rs, at, j * STEP * (int)ld * 2 + 16, 0);
+            }
+        }
     }
     // ORDERED: 32-column blocks in operand order (frag_p)
     template <bool ORDERED = false>
-    __device__ __forceinline__ void put(unsigned char *tile, int pitch, const bf16 *src, long long ld, int n, int D) const {
-        if (VEC) {
+    __device__ __forceinline__ void put(unsigned char *tile, int pitch, int D) const {
+        const int c = 8 * (threadIdx.x % PR);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int e = threadIdx.x + j * NT, r = e / PR, c = 8 * (e % PR);
-                if (C * PR % NT == 0 || r < C) {
-                    const u32x4 w = v[VEC ? j : 0];
-                    unsigned char *d = tile + r * pitch;
-                    if (ORDERED) {
-                        *reinterpret_cast<u32x2 *>(d + 2 * operand_pos(c)) = u32x2{w.x, w.y};
-                        *reinterpret_cast<u32x2 *>(d + 2 * operand_pos(c + 4)) = u32x2{w.z, w.w};
-                    } else {
-                        *reinterpret_cast<u32x4 *>(d + 2 * c) = w;
+        for (int j = 0; j < N; ++j) {
+            const int r = threadIdx.x / PR + j * STEP;
+            if (C * PR % NT == 0 || r < C) {
+                u32x4 w = v[j];
+                if (!VEC) {
+                    const unsigned q[5] = {w.x, w.y, w.z, w.w, last[VEC ? 0 : j]};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned both = __builtin_amdgcn_alignbit(q[i + 1], q[i], (unsigned)shift);
+                        w[i] = c + 2 * i + 1 < D ? both : c + 2 * i < D ? both & 0xffffu : 0u;
                     }
                 }
-            }
-        } else {
-#pragma unroll 1
-            for (int e = threadIdx.x; e < C * DP / 2; e += NT) {
-                const int r = e / (DP / 2), c = 2 * (e % (DP / 2));
-                bf16x2 w = bf16x2{(bf16)0.0f, (bf16)0.0f};
-                if (r < n && c < D) w[0] = src[(long long)r * ld + c];
-                if (r < n && c + 1 < D) w[1] = src[(long long)r * ld + c + 1];
-                *reinterpret_cast<bf16x2 *>(tile + r * pitch + 2 * (ORDERED ? operand_pos(c & ~3) + (c & 3) : c)) = w;
+                unsigned char *d = tile + r * pitch;
+                if (ORDERED) {
+                    *reinterpret_cast<u32x2 *>(d + 2 * operand_pos(c)) = u32x2{w.x, w.y};
+                    *reinterpret_cast<u32x2 *>(d + 2 * operand_pos(c + 4)) = u32x2{w.z, w.w};
+                } else {
+                    *reinterpret_cast<u32x4 *>(d + 2 * c) = w;
+                }
             }
         }
     }
 };
 
-// the same for fp32 tiles (C x DP, PITCH floats a row): groups of four columns, register-held or element by element
+// the same for fp32 tiles (C x DP, PITCH floats a row), groups of four columns: a group may begin on any word, so only a row's last group differs
 template <int C, int DP, int PITCH, int NT, bool VEC>
 struct TileRegsF {
-    static constexpr int PR = DP / 4, N = (C * PR + NT - 1) / NT;
+    static constexpr int PR = DP / 4, N = (C * PR + NT - 1) / NT, STEP = NT / PR;
     f4 v[N];
     int voff;
     __device__ __forceinline__ void init(long long ld, int D) {
@@ -218,28 +231,26 @@ struct TileRegsF {
         voff = c < D && r < C ? (r * (int)ld + c) * 4 : SS2D_BUF_OOR;
     }
     __device__ __forceinline__ void load(const float *src, long long ld, int n, int D) {
-        if (VEC) {
-            const __amdgpu_buffer_rsrc_t rs = make_rsrc(src, (unsigned)(n * (int)ld * 4));
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rs, voff, j * (NT / PR) * (int)ld * 4, 0));
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int e = threadIdx.x + j * NT, r = e / PR, c = 4 * (e % PR);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool ok = r < n && r < C && c + i < D;
-                    const float x = src[ok ? (long long)r * ld + c + i : 0];
-                    v[j][i] = ok ? x : 0.0f;
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void put(float *tile) const {
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(src, VEC ? (unsigned)(n * (int)ld * 4) : n > 0 ? (unsigned)(((n - 1) * (int)ld + D) * 4) : 0u);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int e = threadIdx.x + j * NT, r = e / PR, c = 4 * (e % PR);
-            if (C * PR % NT == 0 || r < C) *reinterpret_cast<f4 *>(tile + r * PITCH + c) = v[j];
+            const int at = VEC || (int)threadIdx.x / PR + j * STEP < n ? voff : SS2D_BUF_OOR;
+            v[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, j * STEP * (int)ld * 4, 0));
+        }
+    }
+    __device__ __forceinline__ void put(float *tile, int D) const {
+        const int c = 4 * (threadIdx.x % PR);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = threadIdx.x / PR + j * STEP;
+            if (C * PR % NT == 0 || r < C) {
+                f4 w = v[j];
+                if (!VEC) {
+#pragma unroll
+                    for (int i = 1; i < 4; ++i) w[i] = c + i < D ? w[i] : 0.0f;
+                }
+                *reinterpret_cast<f4 *>(tile + r * PITCH + c) = w;
+            }
         }
     }
 };
@@ -250,12 +261,12 @@ struct RowsOut {
     __amdgpu_buffer_rsrc_t rs;
     template <typename T>
     __device__ __forceinline__ RowsOut(T *base, int n, long long ld) : rs(make_rsrc(base, (unsigned)(n * (int)ld * (int)sizeof(T)))) {}
-    // four columns c .. c + 3 of row r (VEC: all four or none inside)
+    // four columns c .. c + 3 of row r; VEC, or D a multiple of 4: all four or none inside
     template <bool VEC>
     __device__ __forceinline__ void put4(bf16 *, int r, int c, long long ld, int D, f4 v) const {
         const u32x2 w = __builtin_bit_cast(u32x2, round4(v));
         const int off = (r * (int)ld + c) * 2;
-        if (VEC) {
+        if (VEC || D % 4 == 0) {
             __builtin_amdgcn_raw_buffer_store_b64(w, rs, c < D ? off : SS2D_BUF_OOR, 0, 0);
         } else {
             const unsigned a = w.x, b = w.y;
@@ -267,7 +278,7 @@ struct RowsOut {
     template <bool VEC>
     __device__ __forceinline__ void put4(float *, int r, int c, long long ld, int D, f4 v) const {
         const int off = (r * (int)ld + c) * 4;
-        if (VEC) {
+        if (VEC || D % 4 == 0) {
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, c < D ? off : SS2D_BUF_OOR, 0, 0);
         } else {
 #pragma unroll
@@ -318,11 +329,17 @@ inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, 
     p.q = q; p.k = k; p.v = v; p.g = g; p.cu = cu; p.tokens = tokens; p.N = N; p.H = H; p.G = G; p.dk = dk; p.dv = dv; p.scale = scale; p.nseg = nseg; p.segc = segc;
     p.qb = st[0]; p.ql = st[1]; p.qh = st[2]; p.kb = st[3]; p.kl = st[4]; p.kh = st[5];
     p.vb = st[6]; p.vl = st[7]; p.vh = st[8]; p.gb = st[9]; p.gl = st[10]; p.gh = st[11];
-    const int m = 8;                                            // 16 bytes of bf16, 32 of fp32
-    bool vec = dk % m == 0 && dv % m == 0 && ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 == 0;
-    for (int i = 0; i < 9; ++i) vec = vec && st[i] % m == 0;
-    // 16-byte pieces come through descriptors of a chunk's rows: dense enough not to overlap, and short of 2^31 bytes
-    vec = vec && st[1] >= dk && st[4] >= dk && st[7] >= dv && st[1] < (1 << 22) && st[4] < (1 << 22) && st[7] < (1 << 22);
+    // rows come through descriptors of a chunk: they must not overlap, nor lie 2^22 elements apart
+    if (st[1] < dk || st[4] < dk || st[7] < dv || st[1] >= (1 << 22) || st[4] >= (1 << 22) || st[7] >= (1 << 22)) {
+        ss2d_set_error("%s: token strides %lld, %lld, %lld", name, st[1], st[4], st[7]);
+        return -4;
+    }
+    const int m = dtype ? 8 : 4;                                // elements of a 16-byte piece
+    bool vec = dk % m == 0 && dv % m == 0;
+    if (dtype) {                                                // fp32 pieces may begin on any word, bf16 ones only on a word's start
+        vec = vec && ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 4 == 0;
+        for (int i = 0; i < 9; ++i) vec = vec && st[i] % 2 == 0;
+    }
     p.vec = vec;
     return 0;
 }

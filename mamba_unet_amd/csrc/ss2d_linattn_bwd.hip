@@ -8,7 +8,8 @@
 //   dg_t = sum_{i >= t > j} M_ij,  M_ij = w_ij (q_i . k_j)(do_i . v_j),
 // with the state in front of the chunk as one more column, D as one more row.  It is taken as row sums minus column sums, added
 // up from the chunk's end; pairs that do not cross t cancel there, but only pairs of ONE chunk, and the diagonal, whose terms
-// are the largest and cross nothing, never enters.
+// are the largest and cross nothing, never enters.  The chunk's first decay is crossed by the pairs with the state alone: their sum, exactly 0 at a
+// start without a state.
 //
 // A workgroup walks one segment of one sequence and value head from its end to its start with D in accumulator registers (a wave owns
 // 16-column slices of dv).  Segments as in the forward: own contributions, a join in order, the walk.
@@ -90,7 +91,7 @@ template <int DK, int DV, int C, bool VEC>
 __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
     constexpr int NT = 1024, PK = DK + 4, PV = DV + 4, PP = C + 4, KT = DK / 16, VT = DV / 16, CT = C / 16;
     constexpr int TW = (KT * VT + 15) / 16;                          // tiles of D a wave owns: wave + 16 m
-    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * C * PP + 10 * 64 + 16 * 64 + 16];
+    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * C * PP + 10 * 64 + 16 * 64 + 32];
     float *Qs = lds, *Ks = Qs + C * PK, *Vs = Ks + C * PK, *Os = Vs + C * PV, *St = Os + C * PV, *Xs = St + DK * PV, *Ys = Xs + C * PP;
     float *decays = Ys + C * PP, *parts = decays + 10 * 64, *corners = parts + 16 * 64;
     const Problem &p = a.p;
@@ -185,15 +186,15 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
     };
     auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: gradients of b inside the chunk, summed from its end
         if (wave == 1) {
-            double x = 0.0, e = 0.0;
+            double x = 0.0, e = 0.0, first = 0.0;
 #pragma unroll
-            for (int w = 0; w < 16; ++w) { x += (double)parts[w * 64 + lane0]; e += (double)corners[w]; }
+            for (int w = 0; w < 16; ++w) { x += (double)parts[w * 64 + lane0]; e += (double)corners[w]; first += (double)corners[16 + w]; }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_down(x, d, 64);
                 if (lane0 + d < 64) x += o;
             }
-            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(x + e);
+            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(lane0 ? x + e : first);
         }
     };
     auto put_state = [&](const f4 (&x)[TW]) {
@@ -222,10 +223,10 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
         const float *bh = decays + (c & 1) * 5 * 64, *bl = bh + 64, *eb = bl + 64, *wt = eb + 64, *tail = wt + 64;
         __syncthreads();
         if (c + 1 < c1) finish_dg(c + 1);
-        qr.put(Qs);
-        kr.put(Ks);
-        vr.put(Vs);
-        orr.put(Os);
+        qr.put(Qs, p.dk);
+        kr.put(Ks, p.dk);
+        vr.put(Vs, p.dv);
+        orr.put(Os, p.dv);
         put_state(sr);
         float corner = 0.0f;                                         // <D, S>
 #pragma unroll
@@ -267,6 +268,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
         }
         const int k = 16 * qk + l16;
         f4 dq = f4{0, 0, 0, 0};
+        float front = 0.0f;                                          // pairs with the state in front of the chunk: all that crosses its first decay
         if (has_q) {
 #pragma unroll
             for (int v = 0; v < VT; ++v)
@@ -275,7 +277,8 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * qi + 4 * gq + r;
-                const float rs = row16_sum(dq[r] * Qs[i * PK + k]);
+                const float qs = dq[r] * Qs[i * PK + k], rs = row16_sum(qs);
+                front += qs;
                 if (l16 == 0) parts[wave * 64 + i] += rs;
             }
         }
@@ -295,6 +298,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
         __syncthreads();                                              // D is there
         const float eend = tail[0];
         corner *= eend;
+        front += corner;
         if (has_q) {
             f4 dk = f4{0, 0, 0, 0};
 #pragma unroll
@@ -323,7 +327,8 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
             for (int r = 0; r < 4; ++r) out.put1(dk[r], 16 * qi + 4 * gq + r, k, ldq, p.dk);
         }
         corner = lanes_sum<64>(corner);
-        if (lane == 0) corners[wave] = corner;
+        front = lanes_sum<64>(front);
+        if (lane == 0) { corners[wave] = corner; corners[16 + wave] = front; }
         if (has_v) {
             const int col = 16 * vt + l16;
             f4 dv = f4{0, 0, 0, 0};
@@ -393,7 +398,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     constexpr int QP = 2 * DK + 32, VP = 2 * DV + 32, PP = 2 * C + 32, SP = 2 * DK + 16;      // bytes a row
     constexpr int NB = DK == 128 && DV == 128 ? 1 : 3;                                        // terms of a state in LDS at once
     constexpr int NI = 4 * KT / NW, NJ = 4 * VT / NW, TW = KT * VT / NW;                               // tiles of a wave: rows of dq / dk, rows of dv, D
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * C * PP + NB * DV * SP + (10 * C + NW * C + NW) * 4];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * C * PP + NB * DV * SP + (10 * C + NW * C + 2 * NW) * 4];
     unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + C * PP, *Yh = Xl + C * PP,
                   *Yl = Yh + C * PP, *St = Yl + C * PP;
     float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + NW * C;
@@ -435,19 +440,19 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     f4 D[TW];
     TileRegs<C, DK, NT, VEC> qr, kr;
     TileRegs<C, DV, NT, VEC> vr, orr;
-    qr.init(p.ql, p.dk);
-    kr.init(p.kl, p.dk);
-    vr.init(p.vl, p.dv);
-    orr.init(ldv, p.dv);
+    qr.init(Q, p.ql, p.dk);
+    kr.init(K, p.kl, p.dk);
+    vr.init(V, p.vl, p.dv);
+    orr.init(DO, ldv, p.dv);
     f4 sr[TW];                                                       // S in D's arrangement
     const f4 *saved = reinterpret_cast<const f4 *>(a.chunk_states) + ((chunk_base(p, s, n, C) + c1 - 1) * p.H + h) * (DK * DV / 4);
     auto rows_of = [&](int c) { const int left = s.len - c * C; return left < C ? left : C; };
     auto fetch = [&](int c) {
         const int nr = rows_of(c);
-        qr.load(Q, p.ql, nr);
-        kr.load(K, p.kl, nr);
-        vr.load(V, p.vl, nr);
-        orr.load(DO, ldv, nr);
+        qr.load(Q, p.ql, nr, p.dk);
+        kr.load(K, p.kl, nr, p.dk);
+        vr.load(V, p.vl, nr, p.dv);
+        orr.load(DO, ldv, nr, p.dv);
         const int ln = fresh(lane0);
         const f4 *src = saved + vt * KT * 64 + ln;
 #pragma unroll
@@ -484,15 +489,15 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     };
     auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: gradients of b inside the chunk, summed from its end
         if (wave == 1) {
-            double x = 0.0, e = 0.0;
+            double x = 0.0, e = 0.0, first = 0.0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) { x += (double)parts[w * C + lane0]; e += (double)corners[w]; }
+            for (int w = 0; w < NW; ++w) { x += (double)parts[w * C + lane0]; e += (double)corners[w]; first += (double)corners[NW + w]; }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_down(x, d, 64);
                 if (lane0 + d < 64) x += o;
             }
-            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(x + e);
+            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(lane0 ? x + e : first);
         }
     };
     auto put_terms = [&](const f4 (&x)[TW], int u0) {                // terms u0 ... u0 + NB - 1 of a state -> St, row dv, column k
@@ -526,10 +531,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
         const float *bh = decays + (c & 1) * 5 * C, *bl = bh + C, *eb = bl + C, *wt = eb + C, *tail = wt + C;
         __syncthreads();
         if (c + 1 < c1) finish_dg(c + 1);
-        qr.put(Qs, QP, Q, p.ql, nr, p.dk);
-        kr.put(Ks, QP, K, p.kl, nr, p.dk);
-        vr.put(Vs, VP, V, p.vl, nr, p.dv);
-        orr.put(Os, VP, DO, ldv, nr, p.dv);
+        qr.put(Qs, QP, p.dk);
+        kr.put(Ks, QP, p.dk);
+        vr.put(Vs, VP, p.dv);
+        orr.put(Os, VP, p.dv);
         float corner = 0.0f;                                         // <D, S>
 #pragma unroll
         for (int t = 0; t < TW; ++t) corner += (sr[t].x * D[t].x + sr[t].y * D[t].y) + (sr[t].z * D[t].z + sr[t].w * D[t].w);
@@ -571,6 +576,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
             if (l16 == 0) *reinterpret_cast<f4 *>(parts + wave * C + j) -= cs;
             if (gq == 0) parts[wave * C + i] += rowsum;
         }
+        float front = 0.0f;                                          // pairs with the state in front of the chunk: all that crosses its first decay
         {   // dq
             const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
             f4 acc[NI];
@@ -604,6 +610,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                 const u32x2 w = *reinterpret_cast<const u32x2 *>(Qs + i * QP + 2 * k);
                 const f2 q0 = bf16pair_to_f2(w.x), q1 = bf16pair_to_f2(w.y);
                 float d = (acc[m].x * q0.x + acc[m].y * q0.y) + (acc[m].z * q1.x + acc[m].w * q1.y);
+                front += d;
                 d += __shfl_xor(d, 16, 64);
                 d += __shfl_xor(d, 32, 64);
                 if (gq == 0) parts[wave * C + i] += d;
@@ -671,6 +678,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                 }
             }
             corner *= eend;
+            front += corner;
 #pragma unroll
             for (int m = 0; m < NI; ++m) {
                 const int j = 16 * (i0 + m) + l16;
@@ -684,7 +692,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                 if (gq == 0) parts[wave * C + j] -= d;
             }
             corner = lanes_sum<64>(corner);
-            if (lane == 0) corners[wave] = corner;
+            front = lanes_sum<64>(front);
+            if (lane == 0) { corners[wave] = corner; corners[NW + wave] = front; }
 #pragma unroll
             for (int m = 0; m < NJ; ++m) dv[m] *= wt[16 * (j0 + m) + l16];
 #pragma unroll
@@ -833,10 +842,9 @@ extern "C" int ss2d_linattn_bwd(int dtype, const void *q, const void *k, const v
     if (nseg > 1 && (!seg_states || !seg_decay)) { ss2d_set_error("linattn_bwd: segments without a workspace"); return -2; }
     a.dout = dout; a.dlast = dlast; a.chunk_states = chunk_states; a.dq = H > G ? dq_heads : dq; a.dk_ = H > G ? dk_heads : dk_out;
     a.dv_ = dv_out; a.dg = dg; a.ds0 = ds0; a.seg_states = seg_states; a.seg_decay = seg_decay;
-    a.p.vec = a.p.vec && (uintptr_t)dout % 16 == 0;
+    a.p.vec = a.p.vec && (dtype == SS2D_DTYPE_F32 || (uintptr_t)dout % 4 == 0);
     const unsigned gaps = cu_seqlens ? GAP_WGS : 0;
     hipStream_t s = (hipStream_t)stream;
-    a.p.vec = a.p.vec && (long long)H * dv < (1 << 22);
     if (nseg > 1) {
         Problem r = a.p;                          // q in the place of k, dout in that of v
         r.k = q; r.kb = r.qb; r.kl = r.ql; r.kh = r.qh;

@@ -137,9 +137,9 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
             saved += p.H * sz;
         }
         __syncthreads();
-        if (MODE == 0) qr.put(Qs);
-        kr.put(Ks);
-        vr.put(Vs);
+        if (MODE == 0) qr.put(Qs, p.dk);
+        kr.put(Ks, p.dk);
+        vr.put(Vs, dvc);
         if (c + STEP >= c0 && c + STEP < c1) fetch(c + STEP);
         __syncthreads();
         const float *bh = decays + (c & 1) * 320, *bl = bh + 64, *eb = bl + 64, *wt = eb + 64, *tail = wt + 64;
@@ -270,15 +270,15 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
     f4 S[KT];
     TileRegs<C, DK, NT, VEC> qr, kr;
     TileRegs<C, DV, NT, VEC> vr;
-    qr.init(p.ql, p.dk);
-    kr.init(p.kl, p.dk);
-    vr.init(p.vl, p.dv);
+    qr.init(Q, p.ql, p.dk);
+    kr.init(K, p.kl, p.dk);
+    vr.init(V, p.vl, p.dv);
     auto rows_of = [&](int c) { const int left = s.len - c * C; return left < C ? left : C; };
     auto fetch = [&](int c) {                    // chunk c, the tensors' pointers at chunk c
         const int nr = rows_of(c);
-        if (MODE == 0) qr.load(Q, p.ql, nr);
-        kr.load(K, p.kl, nr);
-        vr.load(V, p.vl, nr);
+        if (MODE == 0) qr.load(Q, p.ql, nr, p.dk);
+        kr.load(K, p.kl, nr, p.dk);
+        vr.load(V, p.vl, nr, p.dv);
     };
     float gr = 0.0f;                             // wave 0: decays, a chunk ahead of the tiles
     auto fetch_g = [&](int c) {
@@ -326,9 +326,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
             saved += (long long)p.H * (DK * DV / 4);
         }
         __syncthreads();
-        if (MODE == 0) qr.template put<true>(Qs, QP, Q, p.ql, nr, p.dk);
-        kr.put(Ks, KP, K, p.kl, nr, p.dk);
-        vr.put(Vs, VP, V, p.vl, nr, p.dv);
+        if (MODE == 0) qr.template put<true>(Qs, QP, p.dk);
+        kr.put(Ks, KP, p.dk);
+        vr.put(Vs, VP, p.dv);
         Q += C * p.ql; K += STEP * C * p.kl; V += STEP * C * p.vl;
         if (MODE >= 1 && c + STEP >= c0 && c + STEP < c1) fetch(c + STEP);
         const float *bh = decays + (c & 1) * 5 * C, *bl = bh + C, *eb = bl + C, *wt = eb + C, *tail = wt + C;

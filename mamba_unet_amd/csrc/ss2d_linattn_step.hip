@@ -1,7 +1,7 @@
 // One new token of linear attention for each of B requests (formulas: ss2d_linattn.h), for gfx950: the recurrent form
 //     S <- exp(g) S + k v^T,   o = scale * S^T q
 // on the states of a pool, in place.  Bound by the state: dk * dv fp32 values are read and written once for every request and head, all
-// else is small.  A workgroup takes one (request, head) and a slice of dv: its threads hold the slice in registers (VW columns x every
+// else is small.  A workgroup takes one (request, head) and a slice of dv: its threads hold the slice in registers (four columns x every
 // RG-th row each), so every state element is loaded once, updated, stored and multiplied into the output, and the partial sums over dk
 // meet in LDS.
 //
@@ -12,7 +12,7 @@
 
 namespace {
 
-constexpr int NT = 256;
+constexpr int NT = 256, NC = 16;
 
 struct StepArgs {
     float *state;
@@ -31,37 +31,43 @@ __device__ __forceinline__ long long slot_of(const StepArgs &a, int b) {
     return a.idx64 ? static_cast<const long long *>(a.idx)[b] : (long long)static_cast<const int *>(a.idx)[b];
 }
 
-// NC: column groups of VW columns a workgroup (a power of two); RG = 256 / NC rows are in flight per trip; NR trips cover dk
-template <int VW, int NC, int NR, typename IO>
+// Four neighbouring columns of a row that lies on any 32-bit word; the last group of a row may hold less than four (n: what is left of the row)
+typedef f4 __attribute__((aligned(4))) f4_any;
+__device__ __forceinline__ f4 load_columns(const float *s, int n) {
+    if (n >= 4) return *reinterpret_cast<const f4_any *>(s);
+    return f4{n > 0 ? s[0] : 0.0f, n > 1 ? s[1] : 0.0f, n > 2 ? s[2] : 0.0f, 0.0f};
+}
+__device__ __forceinline__ void store_columns(float *s, int n, f4 v) {
+    if (n >= 4) { *reinterpret_cast<f4_any *>(s) = v; return; }
+    if (n > 0) s[0] = v.x;
+    if (n > 1) s[1] = v.y;
+    if (n > 2) s[2] = v.z;
+}
+
+// NC groups of four columns a workgroup; RG = 256 / NC rows are in flight per trip, NR trips cover dk
+template <int NR, typename IO>
 __global__ __launch_bounds__(NT) void la_step_kernel(const StepArgs a) {
     constexpr int RG = NT / NC;
-    __shared__ float red[RG][NC * VW + 1];
+    __shared__ float red[RG][NC * 4 + 1];
     const int tid = threadIdx.x, cg = tid % NC, rg = tid / NC;
-    const int tiles = (a.dv + NC * VW - 1) / (NC * VW);
+    const int tiles = (a.dv + NC * 4 - 1) / (NC * 4);
     int id = blockIdx.x;
     const int tile = id % tiles; id /= tiles;
     const int h = id % a.H, b0 = id / a.H;
-    const int c0 = (tile * NC + cg) * VW;
-    const bool cok = c0 < a.dv;                            // VW > 1 only with dv a multiple of VW
+    const int c0 = (tile * NC + cg) * 4, left = a.dv - c0;  // columns of the row from c0 on
     IO *O = static_cast<IO *>(a.o);
     const long long slot = slot_of(a, b0);
     if (slot < 0 || slot >= a.pool) {                      // no state: the output is zero
-        if (rg == 0 && cok)
-            for (int e = 0; e < VW; ++e) st1(O + ((long long)b0 * a.H + h) * a.dv + c0 + e, 0.0f);
+        if (rg == 0)
+            for (int e = 0; e < 4 && e < left; ++e) st1(O + ((long long)b0 * a.H + h) * a.dv + c0 + e, 0.0f);
         return;
     }
     float *S = a.state + slot * a.slot_stride + (long long)h * a.dk * a.dv + c0;
-    float s[NR][VW];
+    f4 s[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
         const int k = rg + RG * r;
-        const bool ok = cok && k < a.dk;
-        if (VW == 4) {
-            const f4 t = *reinterpret_cast<const f4 *>(ok ? S + (long long)k * a.dv : a.state);
-            s[r][0] = t.x; s[r][VW > 1 ? 1 : 0] = VW > 1 ? t.y : t.x; s[r][VW > 2 ? 2 : 0] = VW > 2 ? t.z : t.x; s[r][VW > 3 ? 3 : 0] = VW > 3 ? t.w : t.x;
-        } else {
-            s[r][0] = ok ? S[(long long)k * a.dv] : 0.0f;
-        }
+        s[r] = load_columns(S + (long long)k * a.dv, k < a.dk ? left : 0);
     }
     int last = b0;                                         // the last request of this slot
     if (a.idx) {
@@ -78,26 +84,26 @@ __global__ __launch_bounds__(NT) void la_step_kernel(const StepArgs a) {
         const IO *kk = static_cast<const IO *>(a.k) + b * a.kb + hk * a.kh;
         const IO *v = static_cast<const IO *>(a.v) + b * a.vb + h * a.vh + c0;
         const float decay = expf(a.g[b * a.gb + h * a.gh]);
-        float vv[VW], o[VW];
+        f4 vv, o = f4{0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < VW; ++e) { vv[e] = cok ? ld1(v + e) : 0.0f; o[e] = 0.0f; }
+        for (int e = 0; e < 4; ++e) vv[e] = e < left ? ld1(v + e) : 0.0f;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const int k = rg + RG * r;
             if (k < a.dk) {
                 const float kv = ld1(kk + k), qv = ld1(q + k);
 #pragma unroll
-                for (int e = 0; e < VW; ++e) {
+                for (int e = 0; e < 4; ++e) {
                     s[r][e] = fmaf(s[r][e], decay, kv * vv[e]);
                     o[e] = fmaf(s[r][e], qv, o[e]);
                 }
             }
         }
 #pragma unroll
-        for (int e = 0; e < VW; ++e) red[rg][cg * VW + e] = o[e];
+        for (int e = 0; e < 4; ++e) red[rg][cg * 4 + e] = o[e];
         __syncthreads();
-        if (tid < NC * VW) {
-            const int c = tile * NC * VW + tid;
+        if (tid < NC * 4) {
+            const int c = tile * NC * 4 + tid;
             float t = 0.0f;
 #pragma unroll
             for (int r = 0; r < RG; ++r) t += red[r][tid];
@@ -108,29 +114,19 @@ __global__ __launch_bounds__(NT) void la_step_kernel(const StepArgs a) {
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
         const int k = rg + RG * r;
-        if (cok && k < a.dk) {
-            if (VW == 4) *reinterpret_cast<f4 *>(S + (long long)k * a.dv) = f4{s[r][0], s[r][VW > 1 ? 1 : 0], s[r][VW > 2 ? 2 : 0], s[r][VW > 3 ? 3 : 0]};
-            else S[(long long)k * a.dv] = s[r][0];
-        }
+        store_columns(S + (long long)k * a.dv, k < a.dk ? left : 0, s[r]);
     }
-}
-
-template <int VW, int NC, typename IO>
-void launch_nc(const StepArgs &a, hipStream_t s) {
-    constexpr int RG = NT / NC;
-    const int tiles = (a.dv + NC * VW - 1) / (NC * VW), nr = (a.dk + RG - 1) / RG;
-    const dim3 grid((unsigned)((long long)a.B * a.H * tiles));
-    if (nr <= 1) ss2d_launch((la_step_kernel<VW, NC, 1, IO>), grid, dim3(NT), 0, s, a);
-    else if (nr <= 2) ss2d_launch((la_step_kernel<VW, NC, 2, IO>), grid, dim3(NT), 0, s, a);
-    else if (nr <= 4) ss2d_launch((la_step_kernel<VW, NC, 4, IO>), grid, dim3(NT), 0, s, a);
-    else if (nr <= 8) ss2d_launch((la_step_kernel<VW, NC, 8, IO>), grid, dim3(NT), 0, s, a);
-    else ss2d_launch((la_step_kernel<VW, NC, 128 / RG < 1 ? 1 : 128 / RG, IO>), grid, dim3(NT), 0, s, a);
 }
 
 template <typename IO>
 void launch(const StepArgs &a, hipStream_t s) {
-    if (a.dv % 4 == 0 && ((uintptr_t)a.state % 16) == 0 && a.slot_stride % 4 == 0) launch_nc<4, 16, IO>(a, s);
-    else launch_nc<1, 64, IO>(a, s);
+    constexpr int RG = NT / NC;
+    const int tiles = (a.dv + NC * 4 - 1) / (NC * 4), nr = (a.dk + RG - 1) / RG;
+    const dim3 grid((unsigned)((long long)a.B * a.H * tiles));
+    if (nr <= 1) ss2d_launch((la_step_kernel<1, IO>), grid, dim3(NT), 0, s, a);
+    else if (nr <= 2) ss2d_launch((la_step_kernel<2, IO>), grid, dim3(NT), 0, s, a);
+    else if (nr <= 4) ss2d_launch((la_step_kernel<4, IO>), grid, dim3(NT), 0, s, a);
+    else ss2d_launch((la_step_kernel<8, IO>), grid, dim3(NT), 0, s, a);
 }
 
 }  // namespace

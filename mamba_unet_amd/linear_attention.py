@@ -18,14 +18,12 @@ _MAX_DIM = 128
 
 
 def _operand(t, io):
-    """t in the storage type, its last axis dense and, where the head size allows 16-byte accesses, everything aligned for them
-    (a slice of a fused projection is used in place; a view at an odd offset is copied)."""
+    """t in the storage type, its last axis dense and its tokens apart by less than 2^22 elements and not overlapping (an expanded or far-flung view is
+    copied; a slice of a fused projection is used in place).  bf16 heads made of 16-byte pieces that begin inside a 32-bit word are copied, too."""
     if t.dtype is not io:
         t = t.to(io)
     n, s = t.shape[-1], t.stride()
-    if n > 1 and s[3] != 1:
-        return t.contiguous()
-    if n % 8 == 0 and (t.data_ptr() % 16 or (s[0] | s[1] | s[2]) % 8):
+    if (n > 1 and s[3] != 1) or not n <= s[1] < 1 << 22 or (n % 8 == 0 and io is torch.bfloat16 and (t.data_ptr() % 4 or (s[0] | s[1] | s[2]) % 2)):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 

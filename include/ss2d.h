@@ -411,8 +411,10 @@ int ss2d_seg_loss_bwd(int dtype, const void *logits, const void *labels, int lab
  * cu_seqlens null: N sequences of `tokens` tokens, rows = N.  Else N + 1 non-decreasing row offsets (device memory, clamped to [0, tokens]) of
  * sequences packed into rows = 1 row; rows outside every sequence get zero outputs and gradients.  Sequences may be empty.
  * A decay below -150 (exp underflows in fp32; -inf: a reset) counts as -150.
- * Segments: a sequence is walked in nseg pieces of seg_chunks chunks (ss2d_linattn_segments, from the tokens of all sequences and the longest one:
- * nseg << 32 | seg_chunks; the last piece takes the rest); nseg > 1 needs seg_states (N * H * nseg * dk * dv floats) and seg_decay (N * H * nseg doubles) as scratch memory.
+ * Segments: long sequences are walked in pieces of seg_chunks chunks side by side.  ss2d_linattn_segments, from the tokens of all sequences and the
+ * longest one, returns nseg << 32 | seg_chunks.  nseg == 1: none is split.  Else seg_states (slots * H * dk * dv floats) and seg_decay (slots * H
+ * doubles) are scratch memory; a batch has nseg pieces of each sequence, the last one taking the rest (slots = N * nseg), packed sequences have as
+ * many as they need (slots = tokens / (seg_chunks * chunk) + N, chunk = ss2d_linattn_chunk).
  * chunk_states (null: none): the forward leaves the state in front of every chunk of ss2d_linattn_chunk(dtype, dk, dv) tokens there for the backward:
  * slots * H * ss2d_linattn_state_floats(dtype, dk, dv) floats with slots = N * ceil(tokens / chunk), packed: tokens / chunk + N. */
 long long ss2d_linattn_state_floats(int dtype, int dk, int dv);

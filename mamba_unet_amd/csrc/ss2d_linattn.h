@@ -20,7 +20,8 @@ struct Problem {
     long long tokens;             // tokens of a row (batch: the length of every sequence)
     int N, H, G, dk, dv;
     float scale;
-    int nseg, segc;               // segments of a sequence, chunks a segment
+    int nseg, segc;               // segments a sequence may have (1: not split), chunks a segment
+    int slots;                    // segments of all sequences: the walks of a head
     int vec;                      // rows are made of 16-byte pieces that begin on 32-bit words
 };
 
@@ -47,7 +48,28 @@ __device__ __forceinline__ Seq get_seq(const Problem &p, int n) {
     }
     return s;
 }
-// a sequence's last segment takes whatever is left: the number of segments comes from a hint of the longest sequence
+// Segments.  A batch has nseg of each sequence, the last one takes whatever is left.  Packed sequences have as many as they need: floor(start / span) + n is
+// a sequence's first slot, which leaves room for every earlier sequence's last, partly filled segment, and a walk finds its sequence by bisection.
+__device__ __forceinline__ int first_slot(const Problem &p, int n, int C) {
+    if (!p.cu || p.nseg == 1) return n * p.nseg;
+    const long long a = p.cu[n];
+    return (int)((unsigned)(a < 0 ? 0 : a > p.tokens ? p.tokens : a) / (unsigned)(p.segc * C)) + n;
+}
+__device__ __forceinline__ void walk_of(const Problem &p, int slot, int C, int &n, int &seg) {       // seg < 0: a slot of no sequence
+    if (!p.cu || p.nseg == 1) {
+        n = slot / p.nseg;
+        seg = slot % p.nseg;
+        return;
+    }
+    int lo = 0, hi = p.N - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first_slot(p, mid, C) <= slot) lo = mid;
+        else hi = mid - 1;
+    }
+    n = lo;
+    seg = slot - first_slot(p, lo, C);
+}
 __device__ __forceinline__ int segment_end(const Problem &p, int seg, int nch) {
     const long long e = (long long)(seg + 1) * p.segc;
     return seg + 1 == p.nseg || e > nch ? nch : (int)e;
@@ -191,6 +213,17 @@ struct TileRegs {
             }
         }
     }
+    // whether a NaN or an infinity is among the values: an exponent of ones carries into the sign's place
+    __device__ __forceinline__ bool not_finite() const {
+        unsigned any = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= (v[j][i] & 0x7f807f80u) + 0x00800080u;
+#pragma unroll
+        for (int j = 0; j < (VEC ? 0 : N); ++j) any |= (last[j] & 0x7f807f80u) + 0x00800080u;     // (words past a row's end: a false alarm only costs time)
+        return any & 0x80008000u;
+    }
     // ORDERED: 32-column blocks in operand order (frag_p)
     template <bool ORDERED = false>
     __device__ __forceinline__ void put(unsigned char *tile, int pitch, int D) const {
@@ -237,6 +270,17 @@ struct TileRegsF {
             const int at = VEC || (int)threadIdx.x / PR + j * STEP < n ? voff : SS2D_BUF_OOR;
             v[j] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, j * STEP * (int)ld * 4, 0));
         }
+    }
+    __device__ __forceinline__ bool not_finite() const {
+        unsigned any = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = v[j][i];
+                any |= (__builtin_bit_cast(unsigned, x) & 0x7f800000u) + 0x00800000u;
+            }
+        return any & 0x80000000u;
     }
     __device__ __forceinline__ void put(float *tile, int D) const {
         const int c = 4 * (threadIdx.x % PR);
@@ -301,7 +345,7 @@ inline int linattn_chunk(int dtype, int dk, int dv) { return dtype || (dk <= 64 
 // Segments.  One workgroup walks a segment; with fewer workgroups than the card holds at once (two or three a CU) it idles, and a segment
 // costs a second pass over k and v (q and dout in the backward) and a state's round trip: so all tokens of all sequences and
 // heads are dealt to that many workgroups, at least four chunks each.
-// Returns the segments of the longest sequence in the upper and the chunks a segment in the lower 32 bits.
+// Returns the segments of the longest sequence in the upper and the chunks a segment in the lower 32 bits; 1 segment: no sequence is split.
 inline long long linattn_segments(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
     const int C = linattn_chunk(dtype, dk, dv);
     const long long nch = (max_len + C - 1) / C, all = (all_tokens + C - 1) / C * H * (backward || dtype ? 1 : (dv + 63) / 64);
@@ -317,6 +361,11 @@ inline long long linattn_state_floats(int dtype, int dk, int dv) {
     return dtype ? (long long)(dk <= 32 ? 32 : dk <= 64 ? 64 : 128) * (dv <= 64 ? 64 : 128) : (long long)dk * dv;
 }
 
+// segments of all sequences, in front of which a state is kept
+inline long long linattn_slots(int packed, long long N, long long tokens, long long nseg, long long segc, int C) {
+    return nseg == 1 ? N : packed ? tokens / (segc * C) + N : N * nseg;
+}
+
 inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, const void *v, const float *g, const long long *st, const int *cu,
                            int N, long long tokens, int H, int G, int dk, int dv, float scale, int nseg, int segc, const char *name) {
     if (dtype != 0 && dtype != 1) { ss2d_set_error("%s: unknown dtype %d", name, dtype); return -1; }
@@ -325,7 +374,12 @@ inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, 
     if (H % G) { ss2d_set_error("%s: %d heads are not a multiple of %d key heads", name, H, G); return -4; }
     if (dk < 1 || dk > 128 || dv < 1 || dv > 128) { ss2d_set_error("%s: dk %d and dv %d must be 1 ... 128", name, dk, dv); return -5; }
     if ((long long)H * dk >= (1 << 22) || (long long)H * dv >= (1 << 22)) { ss2d_set_error("%s: %d heads are too many", name, H); return -6; }
-    if ((long long)N * H * nseg * 2 > 0x7ffffff0LL || (long long)N * H > 65535LL * 32) { ss2d_set_error("%s: too many sequences and heads", name); return -6; }
+    const int C = linattn_chunk(dtype, dk, dv);
+    if (segc > 0x7fffffff / C) segc = 0x7fffffff / C;
+    const long long slots = linattn_slots(cu ? 1 : 0, N, tokens, nseg, segc, C);
+    if (slots * H * 2 > 0x7ffffff0LL || (long long)N * H > 65535LL * 32) { ss2d_set_error("%s: too many sequences and heads", name); return -6; }
+    if (cu && nseg > 1) nseg = 0x7fffffff;
+    p.slots = (int)slots;
     p.q = q; p.k = k; p.v = v; p.g = g; p.cu = cu; p.tokens = tokens; p.N = N; p.H = H; p.G = G; p.dk = dk; p.dv = dv; p.scale = scale; p.nseg = nseg; p.segc = segc;
     p.qb = st[0]; p.ql = st[1]; p.qh = st[2]; p.kb = st[3]; p.kl = st[4]; p.kh = st[5];
     p.vb = st[6]; p.vl = st[7]; p.vh = st[8]; p.gb = st[9]; p.gl = st[10]; p.gh = st[11];
@@ -348,4 +402,4 @@ inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, 
 
 // the pass over segments that leaves their own contributions (forward: k v^T; reverse: q dout^T, with q in the place of k and dout in that of v),
 // defined beside the forward
-void linattn_segment_pass(int dtype, const linattn::Problem &p, float *seg_states, double *seg_decay, const float *want_end, bool reverse, hipStream_t s);
+void linattn_segment_pass(int dtype, const linattn::Problem &p, float *seg_states, double *seg_decay, bool reverse, hipStream_t s);

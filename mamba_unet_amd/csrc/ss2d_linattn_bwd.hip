@@ -42,35 +42,35 @@ __device__ __forceinline__ float row16_sum(float v) {
     return v;
 }
 
-// seg_states[s] = D behind segment s
+// seg_states[slot] = D behind the segment
 __global__ __launch_bounds__(NT) void la_join_bwd_kernel(const BwdArgs a, int C) {
     const Problem &p = a.p;
     const long long sz = (long long)p.dk * p.dv;
-    const long long e = (long long)blockIdx.x * NT + threadIdx.x;
-    const long long nh = blockIdx.y;
-    if (e >= sz) return;
-    const Seq s = get_seq(p, (int)(nh / p.H));
-    const int nch = (s.len + C - 1) / C, ns = segments_of(p, nch);
+    const int tiles = (int)((sz + NT - 1) / NT), nh = blockIdx.x / tiles, n = nh / p.H;
+    const long long e = (long long)(blockIdx.x % tiles) * NT + threadIdx.x;
+    const Seq s = get_seq(p, n);
+    const int ns = segments_of(p, (s.len + C - 1) / C);
+    if (e >= sz || ns <= 1) return;
     float v = a.dlast ? a.dlast[nh * sz + e] : 0.0f;
-    float *u = a.seg_states + nh * p.nseg * sz + e;
-    const double *d = a.seg_decay + nh * p.nseg;
+    const long long first = (long long)first_slot(p, n, C) * p.H + nh % p.H, step = p.H * sz;
+    float *u = a.seg_states + first * sz + e;
+    const double *d = a.seg_decay + first;
     for (int i = ns - 1; i >= 0; i -= 8) {
         float own[8], f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int k = i - j > 0 ? i - j : 0;
-            own[j] = u[k * sz];
-            f[j] = hw_exp2((float)d[k]);
+            const int k = i - j > 1 ? i - j : 1;             // (the first segment's contribution is not there, and not used)
+            own[j] = u[k * step];
+            f[j] = hw_exp2((float)d[(long long)k * p.H]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (i - j >= 0) {
-                u[(i - j) * sz] = v;
+                u[(i - j) * step] = v;
                 v = v * f[j] + own[j];
             }
         }
     }
-    if (a.ds0) a.ds0[nh * sz + e] = v;
 }
 
 template <typename IO>
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int walks = p.N * p.H * p.nseg;
+    const int walks = p.slots * p.H;
     const int hq = p.H > p.G ? p.H : p.G;                            // heads of dq / dk as written
     if ((int)blockIdx.x >= walks) {                                  // packed rows that belong to no sequence
         const int w = (int)blockIdx.x - walks;
@@ -109,7 +109,10 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
     }
     int id = xcd_remap(blockIdx.x, walks);
     const int h = id % p.H; id /= p.H;
-    const int seg = id % p.nseg, n = id / p.nseg;
+    const int slot = id;
+    int n, seg;
+    walk_of(p, slot, C, n, seg);
+    if (seg < 0) return;
     const Seq s = get_seq(p, n);
     const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
     const int c1 = segment_end(p, seg, nch);
@@ -136,7 +139,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
     };
     f4 D[TW], sr[TW];
     {
-        const float *init = p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
+        const float *init = segments_of(p, nch) > 1 ? a.seg_states + ((long long)slot * p.H + h) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
 #pragma unroll
         for (int m = 0; m < TW; ++m)
 #pragma unroll
@@ -375,7 +378,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
     }
     __syncthreads();
     if (c0 < c1) finish_dg(c0);
-    if (a.ds0 && p.nseg == 1) {
+    if (a.ds0 && c0 == 0) {
         float *d = a.ds0 + nh * sz;
 #pragma unroll
         for (int m = 0; m < TW; ++m)
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int walks = p.N * p.H * p.nseg;
+    const int walks = p.slots * p.H;
     const int hq = p.H > p.G ? p.H : p.G;                            // heads of dq / dk as written
     if ((int)blockIdx.x >= walks) {                                  // packed rows that belong to no sequence
         const int w = (int)blockIdx.x - walks;
@@ -417,7 +420,10 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     }
     int id = xcd_remap(blockIdx.x, walks);
     const int h = id % p.H; id /= p.H;
-    const int seg = id % p.nseg, n = id / p.nseg;
+    const int slot = id;
+    int n, seg;
+    walk_of(p, slot, C, n, seg);
+    if (seg < 0) return;
     const Seq s = get_seq(p, n);
     const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
     const int c1 = segment_end(p, seg, nch);
@@ -466,7 +472,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     if (c0 < c1) fetch(c1 - 1);
     {
         const int col = 16 * vt + (lane0 & 15);
-        const float *init = p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
+        const float *init = segments_of(p, nch) > 1 ? a.seg_states + ((long long)slot * p.H + h) * sz : a.dlast ? a.dlast + nh * sz : nullptr;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
@@ -746,7 +752,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
     }
     __syncthreads();
     if (c0 < c1) finish_dg(c0);
-    if (a.ds0 && p.nseg == 1) {
+    if (a.ds0 && c0 == 0) {
         const int col = 16 * vt + (lane0 & 15);
         float *d = a.ds0 + nh * sz;
 #pragma unroll
@@ -788,7 +794,7 @@ void launch_head_sum(const float *a, const float *b, void *oa, void *ob, long lo
 
 template <int DK, int DV, int C>
 void launch_bwd(const BwdArgs &a, unsigned gaps, hipStream_t s) {
-    const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg);
+    const unsigned walks = (unsigned)((long long)a.p.slots * a.p.H);
     if (a.p.vec) ss2d_launch((la_bwd_kernel<DK, DV, C, true>), dim3(walks + gaps), dim3(1024), 0, s, a);
     else ss2d_launch((la_bwd_kernel<DK, DV, C, false>), dim3(walks + gaps), dim3(1024), 0, s, a);
 }
@@ -807,7 +813,7 @@ void dispatch_bwd_f32(const BwdArgs &a, unsigned gaps, hipStream_t s) {
 
 template <int DK, int DV, bool VEC>
 void launch_bwd_bf16(const BwdArgs &a, unsigned gaps, hipStream_t s) {
-    const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg);
+    const unsigned walks = (unsigned)((long long)a.p.slots * a.p.H);
     constexpr int NW = DK <= 32 ? 8 : 16;
     if (a.p.H > a.p.G) ss2d_launch((la_bwd_bf16_kernel<DK, DV, NW, VEC, float>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
     else ss2d_launch((la_bwd_bf16_kernel<DK, DV, NW, VEC, bf16>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
@@ -849,9 +855,8 @@ extern "C" int ss2d_linattn_bwd(int dtype, const void *q, const void *k, const v
         Problem r = a.p;                          // q in the place of k, dout in that of v
         r.k = q; r.kb = r.qb; r.kl = r.ql; r.kh = r.qh;
         r.v = dout; r.vb = tokens * H * dv; r.vl = (long long)H * dv; r.vh = dv;
-        linattn_segment_pass(dtype, r, seg_states, seg_decay, ds0, true, s);
-        const long long sz = (long long)dk * dv;
-        ss2d_launch(la_join_bwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(N * H)), dim3(NT), 0, s, a, linattn_chunk(dtype, dk, dv));
+        linattn_segment_pass(dtype, r, seg_states, seg_decay, true, s);
+        ss2d_launch(la_join_bwd_kernel, dim3((unsigned)((dk * dv + NT - 1) / NT * N * H)), dim3(NT), 0, s, a, linattn_chunk(dtype, dk, dv));
     }
     if (dtype == SS2D_DTYPE_F32) dispatch_bwd_f32(a, gaps, s);
     else if (a.p.vec) dispatch_bwd_bf16<true>(a, gaps, s);

@@ -20,8 +20,8 @@ struct FwdArgs {
     const float *s0;              // (N, H, dk, dv) or null
     float *last;                  // (N, H, dk, dv) or null
     float *chunk_states;          // (slots, H, dk, dv): the state in front of every chunk, or null
-    float *seg_states;            // (N, H, nseg, dk, dv): contributions, then the states in front of the segments; null with nseg == 1
-    double *seg_decay;            // (N, H, nseg): log2 of a segment's decay
+    float *seg_states;            // (slots, H, dk, dv): contributions, then the states in front of the segments; null with nseg == 1
+    double *seg_decay;            // (slots, H): log2 of a segment's decay
 };
 
 constexpr int GAP_WGS = 16;
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, gq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int dvt = (p.dv + 63) / 64, walks = p.N * p.H * p.nseg * dvt;
+    const int dvt = (p.dv + 63) / 64, walks = p.slots * p.H * dvt;
     if ((int)blockIdx.x >= walks) {              // packed rows that belong to no sequence: their output is zero
         if (MODE == 0) zero_gaps(p, static_cast<float *>(a.o), (long long)p.H * p.dv, blockIdx.x - walks);
         return;
@@ -56,14 +56,17 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     int id = xcd_remap(blockIdx.x, walks);
     const int vt = id % dvt; id /= dvt;
     const int h = id % p.H; id /= p.H;
-    const int seg = id % p.nseg, n = id / p.nseg;
+    const int slot = id;
+    int n, seg;
+    walk_of(p, slot, C, n, seg);
+    if (seg < 0) return;
     const Seq s = get_seq(p, n);
     const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
     const int c1 = segment_end(p, seg, nch);
     const bool empty = s.len == 0;
     if (c0 >= c1 && !(empty && seg == 0)) return;
-    if (MODE == 1 && c1 == nch && !empty && !a.last) return;     // nothing starts from the last segment's end
-    if (MODE == 2 && c0 == 0 && !a.last) return;                 // (here: the gradient in front of the first segment is not wanted)
+    if (MODE == 1 && c1 == nch) return;          // no segment starts from the last one's end
+    if (MODE == 2 && c0 == 0) return;            // (here: from the first one's)
     const int hk = h / (p.H / p.G), col = 64 * vt + 16 * wave + l16, first = MODE == 2 ? c1 - 1 : c0, dvc = p.dv - 64 * vt;
     const bool cok = col < p.dv;
     const float *Q = static_cast<const float *>(p.q) + s.row * p.qb + (s.start + (long long)c0 * C) * p.ql + hk * p.qh;
@@ -73,7 +76,7 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     const long long ldo = (long long)p.H * p.dv, nh = (long long)n * p.H + h, sz = (long long)p.dk * p.dv;
     float *O = static_cast<float *>(a.o) + ((s.row * p.tokens + s.start + (long long)c0 * C) * p.H + h) * (long long)p.dv;
     f4 S[KT];
-    const float *init = MODE >= 1 ? nullptr : p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
+    const float *init = MODE >= 1 ? nullptr : segments_of(p, nch) > 1 ? a.seg_states + ((long long)slot * p.H + h) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -118,6 +121,10 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     scan(first);
     fetch_g(first + STEP);
     if (c0 < c1) fetch(first);
+    // A NaN or an infinity in v_j times the zero weight of an earlier row would reach that row.  Once one has been met, such values stay out of the
+    // products and are added to the rows from j on alone, and their columns of the state become NaN.
+    float *poison = decays + 300;                // (the first chunk's set of decays ends at 257)
+    if (MODE == 0 && tid == 0) *poison = 0.0f;
 #pragma unroll 1
     for (int c = first; c >= c0 && c < c1; c += STEP) {
         const int nr = rows_of(c);
@@ -140,6 +147,7 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
         if (MODE == 0) qr.put(Qs, p.dk);
         kr.put(Ks, p.dk);
         vr.put(Vs, dvc);
+        if (MODE == 0 && vr.not_finite()) *poison = 1.0f;
         if (c + STEP >= c0 && c + STEP < c1) fetch(c + STEP);
         __syncthreads();
         const float *bh = decays + (c & 1) * 320, *bl = bh + 64, *eb = bl + 64, *wt = eb + 64, *tail = wt + 64;
@@ -172,6 +180,19 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
         for (int jt = 0; jt < CT; ++jt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) vv[jt][r] = Vs[(16 * jt + 4 * gq + r) * PV + 16 * wave + l16];
+        float eend = tail[0];
+        const bool poisoned = MODE == 0 && *poison != 0.0f;
+        if (poisoned) {
+            int bad = 0;
+#pragma unroll
+            for (int jt = 0; jt < CT; ++jt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!__builtin_isfinite(vv[jt][r])) { vv[jt][r] = 0.0f; bad = 1; }
+            bad |= __shfl_xor(bad, 16, 64);
+            bad |= __shfl_xor(bad, 32, 64);
+            if (bad) eend = __builtin_nanf("");
+        }
         if (MODE == 0) {
             f4 acc[CT];
 #pragma unroll
@@ -194,6 +215,18 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
                     for (int r = 0; r < 4; ++r) acc[it] = mfma4(x[r], vv[jt][r], acc[it]);
                 }
             }
+            if (poisoned) {
+#pragma unroll 1
+                for (int j = 0; j < C; ++j) {
+                    const float x = Vs[j * PV + 16 * wave + l16];
+                    if (__builtin_isfinite(x)) continue;
+#pragma unroll
+                    for (int it = 0; it < CT; ++it)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (j <= 16 * it + 4 * gq + r) acc[it][r] += Ps[(16 * it + 4 * gq + r) * PP + j] * x;
+                }
+            }
             const RowsOut out(O, nr, ldo);
 #pragma unroll
             for (int it = 0; it < CT; ++it)
@@ -203,7 +236,6 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
         }
         scan(c + STEP);
         fetch_g(c + 2 * STEP);
-        const float eend = tail[0];
 #pragma unroll
         for (int t = 0; t < KT; ++t) S[t] *= eend;
 #pragma unroll
@@ -217,7 +249,7 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
                 for (int r = 0; r < 4; ++r) S[t] = mfma4(Ks[(16 * jt + 4 * gq + r) * PK + 16 * t + l16], vv[jt][r], S[t]);
         }
     }
-    float *dst = MODE >= 1 ? a.seg_states + (nh * p.nseg + seg) * sz : (a.last && p.nseg == 1) ? a.last + nh * sz : nullptr;
+    float *dst = MODE >= 1 ? a.seg_states + ((long long)slot * p.H + h) * sz : a.last && c1 == nch ? a.last + nh * sz : nullptr;
     if (dst) {
 #pragma unroll
         for (int t = 0; t < KT; ++t)
@@ -226,7 +258,7 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
                 const int k = 16 * t + 4 * gq + r;
                 if (cok && k < p.dk) dst[k * p.dv + col] = S[t][r];
             }
-        if (MODE >= 1 && tid == 0 && vt == 0) a.seg_decay[nh * p.nseg + seg] = total;
+        if (MODE >= 1 && tid == 0 && vt == 0) a.seg_decay[(long long)slot * p.H + h] = total;
     }
 }
 
@@ -244,21 +276,24 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int walks = p.N * p.H * p.nseg;
+    const int walks = p.slots * p.H;
     if ((int)blockIdx.x >= walks) {              // packed rows that belong to no sequence: their output is zero
         if (MODE == 0) zero_gaps(p, static_cast<bf16 *>(a.o), (long long)p.H * p.dv, blockIdx.x - walks);
         return;
     }
     int id = xcd_remap(blockIdx.x, walks);       // heads of a group run next to each other on one XCD: they read the same q and k
     const int h = id % p.H; id /= p.H;
-    const int seg = id % p.nseg, n = id / p.nseg;
+    const int slot = id;
+    int n, seg;
+    walk_of(p, slot, C, n, seg);
+    if (seg < 0) return;
     const Seq s = get_seq(p, n);
     const int c0 = seg * p.segc, nch = (s.len + C - 1) / C;
     const int c1 = segment_end(p, seg, nch);
     const bool empty = s.len == 0;
     if (c0 >= c1 && !(empty && seg == 0)) return;
-    if (MODE == 1 && c1 == nch && !empty && !a.last) return;     // nothing starts from the last segment's end
-    if (MODE == 2 && c0 == 0 && !a.last) return;                 // (here: the gradient in front of the first segment is not wanted)
+    if (MODE == 1 && c1 == nch) return;          // no segment starts from the last one's end
+    if (MODE == 2 && c0 == 0) return;            // (here: from the first one's)
     const int hk = h / (p.H / p.G), first = MODE == 2 ? c1 - 1 : c0;
     const bf16 *Q = static_cast<const bf16 *>(p.q) + s.row * p.qb + (s.start + (long long)c0 * C) * p.ql + hk * p.qh;
     const bf16 *K = static_cast<const bf16 *>(p.k) + s.row * p.kb + (s.start + (long long)first * C) * p.kl + hk * p.kh;
@@ -286,7 +321,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
     };
     fetch_g(first);
     if (c0 < c1) fetch(first);
-    const float *init = MODE >= 1 ? nullptr : p.nseg > 1 ? a.seg_states + (nh * p.nseg + seg) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
+    const float *init = MODE >= 1 ? nullptr : segments_of(p, nch) > 1 ? a.seg_states + ((long long)slot * p.H + h) * sz : a.s0 ? a.s0 + nh * sz : nullptr;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -317,6 +352,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
         *reinterpret_cast<u32x2 *>(Ph + at) = u32x2{0, 0};
         *reinterpret_cast<u32x2 *>(Pl + at) = u32x2{0, 0};
     }
+    // A NaN or an infinity in v_j times the zero weight of an earlier row would reach that row.  Once one has been met, such values stay out of the
+    // products and are added to the rows from j on alone, and their columns of the state become NaN.
+    float *poison = decays + 300;                // (the first chunk's set of decays ends at 257)
+    if (MODE == 0 && tid == 0) *poison = 0.0f;
 #pragma unroll 1
     for (int c = first; c >= c0 && c < c1; c += STEP) {
         const int nr = rows_of(c);
@@ -329,6 +368,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
         if (MODE == 0) qr.template put<true>(Qs, QP, p.dk);
         kr.put(Ks, KP, p.dk);
         vr.put(Vs, VP, p.dv);
+        if (MODE == 0 && vr.not_finite()) *poison = 1.0f;
         Q += C * p.ql; K += STEP * C * p.kl; V += STEP * C * p.vl;
         if (MODE >= 1 && c + STEP >= c0 && c + STEP < c1) fetch(c + STEP);
         const float *bh = decays + (c & 1) * 5 * C, *bl = bh + C, *eb = bl + C, *wt = eb + C, *tail = wt + C;
@@ -365,6 +405,25 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
         bf16x8 vf[2];
 #pragma unroll
         for (int js = 0; js < 2; ++js) vf[js] = frag_t(Vs, VP, wave, js, lane);
+        float eend = tail[0];
+        const bool poisoned = MODE == 0 && *poison != 0.0f;
+        if (poisoned) {
+            int bad = 0;
+#pragma unroll
+            for (int js = 0; js < 2; ++js) {
+                u32x4 w = __builtin_bit_cast(u32x4, vf[js]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned m = ((w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;       // the halves that are not finite
+                    bad |= m != 0;
+                    w[i] &= ~(m | (m - (m >> 15)));
+                }
+                vf[js] = __builtin_bit_cast(bf16x8, w);
+            }
+            bad |= __shfl_xor(bad, 16, 64);
+            bad |= __shfl_xor(bad, 32, 64);
+            if (bad) eend = __builtin_nanf("");
+        }
         if (MODE == 0) {
             f4 acc[4];
 #pragma unroll
@@ -391,6 +450,23 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
                     acc[it] = mfma8(vf[js], frag_p(Pl, PP, 16 * it + l16, js, gq), acc[it]);
                 }
             }
+            if (poisoned) {
+#pragma unroll 1
+                for (int j = 0; j < C; ++j) {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(Vs + j * VP + 2 * (16 * wave + 4 * gq));
+                    const f2 x0 = bf16pair_to_f2(x.x), x1 = bf16pair_to_f2(x.y);
+                    const float v[4] = {x0.x, x0.y, x1.x, x1.y};
+                    const int at = 2 * (operand_pos(j & ~3) + (j & 3));
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) {
+                        const unsigned char *w = Ph + (16 * it + l16) * PP + at;
+                        const float ph = (float)*reinterpret_cast<const bf16 *>(w), pl = (float)*reinterpret_cast<const bf16 *>(w + (Pl - Ph));
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (j <= 16 * it + l16 && !__builtin_isfinite(v[r])) acc[it][r] += (ph + pl) * v[r];
+                    }
+                }
+            }
 #pragma unroll
             for (int it = 0; it < 4; ++it) out.template put4<VEC>(O, 16 * it + l16, 16 * wave + 4 * gq, ldo, p.dv, acc[it]);
             O += C * ldo;
@@ -399,7 +475,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
         if (MODE == 0 && c + 1 < c1) fetch(c + 1);   // in flight during the state's products; earlier, its registers would cost a workgroup a CU
         scan(c + STEP);
         fetch_g(c + 2 * STEP);
-        const float eend = tail[0];
         bf16x8 vw[2][3];
 #pragma unroll
         for (int js = 0; js < 2; ++js) {
@@ -420,7 +495,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
             }
         }
     }
-    float *dst = MODE >= 1 ? a.seg_states + (nh * p.nseg + seg) * sz : (a.last && p.nseg == 1) ? a.last + nh * sz : nullptr;
+    float *dst = MODE >= 1 ? a.seg_states + ((long long)slot * p.H + h) * sz : a.last && c1 == nch ? a.last + nh * sz : nullptr;
     if (dst) {
 #pragma unroll
         for (int t = 0; t < KT; ++t)
@@ -429,44 +504,44 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
                 const int k = 16 * t + 4 * (lane0 >> 4) + r;
                 if (col < p.dv && k < p.dk) dst[k * p.dv + col] = S[t][r];
             }
-        if (MODE >= 1 && tid == 0) a.seg_decay[nh * p.nseg + seg] = total;
+        if (MODE >= 1 && tid == 0) a.seg_decay[(long long)slot * p.H + h] = total;
     }
 }
 
-// joins the segments of a (sequence, head): seg_states[s] = state in front of segment s; one thread per state element
+// joins the segments of a (sequence, head): seg_states[slot] = state in front of the segment; one thread per state element
 __global__ __launch_bounds__(NT) void la_join_fwd_kernel(const FwdArgs a, int C) {
     const Problem &p = a.p;
     const long long sz = (long long)p.dk * p.dv;
-    const long long e = (long long)blockIdx.x * NT + threadIdx.x;
-    const long long nh = blockIdx.y;
-    if (e >= sz) return;
-    const Seq s = get_seq(p, (int)(nh / p.H));
-    const int nch = (s.len + C - 1) / C, ns = segments_of(p, nch);
+    const int tiles = (int)((sz + NT - 1) / NT), nh = blockIdx.x / tiles, n = nh / p.H;
+    const long long e = (long long)(blockIdx.x % tiles) * NT + threadIdx.x;
+    const Seq s = get_seq(p, n);
+    const int ns = segments_of(p, (s.len + C - 1) / C);
+    if (e >= sz || ns <= 1) return;
     float v = a.s0 ? a.s0[nh * sz + e] : 0.0f;
-    float *u = a.seg_states + nh * p.nseg * sz + e;
-    const double *d = a.seg_decay + nh * p.nseg;
+    const long long first = (long long)first_slot(p, n, C) * p.H + nh % p.H, step = p.H * sz;
+    float *u = a.seg_states + first * sz + e;
+    const double *d = a.seg_decay + first;
     for (int i = 0; i < ns; i += 8) {                       // eight segments' loads are in flight at once
         float own[8], f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int k = i + j < ns ? i + j : ns - 1;      // (without `last` the last segment's contribution is not there, and not used)
-            own[j] = u[k * sz];
-            f[j] = hw_exp2((float)d[k]);
+            const int k = i + j < ns - 1 ? i + j : ns - 2;  // (the last segment's contribution is not there, and not used)
+            own[j] = u[k * step];
+            f[j] = hw_exp2((float)d[(long long)k * p.H]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (i + j < ns) {
-                u[(i + j) * sz] = v;
+                u[(i + j) * step] = v;
                 v = v * f[j] + own[j];
             }
         }
     }
-    if (a.last) a.last[nh * sz + e] = v;
 }
 
 template <int MODE, bool VEC, int DK, int C>
 void launch_f32(const FwdArgs &a, unsigned gaps, hipStream_t s) {
-    const unsigned walks = (unsigned)((long long)a.p.N * a.p.H * a.p.nseg * ((a.p.dv + 63) / 64));
+    const unsigned walks = (unsigned)((long long)a.p.slots * a.p.H * ((a.p.dv + 63) / 64));
     ss2d_launch((la_fwd_kernel<DK, C, MODE, VEC>), dim3(walks + gaps), dim3(NT), 0, s, a);
 }
 template <int MODE, bool VEC>
@@ -479,7 +554,7 @@ void dispatch_f32(const FwdArgs &a, unsigned gaps, hipStream_t s) {
 }
 template <int MODE, bool VEC, int DK, int NW>
 void launch_bf16(const FwdArgs &a, unsigned gaps, hipStream_t s) {
-    ss2d_launch((la_fwd_bf16_kernel<DK, NW, MODE, VEC>), dim3((unsigned)((long long)a.p.N * a.p.H * a.p.nseg) + gaps), dim3(64 * NW), 0, s, a);
+    ss2d_launch((la_fwd_bf16_kernel<DK, NW, MODE, VEC>), dim3((unsigned)((long long)a.p.slots * a.p.H) + gaps), dim3(64 * NW), 0, s, a);
 }
 template <int MODE, bool VEC>
 void dispatch_bf16(const FwdArgs &a, unsigned gaps, hipStream_t s) {
@@ -502,10 +577,9 @@ void dispatch(int dtype, const FwdArgs &a, unsigned gaps, hipStream_t s) {
 
 }  // namespace
 
-void linattn_segment_pass(int dtype, const linattn::Problem &p, float *seg_states, double *seg_decay, const float *want_end, bool reverse, hipStream_t s) {
+void linattn_segment_pass(int dtype, const linattn::Problem &p, float *seg_states, double *seg_decay, bool reverse, hipStream_t s) {
     FwdArgs a{};
     a.p = p; a.seg_states = seg_states; a.seg_decay = seg_decay;
-    a.last = const_cast<float *>(want_end);      // only asked for being there
     reverse ? dispatch<2>(dtype, a, 0, s) : dispatch<1>(dtype, a, 0, s);
 }
 
@@ -528,9 +602,8 @@ extern "C" int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const v
     const unsigned gaps = cu_seqlens ? GAP_WGS : 0;
     hipStream_t s = (hipStream_t)stream;
     if (nseg > 1) {
-        linattn_segment_pass(dtype, a.p, seg_states, seg_decay, last, false, s);
-        const long long sz = (long long)dk * dv;
-        ss2d_launch(la_join_fwd_kernel, dim3((unsigned)((sz + NT - 1) / NT), (unsigned)(N * H)), dim3(NT), 0, s, a, linattn_chunk(dtype, dk, dv));
+        linattn_segment_pass(dtype, a.p, seg_states, seg_decay, false, s);
+        ss2d_launch(la_join_fwd_kernel, dim3((unsigned)((dk * dv + NT - 1) / NT * N * H)), dim3(NT), 0, s, a, linattn_chunk(dtype, dk, dv));
     }
     dispatch<0>(dtype, a, gaps, s);
     rc = ss2d_take_launch_rc();

@@ -87,14 +87,14 @@ def _strides(q, k, v, g):
     return _TWELVE(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *gs)
 
 
-def _segments(lib, dev, code, N, tokens, H, longest, dk, dv, backward):
+def _segments(lib, dev, code, N, rows, L, H, longest, dk, dv, packed, backward):
     """(segments, chunks a segment, state scratch, decay scratch)"""
-    plan = lib.ss2d_linattn_segments(code, tokens, longest, H, dk, dv, backward)
+    plan = lib.ss2d_linattn_segments(code, rows * L, longest, H, dk, dv, backward)
     nseg, segc = plan >> 32, plan & 0xffffffff
     if nseg == 1:
         return 1, segc, None, None
-    return (nseg, segc, torch.empty((N, H, nseg, dk, dv), device=dev, dtype=torch.float32),
-            torch.empty((N, H, nseg), device=dev, dtype=torch.float64))
+    slots = L // (segc * lib.ss2d_linattn_chunk(code, dk, dv)) + N if packed else N * nseg
+    return (nseg, segc, torch.empty((slots, H, dk, dv), device=dev, dtype=torch.float32), torch.empty((slots, H), device=dev, dtype=torch.float64))
 
 
 def _ptr(t):
@@ -118,7 +118,7 @@ def _forward(q, k, v, g, s0, cu, scale, dims, longest, want_last, want_chunks):
         C = lib.ss2d_linattn_chunk(code, dk, dv)
         slots = N * -(-L // C) if cu is None else L // C + N
         chunks = torch.empty((slots, H, lib.ss2d_linattn_state_floats(code, dk, dv)), device=dev, dtype=torch.float32)
-    nseg, segc, ws, wd = _segments(lib, dev, code, N, B * L, H, longest, dk, dv, 0)
+    nseg, segc, ws, wd = _segments(lib, dev, code, N, B, L, H, longest, dk, dv, cu is not None, 0)
     args = (code, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), _strides(q, k, v, g), _ptr(cu), _ptr(s0), out.data_ptr(), _ptr(last), _ptr(chunks),
             _ptr(ws), _ptr(wd), N, L, H, G, dk, dv, scale, nseg, segc)
     stream = _lib.stream_of(dev.index)
@@ -167,7 +167,7 @@ class LinearAttentionFn(torch.autograd.Function):
         hq, hk = [torch.empty((B, L, H, dk), device=dev, dtype=torch.float32) for _ in range(2)] if H > G else (None, None)
         lib = _lib.load()
         code = _BF16 if io is torch.bfloat16 else _F32
-        nseg, segc, ws, wd = _segments(lib, dev, code, N, B * L, H, longest, dk, dv, 1)
+        nseg, segc, ws, wd = _segments(lib, dev, code, N, B, L, H, longest, dk, dv, cu is not None, 1)
         args = (code, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), _strides(q, k, v, g), _ptr(cu), go.data_ptr(), _ptr(gl), chunks.data_ptr(),
                 dq.data_ptr(), dk_.data_ptr(), dv_.data_ptr(), dg.data_ptr(), _ptr(ds0), _ptr(hq), _ptr(hk), _ptr(ws), _ptr(wd), N, L, H, G, dk, dv, scale, nseg, segc)
         stream = _lib.stream_of(dev.index)
@@ -191,7 +191,7 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, cu_s
 
     bf16 tensors (all of q, k, v) stay bf16 in memory, everything else is fp32; states, decays and sums are fp32 or wider.
     cu_seqlens (n + 1 int32 offsets, non-decreasing): l tokens of one row (b = 1) hold n sequences, some possibly empty; rows that
-    belong to none give zeros.  max_seqlen: an upper estimate of the longest of them (a hint for splitting the work, default l).
+    belong to none give zeros.  max_seqlen: an estimate of the longest of them (a hint whether to split any, default l).
     Without cu_seqlens n = b."""
     dims = _check(q, k, v, log_decay, initial_state, cu_seqlens)
     B, L, G, dk, H, dv, N = dims

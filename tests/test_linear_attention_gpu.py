@@ -447,3 +447,62 @@ def test_refusals():
     version = state._version
     linear_attention_step(**ok)
     assert state._version > version
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dk,dv", [(16, 64), (64, 32), (33, 100), (128, 128)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_that_are_not_finite_reach_later_rows_only(dtype, dk, dv, bad):
+    t = {n: x.cuda() for n, x in make([300], False, 2, 2, dk, dv, dtype, seed=5).items()}
+    call = lambda **kw: linear_attention_fn(*[kw.get(n, t[n]) for n in ("q", "k", "v", "g")], initial_state=t["s0"], return_last_state=True)  # noqa: E731
+    out, last = call()
+    v = t["v"].clone()
+    v[0, 100, 0, 5], v[0, 37, 1, 7], v[0, 150, 1, 7] = bad, -bad, bad
+    got, end = call(v=v)
+    assert torch.equal(got[0, :100, 0], out[0, :100, 0]) and torch.equal(got[0, :37, 1], out[0, :37, 1])
+    assert not torch.isfinite(got[0, 100:, 0, 5]).any() and not torch.isfinite(got[0, 37:, 1, 7]).any()
+    assert not torch.isfinite(end[0, 0, :, 5]).any() and not torch.isfinite(end[0, 1, :, 7]).any()
+    keep = torch.ones(2, dv, dtype=torch.bool, device="cuda")
+    keep[0, 5] = keep[1, 7] = False
+    assert torch.equal(got[0, :, keep], out[0, :, keep]) and torch.equal(end[0].transpose(1, 2)[keep], last[0].transpose(1, 2)[keep])
+    for n in ("k", "q", "g"):
+        x = t[n].clone()
+        x[0, 90, 1] = float("nan")
+        got, _ = call(**{n: x})
+        assert torch.equal(got[0, :90], out[0, :90]) and torch.equal(got[0, :, 0], out[0, :, 0]) and torch.isnan(got[0, 90, 1]).all()
+        assert n != "q" or torch.equal(got[0, 91:], out[0, 91:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hint", [None, 1, 900])
+def test_many_packed_sequences_of_which_a_few_are_long(dtype, hint):
+    lens = [0, 1, 2, 0, 63, 64, 65, 3] * 4 + [900] + [5, 0, 128] * 3 + [1500, 0, 0]
+    t = make(lens, True, 2, 1, 32, 16, dtype, seed=11)
+    scale = 32 ** -0.5
+    want, size = reference(t, lens, True, scale), reference(t, lens, True, scale, absolute=True)
+    check(run(t, lens, True, max_seqlen=hint), want, size, steps_of(lens, 32, 16))
+
+
+def test_more_sequences_than_a_grid_axis_holds():
+    """70000 sequences of one token and one that is split: the states' scratch holds a segment each, not the longest one's number of them."""
+    n, L, dk, dv = 70000, 600, 4, 3
+    r = torch.Generator().manual_seed(3)
+    T = n + L
+    q, k, v, g = (torch.randn(1, T, 2, d, generator=r).cuda() for d in (dk, dk, dv, 1))
+    g = -g[..., 0].abs()
+    cu = torch.cat([torch.arange(n // 2 + 1), torch.arange(n // 2, n + 1) + L]).to(torch.int32).cuda()       # the long one in the middle
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        out, last = linear_attention_fn(q, k, v, g, scale=1.0, cu_seqlens=cu, return_last_state=True)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 64 << 20
+    one = torch.cat([torch.arange(n // 2), torch.arange(n // 2, n) + L]).cuda()
+    d = lambda x: x[0, one].double()  # noqa: E731
+    want = (d(q) * d(k)).sum(-1, keepdim=True) * d(v)
+    assert bool(((out[0, one].double() - want).abs() <= (dk + 4) * U * (d(q) * d(k)).abs().sum(-1, keepdim=True) * d(v).abs() + 1e-30).all())
+    lo = n // 2
+    t = {"q": q[:, lo:lo + L], "k": k[:, lo:lo + L], "v": v[:, lo:lo + L], "g": g[:, lo:lo + L], "s0": None, "do": torch.zeros(1, L, 2, dv), "ds": torch.zeros(1, 2, dk, dv)}
+    t = {m: None if x is None else x.cpu() for m, x in t.items()}
+    ref, size = (reference(t, [L], False, 1.0, absolute=a) for a in (False, True))
+    check({"out": out[:, lo:lo + L], "last": last[lo:lo + 1]}, ref, size, steps_of([L], dk, dv))

@@ -21,7 +21,7 @@ def test_cpu_tensors_are_rejected():
 
 
 def _fwd(lib, **kw):
-    a = dict(dtype=0, q=16, k=16, v=16, g=16, st=(ctypes.c_longlong * 12)(), cu=None, s0=None, out=16, last=None, chunks=None, ws=None, wd=None, N=1, L=8,
+    a = dict(dtype=0, q=16, k=16, v=16, g=16, st=(ctypes.c_longlong * 12)(*[128] * 12), cu=None, s0=None, out=16, last=None, chunks=None, ws=None, wd=None, N=1, L=8,
              H=2, G=2, dk=16, dv=16, nseg=1, segc=1)
     a.update(kw)
     return lib.ss2d_linattn_fwd(a["dtype"], a["q"], a["k"], a["v"], a["g"], a["st"], a["cu"], a["s0"], a["out"], a["last"], a["chunks"], a["ws"], a["wd"], a["N"],
@@ -31,7 +31,9 @@ def _fwd(lib, **kw):
 @pytest.mark.parametrize("kw,rc,word", [(dict(dtype=3), -1, b"dtype"), (dict(q=None), -2, b"null"), (dict(st=None), -2, b"null"), (dict(out=None), -2, b"null"),
                                         (dict(N=0), -3, b"size"), (dict(L=0), -3, b"size"), (dict(L=1 << 31), -3, b"size"), (dict(nseg=0), -3, b"size"),
                                         (dict(H=3), -4, b"multiple"), (dict(dk=129), -5, b"128"), (dict(dv=0), -5, b"128"),
-                                        (dict(N=1 << 30, H=8, G=8), -6, b"many"), (dict(nseg=2), -2, b"workspace")])
+                                        (dict(N=1 << 30, H=8, G=8), -6, b"many"), (dict(nseg=2), -2, b"workspace"),
+                                        (dict(st=(ctypes.c_longlong * 12)(*[15] * 12)), -4, b"strides"),
+                                        (dict(st=(ctypes.c_longlong * 12)(*[1 << 22] * 12)), -4, b"strides")])
 def test_linattn_fwd_refuses(kw, rc, word):
     from mamba_unet_amd import _lib
     lib = _lib.load()
@@ -41,7 +43,7 @@ def test_linattn_fwd_refuses(kw, rc, word):
 def test_linattn_bwd_and_step_refuse():
     from mamba_unet_amd import _lib
     lib = _lib.load()
-    st = (ctypes.c_longlong * 12)()
+    st = (ctypes.c_longlong * 12)(*[128] * 12)
     bwd = lambda dout=16, H=2, heads=None: lib.ss2d_linattn_bwd(0, 16, 16, 16, 16, st, None, dout, None, 16, 16, 16, 16, 16, None, heads, heads, None, None,  # noqa: E731
                                                                 1, 8, H, 2, 16, 16, 1.0, 1, 1, None)
     assert bwd(dout=None) == -2 and bwd(H=4) == -2 and b"shared key heads" in lib.ss2d_last_error()

@@ -123,8 +123,8 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
     if (c0 < c1) fetch(first);
     // A NaN or an infinity in v_j times the zero weight of an earlier row would reach that row.  Once one has been met, such values stay out of the
     // products and are added to the rows from j on alone, and their columns of the state become NaN.
-    float *poison = decays + 300;                // (the first chunk's set of decays ends at 257)
-    if (MODE == 0 && tid == 0) *poison = 0.0f;
+    int *poison = reinterpret_cast<int *>(decays + 300);                // (the first chunk's set of decays ends at 257)
+    if (MODE == 0 && tid == 0) *poison = 0;
 #pragma unroll 1
     for (int c = first; c >= c0 && c < c1; c += STEP) {
         const int nr = rows_of(c);
@@ -147,10 +147,11 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
         if (MODE == 0) qr.put(Qs, p.dk);
         kr.put(Ks, p.dk);
         vr.put(Vs, dvc);
-        if (MODE == 0 && vr.not_finite()) *poison = 1.0f;
+        if (MODE == 0 && vr.not_finite()) *poison = 1;
         if (c + STEP >= c0 && c + STEP < c1) fetch(c + STEP);
         __syncthreads();
         const float *bh = decays + (c & 1) * 320, *bl = bh + 64, *eb = bl + 64, *wt = eb + 64, *tail = wt + 64;
+        const bool poisoned = MODE == 0 && __builtin_amdgcn_readfirstlane(*poison);
         if (MODE == 0) {
             // P[i][j] = scale exp(b_i - b_j) q_i . k_j, j <= i: tiles (it, jt) dealt to the waves
 #pragma unroll 1
@@ -181,18 +182,6 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) vv[jt][r] = Vs[(16 * jt + 4 * gq + r) * PV + 16 * wave + l16];
         float eend = tail[0];
-        const bool poisoned = MODE == 0 && *poison != 0.0f;
-        if (poisoned) {
-            int bad = 0;
-#pragma unroll
-            for (int jt = 0; jt < CT; ++jt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (!__builtin_isfinite(vv[jt][r])) { vv[jt][r] = 0.0f; bad = 1; }
-            bad |= __shfl_xor(bad, 16, 64);
-            bad |= __shfl_xor(bad, 32, 64);
-            if (bad) eend = __builtin_nanf("");
-        }
         if (MODE == 0) {
             f4 acc[CT];
 #pragma unroll
@@ -206,8 +195,20 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
                     for (int r = 0; r < 4; ++r) acc[it] = mfma4(x[r], S[kt][r], acc[it]);
                 }
 #pragma unroll
+            for (int it = 0; it < CT; ++it) acc[it] *= *reinterpret_cast<const f4 *>(eb + 16 * it + 4 * gq);
+            if (poisoned) {
+                int bad = 0;
+#pragma unroll
+                for (int jt = 0; jt < CT; ++jt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!__builtin_isfinite(vv[jt][r])) { vv[jt][r] = 0.0f; bad = 1; }
+                bad |= __shfl_xor(bad, 16, 64);
+                bad |= __shfl_xor(bad, 32, 64);
+                if (bad) eend = __builtin_nanf("");
+            }
+#pragma unroll
             for (int it = 0; it < CT; ++it) {
-                acc[it] *= *reinterpret_cast<const f4 *>(eb + 16 * it + 4 * gq);
 #pragma unroll
                 for (int jt = 0; jt <= it; ++jt) {
                     const f4 x = *reinterpret_cast<const f4 *>(Ps + (16 * it + l16) * PP + 16 * jt + 4 * gq);
@@ -354,8 +355,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
     }
     // A NaN or an infinity in v_j times the zero weight of an earlier row would reach that row.  Once one has been met, such values stay out of the
     // products and are added to the rows from j on alone, and their columns of the state become NaN.
-    float *poison = decays + 300;                // (the first chunk's set of decays ends at 257)
-    if (MODE == 0 && tid == 0) *poison = 0.0f;
+    int *poison = reinterpret_cast<int *>(decays + 300);                // (the first chunk's set of decays ends at 257)
+    if (MODE == 0 && tid == 0) *poison = 0;
 #pragma unroll 1
     for (int c = first; c >= c0 && c < c1; c += STEP) {
         const int nr = rows_of(c);
@@ -368,11 +369,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
         if (MODE == 0) qr.template put<true>(Qs, QP, p.dk);
         kr.put(Ks, KP, p.dk);
         vr.put(Vs, VP, p.dv);
-        if (MODE == 0 && vr.not_finite()) *poison = 1.0f;
+        if (MODE == 0 && vr.not_finite()) *poison = 1;
         Q += C * p.ql; K += STEP * C * p.kl; V += STEP * C * p.vl;
         if (MODE >= 1 && c + STEP >= c0 && c + STEP < c1) fetch(c + STEP);
         const float *bh = decays + (c & 1) * 5 * C, *bl = bh + C, *eb = bl + C, *wt = eb + C, *tail = wt + C;
         __syncthreads();
+        const bool poisoned = MODE == 0 && __builtin_amdgcn_readfirstlane(*poison);
         if (MODE == 0) {
             // P[i][j] = scale exp(b_i - b_j) q_i . k_j, j <= i: the ten 16 x 16 tiles are dealt to the waves and worked on side by side (a wave with one
             // less repeats the last one: the same values)
@@ -406,24 +408,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
 #pragma unroll
         for (int js = 0; js < 2; ++js) vf[js] = frag_t(Vs, VP, wave, js, lane);
         float eend = tail[0];
-        const bool poisoned = MODE == 0 && *poison != 0.0f;
-        if (poisoned) {
-            int bad = 0;
-#pragma unroll
-            for (int js = 0; js < 2; ++js) {
-                u32x4 w = __builtin_bit_cast(u32x4, vf[js]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const unsigned m = ((w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;       // the halves that are not finite
-                    bad |= m != 0;
-                    w[i] &= ~(m | (m - (m >> 15)));
-                }
-                vf[js] = __builtin_bit_cast(bf16x8, w);
-            }
-            bad |= __shfl_xor(bad, 16, 64);
-            bad |= __shfl_xor(bad, 32, 64);
-            if (bad) eend = __builtin_nanf("");
-        }
         if (MODE == 0) {
             f4 acc[4];
 #pragma unroll
@@ -442,8 +426,26 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
             }
             const RowsOut out(O, nr, ldo);
 #pragma unroll
+            for (int it = 0; it < 4; ++it) acc[it] *= eb[16 * it + l16];
+            if (poisoned) {
+                int bad = 0;
+#pragma unroll
+                for (int js = 0; js < 2; ++js) {
+                    u32x4 w = __builtin_bit_cast(u32x4, vf[js]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned m = ((w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;       // the halves that are not finite
+                        bad |= m != 0;
+                        w[i] &= ~(m | (m - (m >> 15)));
+                    }
+                    vf[js] = __builtin_bit_cast(bf16x8, w);
+                }
+                bad |= __shfl_xor(bad, 16, 64);
+                bad |= __shfl_xor(bad, 32, 64);
+                if (bad) eend = __builtin_nanf("");
+            }
+#pragma unroll
             for (int it = 0; it < 4; ++it) {
-                acc[it] *= eb[16 * it + l16];
 #pragma unroll
                 for (int js = 0; js <= it / 2; ++js) {
                     acc[it] = mfma8(vf[js], frag_p(Ph, PP, 16 * it + l16, js, gq), acc[it]);

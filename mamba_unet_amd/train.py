@@ -148,20 +148,27 @@ def set_lr(optimizer, lr: float):
             g["lr"] = lr
 
 
-_dtype_of = attrgetter("dtype")
+_dtype_of, _requires_grad = attrgetter("dtype"), attrgetter("requires_grad")
+
+
+def _gradient(g):
+    if g is None or not (g.requires_grad or type(g) is torch.nn.Parameter):
+        return g
+    if not g.is_leaf:
+        raise ValueError("clip_grad_norm: a tensor with a gradient of its own that is no leaf: give gradients (detached), or the leaves they belong to")
+    return g.grad
 
 
 def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """Scales the gradients in place by min(1, max_norm / (norm + 1e-6)) with their global norm (2 or inf) and returns the norm, a 0-dim
     fp32 tensor: what torch.nn.utils.clip_grad_norm_ computes, without a host read of the norm (so it can be captured in a HIP graph) and in two
-    launches for up to 240 tensors.  `grads`: tensors, or parameters, whose .grad is taken (None: left out); fp32 or bf16, on one
-    GPU, none sharing memory with another.  The norm is summed in 64 bits in a fixed order; one that is not a number makes every
+    launches for up to 240 tensors.  `grads`: tensors, or parameters and other leaves that require gradients, whose .grad is taken (None: left
+    out); fp32 or bf16, on one GPU, none sharing memory with another.  The norm is summed in 64 bits in a fixed order; one that is not a number makes every
     gradient not a number.  max_norm = inf only measures."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     kinds = set(map(type, grads))
-    if torch.nn.Parameter in kinds or type(None) in kinds:
-        grads = [g.grad if type(g) is torch.nn.Parameter else g for g in grads]
-        grads = [g for g in grads if g is not None]
+    if torch.nn.Parameter in kinds or type(None) in kinds or any(map(_requires_grad, grads)):
+        grads = [g for g in map(_gradient, grads) if g is not None]
     max_norm, norm_type = float(max_norm), float(norm_type)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm: max_norm must be >= 0, got {max_norm}")

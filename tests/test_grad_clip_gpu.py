@@ -107,6 +107,16 @@ def test_parameters_and_measuring_only():
     assert float(clip_grad_norm([torch.empty(0).cuda()], 1.0)) == 0.0
 
 
+def test_leaves_that_are_no_parameters_keep_their_values():
+    a, b = (torch.full((6,), x, device="cuda", requires_grad=True) for x in (7.0, 9.0))
+    a.grad = torch.full((6,), 2.0, device="cuda")
+    n = math.sqrt(24)
+    assert abs(float(clip_grad_norm([a, b, None], 1.0)) - n) <= 1e-6 * n
+    assert bool((a == 7.0).all()) and bool((b == 9.0).all()) and b.grad is None and abs(float(a.grad.norm()) - 1.0) <= 1e-5
+    with pytest.raises(ValueError, match="no leaf"):
+        clip_grad_norm([a * 2], 1.0)
+
+
 def test_refusals():
     a = torch.randn(10).cuda()
     with pytest.raises(ValueError, match="shares memory"):
@@ -170,3 +180,22 @@ def test_training_step_clips():
             # the backward's float atomics change gradients in their last digits (1e-5 of them); a step without the clip would be 10 times as long
             for other in nets[1:]:
                 assert float((flat(nets[0]) - flat(other)).norm()) <= 1e-2 * moved
+
+
+def test_cross_supervised_step_clips_each_network():
+    import copy
+    from mamba_unet_amd.train import semi_step
+    torch.manual_seed(7)
+    nets = [torch.nn.Conv2d(1, 4, 3, padding=1).cuda() for _ in range(2)]
+    images, labels = torch.randn(4, 1, 32, 32, device="cuda"), torch.randint(0, 4, (4, 32, 32), device="cuda")
+    grads = []
+    for max_norm in (None, 0.02):
+        two = [copy.deepcopy(n) for n in nets]
+        opts = [torch.optim.SGD(n.parameters(), lr=0.5) for n in two]
+        semi_step(*two, *opts, images, labels, 2, 4, 0, 30000, 0.1, max_grad_norm=max_norm)
+        grads.append([[p.grad.double() for p in n.parameters()] for n in two])
+    for plain, clipped in zip(*grads):
+        norm = torch.stack([g.norm() for g in plain]).norm()
+        assert norm > 0.02
+        for a, b in zip(plain, clipped):      # the two runs' gradients come from the same kernels; a factor and a product: 2 roundings, the norm's own half step
+            assert float((b - a * (0.02 / (norm + 1e-6))).abs().max()) <= 3 * 2.0 ** -24 * float(a.abs().max()) + 1e-12

@@ -774,10 +774,8 @@ def _norm_rows(t, io, D):
     else:
         ld = t.stride(-2) if t.dim() > 1 else D
         rows = all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 2))
-        if t.stride(-1) != 1 or not rows or ld < D or (D % 8 == 0 and ld % 8):
+        if t.stride(-1) != 1 or not rows or ld < D:
             t, ld = t.contiguous(), D
-    if D % 8 == 0 and t.data_ptr() % 16:
-        t, ld = t.clone(memory_format=torch.contiguous_format), D
     return t, ld
 
 

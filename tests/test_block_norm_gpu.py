@@ -194,3 +194,20 @@ def test_captured_and_repeated_runs_are_equal():
         torch.cuda.synchronize()
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("types", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16)], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("D", [5, 64, 65, 1032, 5000])
+def test_rows_at_any_offset_and_distance(D, types):
+    t = make((3, 4, D), *types)
+    d = {n: v.cuda() for n, v in t.items()}
+    want_x, want_h = call(d, False)
+    for at, pitch in ((1, D + 1), (3, D + 5), (2, D + 7)):
+        views = {}
+        for n in ("x", "y", "z"):
+            wide = torch.full((3, 4, pitch), float("nan"), device="cuda", dtype=d[n].dtype).flatten()
+            wide = torch.cat([wide.new_zeros(at), wide])[at:].view(3, 4, pitch)
+            views[n] = wide[..., pitch - D:] if n == "z" else wide[..., :D]
+            views[n].copy_(d[n])
+        x, h = call({**d, **views}, False)
+        assert torch.equal(x, want_x) and torch.equal(h, want_h)

@@ -5,7 +5,7 @@ code/networks/vision_mamba.py): `selective_scan_fn`, `SS2D`, `VSSBlock`, `VSSLay
 `VSSM`, `MambaUnet`.  All hot-path compute goes through libss2d_hip.so (include/ss2d.h); there is no
 CPU path."""
 from .selective_scan_interface import SelectiveScanFn, scan_core_fn, scan_merge_fn, selective_scan_fn  # noqa: F401
-from .linear_attention import LinearAttentionFn, linear_attention_fn, linear_attention_step  # noqa: F401
+from .linear_attention import linear_attention_fn, linear_attention_step  # noqa: F401
 from .ss2d import SS2D, DropPath, VSSBlock, VSSLayer, VSSLayer_up  # noqa: F401
 from .ss2d_ops import (cross_merge, cross_scan, dwconv3x3_silu, layer_norm, linear_nobias, linear_wgrad, norm_gate_residual, outnorm_gate,  # noqa: F401
                        scan_params)
@@ -15,5 +15,5 @@ from .vssm import (VSSM, FinalPatchExpand_X4, MambaUnet, MambaUnetConfig, PatchE
 
 __all__ = ["selective_scan_fn", "SelectiveScanFn", "SS2D", "VSSBlock", "VSSLayer", "VSSLayer_up", "VSSM",
            "MambaUnet", "MambaUnetConfig", "cross_scan", "cross_merge", "dwconv3x3_silu", "DropPath",
-           "linear_attention_fn", "LinearAttentionFn", "linear_attention_step", "norm_gate_residual", "clip_grad_norm",
+           "linear_attention_fn", "linear_attention_step", "norm_gate_residual", "clip_grad_norm",
            "PatchEmbed2D", "PatchMerging2D", "PatchExpand", "FinalPatchExpand_X4"]

@@ -111,6 +111,24 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_host_ops = None
+
+
+def host():
+    """The native host side of the operators that are called through it (csrc/host_ops.cpp), with this library's entry points."""
+    global _host_ops
+    if _host_ops is None:
+        import torch  # noqa: F401  (its libraries are what the extension is linked to)
+        lib = load()
+        try:
+            from . import _host as ops
+        except ImportError as e:
+            raise SS2DLibraryError(f"{os.path.join(_HERE, '_host.so')} not found or not loadable ({e}): build it with `make -C mamba_unet_amd/csrc`") from e
+        ops.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in ops.names()})
+        _host_ops = ops
+    return _host_ops
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = load().ss2d_last_error().decode(errors="replace")
@@ -146,13 +164,6 @@ def on_device(dev):
     if idx is None or idx == torch.cuda.current_device():
         return _NO_CTX
     return torch.cuda.device(dev)
-
-
-def stream_of(index):
-    """Raw handle of torch's current stream on device `index` when that is the current device, else None (the caller then enters
-    torch.cuda.device(index)).  For operators whose time is the host's: no context manager, no Stream object."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(index) if torch._C._cuda_getDevice() == index else None
 
 
 def stream():

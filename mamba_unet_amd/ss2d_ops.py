@@ -765,102 +765,6 @@ def outnorm_gate(y: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, bias: t
     return _OutNormGate.apply(y, z, weight, bias, eps, holder, scale)
 
 
-def _norm_rows(t, io, D):
-    """t as (rows, D) rows in the storage type with a dense last axis and one distance between rows: in place where t has that
-    layout (a channel slice of a wider tensor), else a copy.  Returns the tensor and the distance."""
-    t = t if t.dtype == io else t.to(io)
-    if t.is_contiguous():
-        ld = D
-    else:
-        ld = t.stride(-2) if t.dim() > 1 else D
-        rows = all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 2))
-        if t.stride(-1) != 1 or not rows or ld < D:
-            t, ld = t.contiguous(), D
-    return t, ld
-
-
-def _fp32_param(t):
-    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
-
-
-def _norm_gate_residual(x, y, z, w1, b1, a, w2, b2, drop, eps, rms, want_stats):
-    """One forward pass: (x', h) in the storage types, the statistics (or None) and what the backward needs."""
-    D = x.shape[-1]
-    rows = x.numel() // D
-    (rt, rcode), (io, code) = _io(x), _io(y)
-    (x_, ldx), (y_, ldy) = _norm_rows(x, rt, D), _norm_rows(y, io, D)
-    z_, ldz = (None, D) if z is None else _norm_rows(z, io, D)
-    w1_, b1_, a_, w2_, b2_, drop_ = _fp32_param(w1), _fp32_param(b1), _fp32_param(a), _fp32_param(w2), _fp32_param(b2), _fp32_param(drop)
-    dev = x.device
-    x_out, h = torch.empty(x.shape, device=dev, dtype=rt), torch.empty(x.shape, device=dev, dtype=io)
-    stats = torch.empty((rows, 4), device=dev, dtype=torch.float32) if want_stats else None
-    rps = rows // drop.numel() if drop is not None and drop.numel() else 0
-    if rows:
-        p = _data_ptr
-        args = (rcode, code, x_.data_ptr(), y_.data_ptr(), p(z_), w1_.data_ptr(), p(b1_), w2_.data_ptr(), p(b2_), p(a_), p(drop_), rps, x_out.data_ptr(),
-                h.data_ptr(), p(stats), rows, D, ldx, ldy, ldz, eps, rms)
-        stream = _lib.stream_of(dev.index)
-        if stream is None:
-            with torch.cuda.device(dev):
-                rc = _lib.load().ss2d_block_norm_fwd(*args, _stream())
-        else:
-            rc = _lib.load().ss2d_block_norm_fwd(*args, stream)
-        if rc:
-            _lib.check(rc, "ss2d_block_norm_fwd")
-    return x_out, h, stats, (x_, y_, z_, w1_, b1_, a_, w2_, drop_), (rcode, code, D, ldx, ldy, ldz, rps, rms, rows)
-
-
-def _data_ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-class _NormGateResidual(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, y, z, w1, b1, a, w2, b2, drop, eps, rms):
-        ctx.set_materialize_grads(False)
-        x_out, h, stats, saved, meta = _norm_gate_residual(x, y, z, w1, b1, a, w2, b2, drop, eps, rms, True)
-        ctx.save_for_backward(*saved, stats)
-        ctx.meta = meta + (x.shape, [None if t is None else t.dtype for t in (x, y, z, w1, b1, a, w2, b2)])
-        return x_out.to(x.dtype), h.to(y.dtype)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dx_out, dh):
-        if dx_out is None and dh is None:
-            return (None,) * 11
-        x, y, z, w1, b1, a, w2, drop, stats = ctx.saved_tensors
-        rcode, code, D, ldx, ldy, ldz, rps, rms, rows, shape, dt = ctx.meta
-        dev, p = x.device, _data_ptr
-        gx, gh = _dense16(dx_out, x.dtype), _dense16(dh, y.dtype)
-        dx, dy = torch.empty(shape, device=dev, dtype=x.dtype), torch.empty(shape, device=dev, dtype=y.dtype)
-        dz = None if z is None else torch.empty(shape, device=dev, dtype=y.dtype)
-        if rows:
-            lib = _lib.load()
-            n = lib.ss2d_block_norm_bwd_workspace_floats(rows, D)
-            dp, ws = torch.empty(5 * D, device=dev, dtype=torch.float32), torch.empty(n, device=dev, dtype=torch.float32)
-            args = (rcode, code, p(gx), p(gh), x.data_ptr(), y.data_ptr(), p(z), w1.data_ptr(), p(b1), w2.data_ptr(), p(a), p(drop), rps, stats.data_ptr(),
-                    dx.data_ptr(), dy.data_ptr(), p(dz), dp.data_ptr(), ws.data_ptr(), rows, D, ldx, ldy, ldz, rms)
-            stream = _lib.stream_of(dev.index)
-            if stream is None:
-                with torch.cuda.device(dev):
-                    rc = lib.ss2d_block_norm_bwd(*args, _stream())
-            else:
-                rc = lib.ss2d_block_norm_bwd(*args, stream)
-            if rc:
-                _lib.check(rc, "ss2d_block_norm_bwd")
-        else:
-            dp = torch.zeros(5 * D, device=dev, dtype=torch.float32)
-        grads = (dx, dy, dz, *dp.split(D))
-        return (*(None if d is None or not n else g if g.dtype is d else g.to(d) for g, d, n in zip(grads, dt, ctx.needs_input_grad)), None, None, None)
-
-
-def _dense16(g, dtype):
-    """g dense, in `dtype`, on a 16-byte boundary"""
-    if g is None or (g.dtype is dtype and g.is_contiguous() and g.data_ptr() % 16 == 0):
-        return g
-    return g.to(dtype).clone(memory_format=torch.contiguous_format)
-
-
 def norm_gate_residual(x, y, post_weight, pre_weight, post_bias=None, pre_bias=None, z=None, res_scale=None, drop_scale=None, eps: float = 1e-5,
                        rms: bool = False):
     """The norms on both sides of a block with its gate and residual scale, fused: with the residual stream x and the block's output y,
@@ -871,30 +775,7 @@ def norm_gate_residual(x, y, post_weight, pre_weight, post_bias=None, pre_bias=N
     with `rms`; statistics in fp32, h from the unrounded x'.  z (y's shape; a channel slice of a wider tensor is read in place), the biases,
     res_scale (D,) and drop_scale (one factor per sample, not differentiated) are optional.  bf16 x and y / z stay bf16 in memory (x may be fp32 with a bf16
     branch); D <= 8192."""
-    named = (("x", x), ("y", y), ("post_weight", post_weight), ("pre_weight", pre_weight), ("z", z), ("post_bias", post_bias), ("pre_bias", pre_bias),
-             ("res_scale", res_scale), ("drop_scale", drop_scale))
-    shape, dev, need = x.shape, x.get_device(), False
-    if not shape or not 1 <= shape[-1] <= 8192:
-        raise ValueError(f"norm_gate_residual: the last axis must hold 1 ... 8192 channels, got {tuple(shape)}")
-    vec = shape[-1:]
-    for name, t in named:
-        if t is None:
-            continue
-        if t.get_device() != dev or dev < 0:
-            _need_gpu(t, f"norm_gate_residual: `{name}`")
-            _need_gpu(x, "norm_gate_residual: `x`")
-            raise ValueError(f"norm_gate_residual: `{name}` is on {t.device}, x on {x.device}")
-        if name == "drop_scale":
-            continue
-        if t.shape != (shape if name in ("x", "y", "z") else vec):
-            raise ValueError(f"norm_gate_residual: `{name}` must be {tuple(shape if name in ('x', 'y', 'z') else vec)}, got {tuple(t.shape)}")
-        need = need or t.requires_grad
-    if drop_scale is not None and (len(shape) < 2 or drop_scale.numel() != shape[0]):
-        raise ValueError("norm_gate_residual: `drop_scale` must hold one factor per sample")
-    if need and torch.is_grad_enabled():
-        return _NormGateResidual.apply(x, y, z, post_weight, post_bias, res_scale, pre_weight, pre_bias, drop_scale, float(eps), int(bool(rms)))
-    x_out, h = _norm_gate_residual(x, y, z, post_weight, post_bias, res_scale, pre_weight, pre_bias, drop_scale, float(eps), int(bool(rms)), False)[:2]
-    return x_out if x_out.dtype is x.dtype else x_out.to(x.dtype), h if h.dtype is y.dtype else h.to(y.dtype)
+    return _lib.host().norm_gate_residual(x, y, post_weight, pre_weight, post_bias, pre_bias, z, res_scale, drop_scale, eps, bool(rms))
 
 
 class _LayerNorm(torch.autograd.Function):

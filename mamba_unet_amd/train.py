@@ -8,8 +8,6 @@
 from __future__ import annotations
 
 import os as _os
-from array import array
-from operator import attrgetter
 
 import torch
 import torch.nn.functional as F
@@ -148,79 +146,13 @@ def set_lr(optimizer, lr: float):
             g["lr"] = lr
 
 
-_dtype_of, _requires_grad = attrgetter("dtype"), attrgetter("requires_grad")
-
-
-def _gradient(g):
-    if g is None or not (g.requires_grad or type(g) is torch.nn.Parameter):
-        return g
-    if not g.is_leaf:
-        raise ValueError("clip_grad_norm: a tensor with a gradient of its own that is no leaf: give gradients (detached), or the leaves they belong to")
-    return g.grad
-
-
 def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """Scales the gradients in place by min(1, max_norm / (norm + 1e-6)) with their global norm (2 or inf) and returns the norm, a 0-dim
     fp32 tensor: what torch.nn.utils.clip_grad_norm_ computes, without a host read of the norm (so it can be captured in a HIP graph) and in two
     launches for up to 240 tensors.  `grads`: tensors, or parameters and other leaves that require gradients, whose .grad is taken (None: left
     out); fp32 or bf16, on one GPU, none sharing memory with another.  The norm is summed in 64 bits in a fixed order; one that is not a number makes every
     gradient not a number.  max_norm = inf only measures."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    kinds = set(map(type, grads))
-    if torch.nn.Parameter in kinds or type(None) in kinds or any(map(_requires_grad, grads)):
-        grads = [g for g in map(_gradient, grads) if g is not None]
-    max_norm, norm_type = float(max_norm), float(norm_type)
-    if not max_norm >= 0.0:
-        raise ValueError(f"clip_grad_norm: max_norm must be >= 0, got {max_norm}")
-    if norm_type not in (2.0, float("inf")):
-        raise ValueError(f"clip_grad_norm: norm_type must be 2 or inf, got {norm_type}")
-    if not grads:
-        return torch.tensor(0.0)
-    devs, types = set(map(torch.Tensor.get_device, grads)), set(map(_dtype_of, grads))
-    if min(devs) < 0:
-        raise RuntimeError("clip_grad_norm: GPU tensors required (no CPU path in mamba_unet_amd)")
-    if len(devs) > 1:
-        raise ValueError(f"clip_grad_norm: gradients on several devices: {sorted(devs)}")
-    if not types <= {torch.float32, torch.bfloat16}:
-        raise ValueError(f"clip_grad_norm: fp32 or bf16 gradients required, got {types}")
-    dev = grads[0].device
-    work = grads
-    if not all(map(torch.Tensor.is_contiguous, grads)):
-        # dense in another order (channels last): the elements are the same; anything else goes through a copy
-        work = [g if g.is_contiguous() else _dense_view(g) for g in grads]
-    n = len(grads)
-    lib = _lib.load()
-    ptrs = array("Q", map(torch.Tensor.data_ptr, work))
-    sizes = array("q", map(torch.Tensor.numel, work))
-    is_bf16 = bytes([t.dtype is torch.bfloat16 for t in grads]) if len(types) > 1 else (b"\1" if torch.bfloat16 in types else b"\0") * n
-    nbytes = lib.ss2d_grad_clip_workspace_bytes(n)
-    norm = torch.empty((), device=dev, dtype=torch.float32)
-    ws = torch.empty(nbytes // 8, device=dev, dtype=torch.float64)
-    args = (is_bf16, ptrs.buffer_info()[0], sizes.buffer_info()[0], n, int(norm_type != 2.0), max_norm, int(max_norm != float("inf")), norm.data_ptr(),
-            ws.data_ptr(), nbytes)
-    stream = _lib.stream_of(dev.index)
-    if stream is None:
-        with torch.cuda.device(dev):
-            rc = lib.ss2d_grad_clip(*args, _lib.stream())
-    else:
-        rc = lib.ss2d_grad_clip(*args, stream)
-    if rc:
-        _lib.check(rc, "ss2d_grad_clip")
-    if max_norm != float("inf"):
-        if work is not grads:
-            with torch.no_grad():
-                for g, w in zip(grads, work):
-                    if w.data_ptr() != g.data_ptr():
-                        g.copy_(w)
-        torch._C._increment_version([g for g in grads if not g.is_inference()] if grads[0].is_inference() else grads)
-    return norm
-
-
-def _dense_view(g):
-    """g's elements as a dense tensor: a view where g fills its memory in some order of its axes, else a copy."""
-    order = sorted((i for i in range(g.dim()) if g.shape[i] != 1), key=lambda i: -g.stride(i))
-    v = g.detach().permute(order + [i for i in range(g.dim()) if g.shape[i] == 1])
-    return v if v.is_contiguous() else g.detach().contiguous()
+    return _lib.host().clip_grad_norm(grads, max_norm, norm_type)
 
 
 def supervised_step(model, optimizer, images, labels, n_classes, it, max_it, base_lr=0.01, autocast_bf16=False, max_grad_norm=None):

@@ -467,7 +467,7 @@ Tensor clip_grad_norm(const py::object &given, double max_norm, double norm_type
         if (o == Py_None) return;
         TORCH_CHECK_TYPE(THPVariable_Check(o), "clip_grad_norm: tensors required, got ", Py_TYPE(o)->tp_name);
         const Tensor &t = THPVariable_Unpack(o);
-        if (!t.requires_grad() && !(ParameterClass && PyObject_IsInstance(o, ParameterClass) == 1)) {
+        if (!t.requires_grad() && !PyType_IsSubtype(Py_TYPE(o), reinterpret_cast<PyTypeObject *>(ParameterClass))) {      // (isinstance would run Python code)
             grads.push_back(t);
             return;
         }

@@ -342,18 +342,22 @@ __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_a
 // tokens of a chunk: the backward holds q, k, v, dout, a dk x dv state and two C x C matrices in 160 KB of LDS
 inline int linattn_chunk(int dtype, int dk, int dv) { return dtype || (dk <= 64 && dv <= 64) ? 64 : 32; }
 
-// Segments.  One workgroup walks a segment; with fewer workgroups than the card holds at once (two or three a CU) it idles, and a segment
-// costs a second pass over k and v (q and dout in the backward) and a state's round trip: so all tokens of all sequences and
-// heads are dealt to that many workgroups, at least four chunks each.
+// Segments.  One workgroup walks a segment; with fewer workgroups than the card holds at once it idles, and a segment costs a second pass over k and v (q
+// and dout in the backward) and a state's round trip.  So all tokens of all sequences and heads are dealt to as many workgroups as are resident
+// (forward: three a CU up to 64 x 64 in bf16, else two; backward: one up to 128 wide keys in bf16, else two shifts of one), at least two chunks each, in equal
+// parts of the longest sequence.  Measured, us, for half the workgroups / these / twice: 24 x 3136 tokens, 3 heads of 16 x 64 fp32, forward
+// and backward 322 / 194 / 215; 65536 tokens, 8 heads of 128 x 128 bf16, forward 283 / 252 / 270; not split 521 and 5383.  Short ones: a bf16 chunk takes
+// 3 us and the two further launches cost as much as two chunks: 256 tokens (4 chunks) 15 us in one walk, 19 split; 512 tokens 26 and 19.
 // Returns the segments of the longest sequence in the upper and the chunks a segment in the lower 32 bits; 1 segment: no sequence is split.
 inline long long linattn_segments(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
     const int C = linattn_chunk(dtype, dk, dv);
     const long long nch = (max_len + C - 1) / C, all = (all_tokens + C - 1) / C * H * (backward || dtype ? 1 : (dv + 63) / 64);
-    const long long wgs = dtype && !backward && dv <= 64 ? 768 : 512;
+    const long long wgs = backward ? (dtype && dk > 64 ? 256 : 512) : dtype && dk <= 64 && dv <= 64 ? 768 : 512;
     long long segc = (all + wgs - 1) / wgs;
-    if (segc < 4) segc = 4;
-    if (segc >= nch) return (1LL << 32) | (nch > 0 ? nch : 1);
-    return (nch + segc - 1) / segc << 32 | segc;
+    if (segc < 2) segc = 2;
+    if (segc >= nch || nch < 6) return (1LL << 32) | (nch > 0 ? nch : 1);
+    const long long nseg = (nch + segc - 1) / segc;
+    return nseg << 32 | (nch + nseg - 1) / nseg;
 }
 
 // floats of one chunk's saved state.  bf16 kernels: accumulator order, padded to whole tiles (16-byte pieces of a wave side by side)

@@ -402,6 +402,10 @@ inline int linattn_problem(Problem &p, int dtype, const void *q, const void *k, 
     return 0;
 }
 
+// W neighbouring elements of a state, on any 32-bit word
+template <int W> struct Elements { typedef float type; };
+template <> struct Elements<4> { typedef f4 __attribute__((aligned(4))) type; };
+
 }  // namespace linattn
 
 // the pass over segments that leaves their own contributions (forward: k v^T; reverse: q dout^T, with q in the place of k and dout in that of v),

@@ -42,31 +42,36 @@ __device__ __forceinline__ float row16_sum(float v) {
     return v;
 }
 
-// seg_states[slot] = D behind the segment
+// seg_states[slot] = D behind the segment; one thread W elements
+template <int W>
 __global__ __launch_bounds__(NT) void la_join_bwd_kernel(const BwdArgs a, int C) {
+    typedef typename Elements<W>::type V;
     const Problem &p = a.p;
     const long long sz = (long long)p.dk * p.dv;
-    const int tiles = (int)((sz + NT - 1) / NT), nh = blockIdx.x / tiles, n = nh / p.H;
-    const long long e = (long long)(blockIdx.x % tiles) * NT + threadIdx.x;
+    const int tiles = (int)((sz + NT * W - 1) / (NT * W)), nh = blockIdx.x / tiles, n = nh / p.H;
+    const long long e = ((long long)(blockIdx.x % tiles) * NT + threadIdx.x) * W;
     const Seq s = get_seq(p, n);
     const int ns = segments_of(p, (s.len + C - 1) / C);
     if (e >= sz || ns <= 1) return;
-    float v = a.dlast ? a.dlast[nh * sz + e] : 0.0f;
+    const auto at = [](float *q) -> V & { return *reinterpret_cast<V *>(q); };
+    V v = V{};
+    if (a.dlast) v = *reinterpret_cast<const V *>(a.dlast + nh * sz + e);
     const long long first = (long long)first_slot(p, n, C) * p.H + nh % p.H, step = p.H * sz;
     float *u = a.seg_states + first * sz + e;
     const double *d = a.seg_decay + first;
     for (int i = ns - 1; i >= 0; i -= 8) {
-        float own[8], f[8];
+        V own[8];
+        float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int k = i - j > 1 ? i - j : 1;             // (the first segment's contribution is not there, and not used)
-            own[j] = u[k * step];
+            own[j] = at(u + k * step);
             f[j] = hw_exp2((float)d[(long long)k * p.H]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (i - j >= 0) {
-                u[(i - j) * step] = v;
+                at(u + (i - j) * step) = v;
                 v = v * f[j] + own[j];
             }
         }
@@ -856,7 +861,10 @@ extern "C" int ss2d_linattn_bwd(int dtype, const void *q, const void *k, const v
         r.k = q; r.kb = r.qb; r.kl = r.ql; r.kh = r.qh;
         r.v = dout; r.vb = tokens * H * dv; r.vl = (long long)H * dv; r.vh = dv;
         linattn_segment_pass(dtype, r, seg_states, seg_decay, true, s);
-        ss2d_launch(la_join_bwd_kernel, dim3((unsigned)((dk * dv + NT - 1) / NT * N * H)), dim3(NT), 0, s, a, linattn_chunk(dtype, dk, dv));
+        const int C = linattn_chunk(dtype, dk, dv), w = dk * dv % 4 == 0 ? 4 : 1;
+        const dim3 grid((unsigned)((dk * dv + NT * w - 1) / (NT * w) * N * H));
+        if (w == 4) ss2d_launch(la_join_bwd_kernel<4>, grid, dim3(NT), 0, s, a, C);
+        else ss2d_launch(la_join_bwd_kernel<1>, grid, dim3(NT), 0, s, a, C);
     }
     if (dtype == SS2D_DTYPE_F32) dispatch_bwd_f32(a, gaps, s);
     else if (a.p.vec) dispatch_bwd_bf16<true>(a, gaps, s);

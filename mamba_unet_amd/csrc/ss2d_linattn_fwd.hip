@@ -510,31 +510,36 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
     }
 }
 
-// joins the segments of a (sequence, head): seg_states[slot] = state in front of the segment; one thread per state element
+// joins the segments of a (sequence, head): seg_states[slot] = state in front of the segment; one thread W state elements
+template <int W>
 __global__ __launch_bounds__(NT) void la_join_fwd_kernel(const FwdArgs a, int C) {
+    typedef typename Elements<W>::type V;
     const Problem &p = a.p;
     const long long sz = (long long)p.dk * p.dv;
-    const int tiles = (int)((sz + NT - 1) / NT), nh = blockIdx.x / tiles, n = nh / p.H;
-    const long long e = (long long)(blockIdx.x % tiles) * NT + threadIdx.x;
+    const int tiles = (int)((sz + NT * W - 1) / (NT * W)), nh = blockIdx.x / tiles, n = nh / p.H;
+    const long long e = ((long long)(blockIdx.x % tiles) * NT + threadIdx.x) * W;
     const Seq s = get_seq(p, n);
     const int ns = segments_of(p, (s.len + C - 1) / C);
     if (e >= sz || ns <= 1) return;
-    float v = a.s0 ? a.s0[nh * sz + e] : 0.0f;
+    const auto at = [](float *q) -> V & { return *reinterpret_cast<V *>(q); };
+    V v = V{};
+    if (a.s0) v = *reinterpret_cast<const V *>(a.s0 + nh * sz + e);
     const long long first = (long long)first_slot(p, n, C) * p.H + nh % p.H, step = p.H * sz;
     float *u = a.seg_states + first * sz + e;
     const double *d = a.seg_decay + first;
     for (int i = 0; i < ns; i += 8) {                       // eight segments' loads are in flight at once
-        float own[8], f[8];
+        V own[8];
+        float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int k = i + j < ns - 1 ? i + j : ns - 2;  // (the last segment's contribution is not there, and not used)
-            own[j] = u[k * step];
+            own[j] = at(u + k * step);
             f[j] = hw_exp2((float)d[(long long)k * p.H]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (i + j < ns) {
-                u[(i + j) * step] = v;
+                at(u + (i + j) * step) = v;
                 v = v * f[j] + own[j];
             }
         }
@@ -605,7 +610,10 @@ extern "C" int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const v
     hipStream_t s = (hipStream_t)stream;
     if (nseg > 1) {
         linattn_segment_pass(dtype, a.p, seg_states, seg_decay, false, s);
-        ss2d_launch(la_join_fwd_kernel, dim3((unsigned)((dk * dv + NT - 1) / NT * N * H)), dim3(NT), 0, s, a, linattn_chunk(dtype, dk, dv));
+        const int C = linattn_chunk(dtype, dk, dv), w = dk * dv % 4 == 0 ? 4 : 1;
+        const dim3 grid((unsigned)((dk * dv + NT * w - 1) / (NT * w) * N * H));
+        if (w == 4) ss2d_launch(la_join_fwd_kernel<4>, grid, dim3(NT), 0, s, a, C);
+        else ss2d_launch(la_join_fwd_kernel<1>, grid, dim3(NT), 0, s, a, C);
     }
     dispatch<0>(dtype, a, gaps, s);
     rc = ss2d_take_launch_rc();

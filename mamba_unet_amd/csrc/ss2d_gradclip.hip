@@ -6,6 +6,8 @@
 //     depend on the order of execution, and scales its run.  A factor of 1 leaves the gradients untouched.
 // Memory-bound: read, then read and write.  The second pass runs through the pieces from the last to the first: what the
 // first pass read last is still in the last-level cache.
+// Measured: 240 tensors of 875,000 bf16 values (420 MB), norm 79 us (5.3 TB/s); 218 tensors of an image network (fp32, 19 M values) 14.5 + 7 us;
+// 218 tensors of 50 values 5 + 2 us.
 // A gradient may start at any element (a piece of a flat bucket): a piece's unaligned ends are done by single elements.
 #include <algorithm>
 #include "ss2d_common.h"
@@ -33,21 +35,33 @@ __device__ __forceinline__ int find_tensor(const Table &t, unsigned piece) {
     return lo;
 }
 
-// f(pointer, count, vector?) over the aligned middle and the unaligned ends of one piece
-template <typename T, typename Vec, typename One>
-__device__ __forceinline__ void walk_piece(T *p, unsigned n, Vec vec, One one) {
+// the aligned middle of a piece in 16-byte vectors, four of them a thread in flight at once (loads under a condition each wait for one another:
+// the norm of 630 MB in 145 us; this way 130, eight at once 135), and its unaligned ends
+template <typename T, typename Four, typename Vec, typename One>
+__device__ __forceinline__ void walk_piece(T *p, unsigned n, Four four, Vec vec, One one) {
     constexpr unsigned V = 16 / sizeof(T);
     unsigned head = (unsigned)((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T);
     head = head < n ? head : n;
     const unsigned nv = (n - head) / V, done = head + nv * V;
     T *m = p + head;
-    for (unsigned i = threadIdx.x; i < nv; i += 4 * NT) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (i + u * NT < nv) vec(m + (size_t)(i + u * NT) * V);
-    }
+    unsigned i = threadIdx.x;
+    for (; i + 3 * NT < nv; i += 4 * NT) four(m + (size_t)i * V);
+    for (; i < nv; i += NT) vec(m + (size_t)i * V);
     if (threadIdx.x < head) one(p + threadIdx.x);
     if (threadIdx.x < n - done) one(p + done + threadIdx.x);
+}
+template <typename T>
+__device__ __forceinline__ void unpack(u32x4 w, float (&v)[16 / sizeof(T)]) {
+    const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 4) {
+            v[i] = __builtin_bit_cast(float, u[i]);
+        } else {
+            v[(2 * i) % (16 / sizeof(T))] = __builtin_bit_cast(float, u[i] << 16);
+            v[(2 * i + 1) % (16 / sizeof(T))] = __builtin_bit_cast(float, u[i] & 0xffff0000u);
+        }
+    }
 }
 
 __device__ __forceinline__ double block_sum(double v, double *red) {
@@ -72,18 +86,29 @@ __device__ __forceinline__ double block_max(double v, double *red) {
 
 template <bool INF, typename T>
 __device__ __forceinline__ double piece_norm(const T *p, unsigned n) {
-    double acc = 0.0;
-    auto add = [&](float x) {
-        if (INF) acc = nan_max(acc, (double)fabsf(x));
-        else acc = fma((double)x, (double)x, acc);
+    constexpr int V = 16 / sizeof(T), STEP = NT * V;
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};                   // four sums: one chain of 64-bit additions would be slower than memory
+    const auto add = [&](double &s, float x) {
+        if (INF) s = nan_max(s, (double)fabsf(x));
+        else s = fma((double)x, (double)x, s);
+    };
+    const auto all = [&](u32x4 w) {
+        float v[V];
+        unpack<T>(w, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) add(acc[e % 4], v[e]);
     };
     walk_piece<const T>(p, n,
         [&](const T *q) {
+            u32x4 w[4];
 #pragma unroll
-            for (unsigned e = 0; e < 16 / sizeof(T); e += 4) { const f4 v = ld4(q + e); add(v.x); add(v.y); add(v.z); add(v.w); }
+            for (int u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const u32x4 *>(q + u * STEP);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) all(w[u]);
         },
-        [&](const T *q) { add(ld1(q)); });
-    return acc;
+        [&](const T *q) { all(*reinterpret_cast<const u32x4 *>(q)); },
+        [&](const T *q) { add(acc[0], ld1(q)); });
+    return INF ? nan_max(nan_max(acc[0], acc[1]), nan_max(acc[2], acc[3])) : (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
 
 template <bool INF>
@@ -107,11 +132,22 @@ __global__ __launch_bounds__(NT) void grad_norm_kernel(const Table t, double *pa
 
 template <typename T>
 __device__ __forceinline__ void piece_scale(T *p, unsigned n, float f) {
+    constexpr int V = 16 / sizeof(T), STEP = NT * V;
+    const auto put = [&](T *q, u32x4 w) {
+        float v[V];
+        unpack<T>(w, v);
+#pragma unroll
+        for (int e = 0; e < V; e += 4) st4(q + e, f4{v[e] * f, v[e + 1] * f, v[e + 2] * f, v[e + 3] * f});
+    };
     walk_piece<T>(p, n,
         [&](T *q) {
+            u32x4 w[4];
 #pragma unroll
-            for (unsigned e = 0; e < 16 / sizeof(T); e += 4) st4(q + e, ld4(q + e) * f);
+            for (int u = 0; u < 4; ++u) w[u] = *reinterpret_cast<const u32x4 *>(q + u * STEP);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) put(q + u * STEP, w[u]);
         },
+        [&](T *q) { put(q, *reinterpret_cast<const u32x4 *>(q)); },
         [&](T *q) { st1(q, ld1(q) * f); });
 }
 

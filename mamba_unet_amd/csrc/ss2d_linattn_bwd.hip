@@ -13,6 +13,10 @@
 //
 // A workgroup walks one segment of one sequence and value head from its end to its start with D in accumulator registers (a wave owns
 // 16-column slices of dv).  Segments as in the forward: own contributions, a join in order, the walk.
+//
+// Measured.  4 x 4096 tokens, 16 heads of 128 x 64 on 2 key heads, bf16: contributions 32 us, join 6, walk 195, sum over the heads of a group 47 (5.7 TB/s).  A
+// chunk takes a workgroup of 16 waves, one a CU (157 KB of LDS), 24,000 cycles: the matrix units are busy 17% of them and LDS 42% (a quarter of that bank
+// conflicts of 8-byte writes), the rest waits between the phases, which need each other's results.  24 x 3136 tokens, 3 heads of 16 x 64 fp32: 15.6 + 4.8 + 120 us.
 #include "ss2d_linattn.h"
 #include "../../include/ss2d.h"
 

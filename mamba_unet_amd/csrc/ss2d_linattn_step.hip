@@ -3,7 +3,8 @@
 // on the states of a pool, in place.  Bound by the state: dk * dv fp32 values are read and written once for every request and head, all
 // else is small.  A workgroup takes one (request, head) and a slice of dv: its threads hold the slice in registers (four columns x every
 // RG-th row each), so every state element is loaded once, updated, stored and multiplied into the output, and the partial sums over dk
-// meet in LDS.
+// meet in LDS.  Measured: 250 requests, 32 heads of 128 x 64, 93 us (527 MB, 5.7 TB/s, some of it from the last-level cache; 111 with a cold one); one request,
+// 16 heads of 64 x 64, 4.7 us, a launch; 128 requests, 16 heads of 64 x 65 (a second workgroup for the last column) 27 us, of 64 x 64 16.
 //
 // With slot indices two requests may name one slot.  Then the first of them applies all of that slot's tokens in request order,
 // and the others leave: the result does not depend on the order of execution.

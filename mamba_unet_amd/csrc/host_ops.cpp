@@ -86,10 +86,8 @@ bool any_requires_grad(std::initializer_list<Named> all) {
 }
 
 // Gradients that come from kernels have no graph of their own: asked for with create_graph they raise when they are differentiated again.
-variable_list once(variable_list out, const variable_list &grads) {
-    bool want = false;
-    for (const Tensor &g : grads) want = want || (g.defined() && g.requires_grad());
-    if (!at::GradMode::is_enabled() || !want) return out;
+variable_list once(variable_list out) {
+    if (!at::GradMode::is_enabled()) return out;
     for (Tensor &t : out)
         if (t.defined()) t = t.detach().set_requires_grad(true);
     return torch::autograd::DelayedError("trying to differentiate twice an operator whose backward is a kernel", (int)out.size())(std::move(out));
@@ -224,7 +222,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
             const at::NoGradGuard no_grad;
             run(ctx, dout, dlast, res);
         }
-        return once(std::move(res), grads);
+        return once(std::move(res));
     }
     static void run(AutogradContext *ctx, const Tensor &dout, const Tensor &dlast, variable_list &res) {
         const variable_list saved = ctx->get_saved_variables();
@@ -260,7 +258,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         }
         if (g.dim() == 1 && want_g) {                  // a decay for each head: the sum over all tokens (in a fixed order, and right in a replayed graph)
             const Tensor all = dg;
-            dg = at::zeros({d.H}, all.options());
+            dg = d.L > 0 ? empty({d.H}, dev) : at::zeros({d.H}, all.options());
             if (d.L > 0) {
                 const Tensor ws = empty({(int64_t)api.ss2d_colsum_workspace_floats((int)d.H)}, dev);
                 const Here here(dev);
@@ -405,7 +403,7 @@ struct NormGateResidual : torch::autograd::Function<NormGateResidual> {
             const at::NoGradGuard no_grad;
             run(ctx, grads[0], grads[1], res);
         }
-        return once(std::move(res), grads);
+        return once(std::move(res));
     }
     static void run(AutogradContext *ctx, const Tensor &dxo, const Tensor &dh, variable_list &res) {
         const variable_list saved = ctx->get_saved_variables();

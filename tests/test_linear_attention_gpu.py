@@ -506,3 +506,61 @@ def test_more_sequences_than_a_grid_axis_holds():
     t = {m: None if x is None else x.cpu() for m, x in t.items()}
     ref, size = (reference(t, [L], False, 1.0, absolute=a) for a in (False, True))
     check({"out": out[:, lo:lo + L], "last": last[lo:lo + 1]}, ref, size, steps_of([L], dk, dv))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_expanded_and_single_row_views(dtype):
+    """Tensors that repeat a row over tokens, batch or heads, and a row whose token stride means nothing, give what copies of them give."""
+    t = {n: x.cuda() for n, x in make([70, 70], False, 4, 2, 16, 24, dtype, seed=9).items()}
+    views = {"q": t["q"][:, :1].expand(-1, 70, -1, -1), "k": t["k"][:1].expand(2, -1, -1, -1), "v": t["v"][:, :, :1].expand(-1, -1, 4, -1), "g": t["g"][:, :, :1].expand(-1, -1, 4)}
+    names = ("q", "k", "v", "g")
+    dense = {n: x.contiguous() for n, x in views.items()}
+    for use in ({"q"}, {"k"}, {"v"}, {"g"}, set(names)):
+        res = []
+        for d in (views, dense):
+            leaves = [(d[n] if n in use else t[n]).detach().requires_grad_() for n in names]
+            out = linear_attention_fn(*leaves, initial_state=t["s0"])
+            res.append([out, *torch.autograd.grad(out, leaves, t["do"])])
+        assert all(torch.equal(a, b) for a, b in zip(*res))
+    one = {n: t[n][:, :1] for n in names}
+    odd = {n: x.as_strided(x.shape, (x.stride(0), 1, *x.stride()[2:])) for n, x in one.items()}
+    want = linear_attention_fn(*[one[n].contiguous() for n in names], initial_state=t["s0"])
+    assert torch.equal(linear_attention_fn(*[odd[n] for n in names], initial_state=t["s0"]), want)
+    far = torch.empty_strided(t["v"].shape, (128, 1 << 23, 24, 1), device="cuda", dtype=dtype)[:, :3].copy_(t["v"][:, :3])
+    q, k, g = (t[n][:, :3] for n in ("q", "k", "g"))
+    assert torch.equal(linear_attention_fn(q, k, far, g), linear_attention_fn(q, k, t["v"][:, :3], g))
+
+
+def test_differentiating_twice_raises():
+    from mamba_unet_amd import norm_gate_residual
+    t = {n: x.cuda() for n, x in make([5], False, 2, 2, 16, 16, torch.float32).items()}
+    q = t["q"].requires_grad_()
+    for out in (linear_attention_fn(q, t["k"], t["v"], t["g"]), norm_gate_residual(q, t["k"], torch.ones(16).cuda(), torch.ones(16).cuda())[1]):
+        g, = torch.autograd.grad(out.sum(), q, create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            (g ** 2).sum().backward()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_in_the_backward(reentrant):
+    from torch.utils.checkpoint import checkpoint
+    t = {n: x.cuda() for n, x in make([130, 130], False, 4, 2, 32, 32, torch.bfloat16, seed=2).items()}
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g")]
+    call = lambda *a: linear_attention_fn(*a)  # noqa: E731
+    grads = []
+    for out in (call(*leaves), checkpoint(call, *leaves, use_reentrant=reentrant)):
+        for x in leaves:
+            x.grad = None
+        out.backward(t["do"])
+        grads.append([x.grad.clone() for x in leaves])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_a_changed_input_is_noticed():
+    t = {n: x.cuda() for n, x in make([40], False, 2, 2, 16, 16, torch.float32).items()}
+    k = t["k"].clone().requires_grad_()
+    out = linear_attention_fn(t["q"].requires_grad_(), k * 1.0, t["v"], t["g"])
+    q2 = t["q"].detach()
+    q2.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()

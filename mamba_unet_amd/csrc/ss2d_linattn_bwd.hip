@@ -96,13 +96,17 @@ constexpr int GAP_WGS = 16;
 // v_mfma_f32_16x16x4_f32.  A lane holds row / column l16 of an operand and contracted indices 4 gq + r of a 16-block in step r: direct operands are
 // 16-byte LDS reads, transposed ones four 4-byte reads, both free of bank conflicts at a pitch of 4 mod 16 floats.  LDS holds the four tiles, X,
 // Y and one state at a time: S (for dq), then D (for dk, dv).  The next chunk is in flight in registers.
-template <int DK, int DV, int C, bool VEC>
-__global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
-    constexpr int NT = 1024, PK = DK + 4, PV = DV + 4, PP = C + 4, KT = DK / 16, VT = DV / 16, CT = C / 16;
-    constexpr int TW = (KT * VT + 15) / 16;                          // tiles of D a wave owns: wave + 16 m
-    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * C * PP + 10 * 64 + 16 * 64 + 32];
-    float *Qs = lds, *Ks = Qs + C * PK, *Vs = Ks + C * PK, *Os = Vs + C * PV, *St = Os + C * PV, *Xs = St + DK * PV, *Ys = Xs + C * PP;
-    float *decays = Ys + C * PP, *parts = decays + 10 * 64, *corners = parts + 16 * 64;
+template <int DK, int DV, int C, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
+    constexpr int NT = 64 * NW, PK = DK + 4, PV = DV + 4, PP = 20, KT = DK / 16, VT = DV / 16, CT = C / 16;
+    constexpr int TW = (KT * VT + NW - 1) / NW;                      // tiles of D a wave owns: wave + NW m
+    constexpr int XY = CT * (CT + 1) / 2 * 16 * PP;                  // X, Y: their tiles up to the diagonal
+    constexpr int NV = (VT * CT + NW - 1) / NW;                      // tiles of dv a wave owns
+    static_assert(KT * CT <= NW && NV <= 2, "tiles of a wave");
+    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * XY + 10 * 64 + NW * 64 + 2 * NW];
+    float *Qs = lds, *Ks = Qs + C * PK, *Vs = Ks + C * PK, *Os = Vs + C * PV, *St = Os + C * PV, *Xs = St + DK * PV, *Ys = Xs + XY;
+    float *decays = Ys + XY, *parts = decays + 10 * 64, *corners = parts + NW * 64;
+    const auto tile_at = [](int it, int jt) { return (it * (it + 1) / 2 + jt) * 16 * PP; };
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -139,11 +143,11 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
     float *DKp = static_cast<float *>(a.dk_) + ((t0 + e0) * hq + h) * (long long)p.dk;
     float *DVp = static_cast<float *>(a.dv_) + ((t0 + e0) * p.H + h) * (long long)p.dv;
     float *DG = a.dg + t0 * p.H + h;
-    // one tile each; the last waves take dq and dk first, the first waves the scores
-    const int wq = 15 - wave, qk = wq % KT, qi = wq / KT, vt = wave % VT, vj = wave / VT;
+    // one tile of dq and dk at most; the last waves take them first, the first waves the scores
+    const int wq = NW - 1 - wave, qk = wq % KT, qi = wq / KT, vt = wave % VT;
     const bool has_q = wq < KT * CT, has_v = wave < VT * CT;
     auto state_at = [&](int m, int r, int ln) {                      // element (t, r) of this lane's part of a state: row k, column dv; -1: outside
-        const int t = wave + 16 * m, k = 16 * (t / VT) + 4 * (ln >> 4) + r, c = 16 * (t % VT) + (ln & 15);
+        const int t = wave + NW * m, k = 16 * (t / VT) + 4 * (ln >> 4) + r, c = 16 * (t % VT) + (ln & 15);
         return t < KT * VT && k < p.dk && c < p.dv ? k * p.dv + c : -1;
     };
     f4 D[TW], sr[TW];
@@ -200,7 +204,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
         if (wave == 1) {
             double x = 0.0, e = 0.0, first = 0.0;
 #pragma unroll
-            for (int w = 0; w < 16; ++w) { x += (double)parts[w * 64 + lane0]; e += (double)corners[w]; first += (double)corners[16 + w]; }
+            for (int w = 0; w < NW; ++w) { x += (double)parts[w * 64 + lane0]; e += (double)corners[w]; first += (double)corners[NW + w]; }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_down(x, d, 64);
@@ -213,7 +217,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
         const int ln = fresh(lane0);
 #pragma unroll
         for (int m = 0; m < TW; ++m) {
-            const int t = wave + 16 * m;
+            const int t = wave + NW * m;
             if (t < KT * VT) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) St[(16 * (t / VT) + 4 * (ln >> 4) + r) * PV + 16 * (t % VT) + (ln & 15)] = x[m][r];
@@ -250,7 +254,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
         parts[wave * 64 + lane] = 0.0f;
         // X, Y and the sums of M below the diagonal
 #pragma unroll 1
-        for (int t = wave; t < CT * (CT + 1) / 2; t += 16) {
+        for (int t = wave; t < CT * (CT + 1) / 2; t += NW) {
             const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
             f4 x = f4{0, 0, 0, 0}, y = f4{0, 0, 0, 0};
 #pragma unroll
@@ -268,8 +272,8 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
                 const int i = 16 * it + 4 * gq + r;
                 const float w = p.scale * hw_exp2((hi[r] - hj) + (li[r] - lj));
                 const float yw = j <= i ? y[r] * w : 0.0f, m = j < i ? x[r] * yw : 0.0f;
-                Xs[i * PP + j] = j <= i ? x[r] * w : 0.0f;
-                Ys[i * PP + j] = yw;
+                Xs[16 * PP * t + (4 * gq + r) * PP + l16] = j <= i ? x[r] * w : 0.0f;
+                Ys[16 * PP * t + (4 * gq + r) * PP + l16] = yw;
                 colsum += m;
                 const float rs = row16_sum(m);
                 if (l16 == 0) parts[wave * 64 + i] += rs;
@@ -301,7 +305,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
                 f4 y;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) y[r] = Ks[(16 * jt + 4 * gq + r) * PK + k];
-                dq = dot4(*reinterpret_cast<const f4 *>(Ys + (16 * qi + l16) * PP + 16 * jt + 4 * gq), y, dq);
+                dq = dot4(*reinterpret_cast<const f4 *>(Ys + tile_at(qi, jt) + l16 * PP + 4 * gq), y, dq);
             }
             const RowsOut out(DQ, nr, ldq);
 #pragma unroll
@@ -329,7 +333,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
                 f4 x, y;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    x[r] = Ys[(16 * it + 4 * gq + r) * PP + 16 * qi + l16];
+                    x[r] = Ys[tile_at(it, qi) + (4 * gq + r) * PP + l16];
                     y[r] = Qs[(16 * it + 4 * gq + r) * PK + k];
                 }
                 dk = dot4(x, y, dk);
@@ -340,9 +344,11 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
         }
         corner = lanes_sum<64>(corner);
         front = lanes_sum<64>(front);
-        if (lane == 0) { corners[wave] = corner; corners[16 + wave] = front; }
-        if (has_v) {
-            const int col = 16 * vt + l16;
+        if (lane == 0) { corners[wave] = corner; corners[NW + wave] = front; }
+#pragma unroll
+        for (int m = 0; m < NV; ++m) {
+            if (!has_v) break;
+            const int vj = m ? CT - 1 - wave / VT : wave / VT, col = 16 * vt + l16;      // a long column of products with a short one
             f4 dv = f4{0, 0, 0, 0};
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
@@ -356,7 +362,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
                 f4 x, y;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    x[r] = Xs[(16 * it + 4 * gq + r) * PP + 16 * vj + l16];
+                    x[r] = Xs[tile_at(it, vj) + (4 * gq + r) * PP + l16];
                     y[r] = Os[(16 * it + 4 * gq + r) * PV + col];
                 }
                 dv = dot4(x, y, dv);
@@ -370,7 +376,7 @@ __global__ __launch_bounds__(1024, 4) void la_bwd_kernel(const BwdArgs a) {
         fetch_g(c - 2);
 #pragma unroll
         for (int m = 0; m < TW; ++m) {
-            const int t = wave + 16 * m;
+            const int t = wave + NW * m;
             if (t >= KT * VT) break;
             D[m] *= eend;
 #pragma unroll
@@ -801,22 +807,22 @@ void launch_head_sum(const float *a, const float *b, void *oa, void *ob, long lo
     else ss2d_launch((la_head_sum_kernel<1, IO>), grid, dim3(NT), 0, s, a, b, static_cast<IO *>(oa), static_cast<IO *>(ob), total, rep, dk);
 }
 
-template <int DK, int DV, int C>
+template <int DK, int DV, int C, int NW>
 void launch_bwd(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     const unsigned walks = (unsigned)((long long)a.p.slots * a.p.H);
-    if (a.p.vec) ss2d_launch((la_bwd_kernel<DK, DV, C, true>), dim3(walks + gaps), dim3(1024), 0, s, a);
-    else ss2d_launch((la_bwd_kernel<DK, DV, C, false>), dim3(walks + gaps), dim3(1024), 0, s, a);
+    if (a.p.vec) ss2d_launch((la_bwd_kernel<DK, DV, C, NW, true>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
+    else ss2d_launch((la_bwd_kernel<DK, DV, C, NW, false>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
 }
 void dispatch_bwd_f32(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     const int dk = a.p.dk, dv = a.p.dv;
     if (dv <= 64) {
-        if (dk <= 16) launch_bwd<16, 64, 64>(a, gaps, s);
-        else if (dk <= 64) launch_bwd<64, 64, 64>(a, gaps, s);
-        else launch_bwd<128, 64, 32>(a, gaps, s);
+        if (dk <= 16) launch_bwd<16, 64, 64, 8>(a, gaps, s);
+        else if (dk <= 64) launch_bwd<64, 64, 64, 16>(a, gaps, s);
+        else launch_bwd<128, 64, 32, 16>(a, gaps, s);
     } else {
-        if (dk <= 16) launch_bwd<16, 128, 32>(a, gaps, s);
-        else if (dk <= 64) launch_bwd<64, 128, 32>(a, gaps, s);
-        else launch_bwd<128, 128, 32>(a, gaps, s);
+        if (dk <= 16) launch_bwd<16, 128, 32, 8>(a, gaps, s);
+        else if (dk <= 64) launch_bwd<64, 128, 32, 16>(a, gaps, s);
+        else launch_bwd<128, 128, 32, 16>(a, gaps, s);
     }
 }
 

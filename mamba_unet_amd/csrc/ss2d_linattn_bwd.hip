@@ -411,14 +411,19 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
 // Direct operands are eight values in a row (one 16-byte LDS read); what they are multiplied with, where it is read transposed, takes its contracted
 // rows in the same order (frag_tc).  Products of two transposed operands (over tokens) use frag_t for both.
 template <int DK, int DV, int NW, bool VEC, typename QT>
-__global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(64 * NW, DK <= 32 && DV <= 64 ? 4 : NW / 4) void la_bwd_bf16_kernel(const BwdArgs a) {
     constexpr int NT = 64 * NW, C = 64, KT = DK / 16, KS = DK / 32, VT = DV / 16, VS = DV / 32;
-    constexpr int QP = 2 * DK + 32, VP = 2 * DV + 32, PP = 2 * C + 32, SP = 2 * DK + 16;      // bytes a row
+    constexpr int QP = 2 * DK + 32, VP = 2 * DV + 32, SP = 2 * DK + 16;      // bytes a row
+    // X and Y: rows of the lower half hold one block of 32 columns, of the upper half two (up to 32 x 64: packed, so that two workgroups fit a CU)
+    constexpr bool PACKED = DK <= 32 && DV <= 64;
+    constexpr int P0 = PACKED ? C + 16 : 2 * C + 32, P1 = PACKED ? 2 * C + 16 : 2 * C + 32, XY = 32 * (P0 + P1);
+    const auto pitch = [](int half) { return half ? P1 : P0; };
+    const auto rows32 = [](int half) { return half ? 32 * (P0 - P1) : 0; };                   // where row 0 would lie at that half's pitch
     constexpr int NB = DK == 128 && DV == 128 ? 1 : 3;                                        // terms of a state in LDS at once
     constexpr int NI = 4 * KT / NW, NJ = 4 * VT / NW, TW = KT * VT / NW;                               // tiles of a wave: rows of dq / dk, rows of dv, D
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * C * PP + NB * DV * SP + (10 * C + NW * C + 2 * NW) * 4];
-    unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + C * PP, *Yh = Xl + C * PP,
-                  *Yl = Yh + C * PP, *St = Yl + C * PP;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + 2 * NW) * 4];
+    unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + XY, *Yh = Xl + XY,
+                  *Yl = Yh + XY, *St = Yl + XY;
     float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + NW * C;
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
@@ -538,7 +543,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
         }
     };
     if (tid < 128) {                             // the tiles of X and Y behind the diagonal that are read with it (32 columns at a time): zero for good
-        const int i = 32 * (tid >> 6) + (tid & 15), at = i * PP + 2 * (32 * (tid >> 6) + 16 + 4 * ((tid >> 4) & 3));
+        const int half = tid >> 6, i = 32 * half + (tid & 15), at = rows32(half) + i * pitch(half) + 2 * (32 * half + 16 + 4 * ((tid >> 4) & 3));
         *reinterpret_cast<u32x2 *>(Xh + at) = u32x2{0, 0};
         *reinterpret_cast<u32x2 *>(Xl + at) = u32x2{0, 0};
         *reinterpret_cast<u32x2 *>(Yh + at) = u32x2{0, 0};
@@ -584,7 +589,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
                 m[r] = j + r < i ? x[r] * y[r] : 0.0f;
                 x[r] = j + r <= i ? x[r] * w : 0.0f;
             }
-            const int at = i * PP + 2 * j;
+            const int at = rows32(it / 2) + i * pitch(it / 2) + 2 * j;
             const bf16x4 xh = round4(x), yh = round4(y);
             *reinterpret_cast<bf16x4 *>(Xh + at) = xh;
             *reinterpret_cast<bf16x4 *>(Xl + at) = round4(rest4(x, xh));
@@ -644,8 +649,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
 #pragma unroll
                 for (int m = 0; m < NI; ++m) {
                     if (js > (i0 + m) / 2) continue;
-                    acc[m] = mfma8(kf, frag_c(Yh, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
-                    acc[m] = mfma8(kf, frag_c(Yl, PP, 16 * (i0 + m) + l16, js, gq), acc[m]);
+                    acc[m] = mfma8(kf, frag_c(Yh + rows32((i0 + m) / 2), pitch((i0 + m) / 2), 16 * (i0 + m) + l16, js, gq), acc[m]);
+                    acc[m] = mfma8(kf, frag_c(Yl + rows32((i0 + m) / 2), pitch((i0 + m) / 2), 16 * (i0 + m) + l16, js, gq), acc[m]);
                 }
             }
             const RowsOut out(DQ, nr, ldq);
@@ -723,14 +728,14 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void la_bwd_bf16_kernel(const BwdA
 #pragma unroll
                 for (int m = 0; m < NI; ++m) {
                     if (is < (i0 + m) / 2) continue;
-                    dk[m] = mfma8(qf, frag_t(Yh, PP, i0 + m, is, lane), dk[m]);
-                    dk[m] = mfma8(qf, frag_t(Yl, PP, i0 + m, is, lane), dk[m]);
+                    dk[m] = mfma8(qf, frag_t(Yh + rows32(is), pitch(is), i0 + m, is, lane), dk[m]);
+                    dk[m] = mfma8(qf, frag_t(Yl + rows32(is), pitch(is), i0 + m, is, lane), dk[m]);
                 }
 #pragma unroll
                 for (int m = 0; m < NJ; ++m) {
                     if (is < (j0 + m) / 2) continue;
-                    dv[m] = mfma8(of, frag_t(Xh, PP, j0 + m, is, lane), dv[m]);
-                    dv[m] = mfma8(of, frag_t(Xl, PP, j0 + m, is, lane), dv[m]);
+                    dv[m] = mfma8(of, frag_t(Xh + rows32(is), pitch(is), j0 + m, is, lane), dv[m]);
+                    dv[m] = mfma8(of, frag_t(Xl + rows32(is), pitch(is), j0 + m, is, lane), dv[m]);
                 }
             }
             const int k = 16 * kt + 4 * gq, v = 16 * vt + 4 * gq;

@@ -16,7 +16,7 @@
 //
 // Measured.  4 x 4096 tokens, 16 heads of 128 x 64 on 2 key heads, bf16: contributions 32 us, join 6, walk 195, sum over the heads of a group 47 (5.7 TB/s).  A
 // chunk takes a workgroup of 16 waves, one a CU (157 KB of LDS), 24,000 cycles: the matrix units are busy 17% of them and LDS 42% (a quarter of that bank
-// conflicts of 8-byte writes), the rest waits between the phases, which need each other's results.  24 x 3136 tokens, 3 heads of 16 x 64 fp32: 15.6 + 4.8 + 120 us.
+// conflicts of 8-byte writes), the rest waits between the phases, which need each other's results.  24 x 3136 tokens, 3 heads of 16 x 64 fp32: 15.6 + 4.8 + 96 us.
 #include "ss2d_linattn.h"
 #include "../../include/ss2d.h"
 
@@ -93,7 +93,8 @@ __device__ void zero_rows(const Problem &p, IO *o, long long row, int w, int nw)
 constexpr int GAP_WGS = 16;
 
 // fp32: 16 waves a workgroup, so that every result of a chunk -- dq, dk (C x dk) and dv (C x dv) -- is at most one 16 x 16 tile a wave on
-// v_mfma_f32_16x16x4_f32.  A lane holds row / column l16 of an operand and contracted indices 4 gq + r of a 16-block in step r: direct operands are
+// v_mfma_f32_16x16x4_f32; keys up to 16 wide: 8 waves with two tiles of dv, and two workgroups a CU (24 x 3136 tokens, 3 heads of 16 x 64: 96 us, one
+// workgroup of 16 waves 120).  A lane holds row / column l16 of an operand and contracted indices 4 gq + r of a 16-block in step r: direct operands are
 // 16-byte LDS reads, transposed ones four 4-byte reads, both free of bank conflicts at a pitch of 4 mod 16 floats.  LDS holds the four tiles, X,
 // Y and one state at a time: S (for dq), then D (for dk, dv).  The next chunk is in flight in registers.
 template <int DK, int DV, int C, int NW, bool VEC>
@@ -405,21 +406,25 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
     }
 }
 
-// The same walk for bf16 tensors on the bf16 matrix instruction: chunks of 64, 16 waves a workgroup (dk <= 32: 8).  LDS holds the four tiles, X and Y (two terms
-// each) and the terms of ONE state at a time, transposed (dv x dk): first S (for dq), then D (for dk and dv); with NB = 1 (128 x 128) one
+// The same walk for bf16 tensors on the bf16 matrix instruction: chunks of 64, 16 waves a workgroup (dk <= 32 and 64 x 64: 8).  LDS holds the four tiles, X and Y (two terms
+// each) and the terms of ONE state at a time, transposed (dv x dk): first S (for dq), then D (for dk and dv); with NB = 1 (64 x 64, 128 x 128) one
 // term at a time.  States enter with three terms where dg is taken from the product (q . S do, k . D v), with two in dv.
 // Direct operands are eight values in a row (one 16-byte LDS read); what they are multiplied with, where it is read transposed, takes its contracted
 // rows in the same order (frag_tc).  Products of two transposed operands (over tokens) use frag_t for both.
+//
+// Up to 64 x 64 two workgroups of eight waves share a CU, so that one works while the other waits at its barriers: X and Y are packed below the diagonal,
+// and at 64 x 64 rows are half a pitch step shorter and a state's terms take turns (24 x 3136 tokens, 3 heads of 16 x 64, forward and
+// backward: 142 us with one workgroup of eight waves a CU, 123 with two; 4 x 4096, 16 heads of 64 x 64: 220 with one of sixteen, 208 with two of eight).
 template <int DK, int DV, int NW, bool VEC, typename QT>
-__global__ __launch_bounds__(64 * NW, DK <= 32 && DV <= 64 ? 4 : NW / 4) void la_bwd_bf16_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la_bwd_bf16_kernel(const BwdArgs a) {
     constexpr int NT = 64 * NW, C = 64, KT = DK / 16, KS = DK / 32, VT = DV / 16, VS = DV / 32;
-    constexpr int QP = 2 * DK + 32, VP = 2 * DV + 32, SP = 2 * DK + 16;      // bytes a row
-    // X and Y: rows of the lower half hold one block of 32 columns, of the upper half two (up to 32 x 64: packed, so that two workgroups fit a CU)
-    constexpr bool PACKED = DK <= 32 && DV <= 64;
+    constexpr bool PACKED = DK <= 64 && DV <= 64, TIGHT = DK == 64 && DV == 64;
+    constexpr int QP = 2 * DK + (TIGHT ? 16 : 32), VP = 2 * DV + (TIGHT ? 16 : 32), SP = 2 * DK + 16;      // bytes a row
+    // X and Y: the first 32 rows need one block of 32 columns, the others two
     constexpr int P0 = PACKED ? C + 16 : 2 * C + 32, P1 = PACKED ? 2 * C + 16 : 2 * C + 32, XY = 32 * (P0 + P1);
     const auto pitch = [](int half) { return half ? P1 : P0; };
     const auto rows32 = [](int half) { return half ? 32 * (P0 - P1) : 0; };                   // where row 0 would lie at that half's pitch
-    constexpr int NB = DK == 128 && DV == 128 ? 1 : 3;                                        // terms of a state in LDS at once
+    constexpr int NB = TIGHT || (DK == 128 && DV == 128) ? 1 : 3;                                      // terms of a state in LDS at once
     constexpr int NI = 4 * KT / NW, NJ = 4 * VT / NW, TW = KT * VT / NW;                               // tiles of a wave: rows of dq / dk, rows of dv, D
     __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + 2 * NW) * 4];
     unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + XY, *Yh = Xl + XY,
@@ -834,7 +839,7 @@ void dispatch_bwd_f32(const BwdArgs &a, unsigned gaps, hipStream_t s) {
 template <int DK, int DV, bool VEC>
 void launch_bwd_bf16(const BwdArgs &a, unsigned gaps, hipStream_t s) {
     const unsigned walks = (unsigned)((long long)a.p.slots * a.p.H);
-    constexpr int NW = DK <= 32 ? 8 : 16;
+    constexpr int NW = DK <= 32 || (DK == 64 && DV == 64) ? 8 : 16;
     if (a.p.H > a.p.G) ss2d_launch((la_bwd_bf16_kernel<DK, DV, NW, VEC, float>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
     else ss2d_launch((la_bwd_bf16_kernel<DK, DV, NW, VEC, bf16>), dim3(walks + gaps), dim3(64 * NW), 0, s, a);
 }

@@ -426,6 +426,7 @@ int ss2d_linattn_fwd(int dtype, const void *q, const void *k, const void *v, con
                      int nseg, int seg_chunks, void *stream);
 /* dout (rows, tokens, H, dv) and dlast (null: 0) -> dq, dk (rows, tokens, G, dk), dv (rows, tokens, H, dv), dg (rows, tokens, H) fp32, ds0 (null: not
  * wanted).  With H > G the value heads' dq / dk go to dq_heads / dk_heads (rows, tokens, H, dk) fp32 first and are added in head order.
+ * A token stride of 0 of g says that a head has one decay: dg then holds the sum over every chunk's tokens at its first one and 0 at the others.
  * No atomics: results do not depend on the order of execution. */
 int ss2d_linattn_bwd(int dtype, const void *q, const void *k, const void *v, const float *g, const long long *strides, const int *cu_seqlens,
                      const void *dout, const float *dlast, const float *chunk_states, void *dq, void *dk_out, void *dv_out, float *dg, float *ds0,

@@ -196,6 +196,11 @@ Attention attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, c
     return r;
 }
 
+// a decay for every token has a token stride (0 says: one for each head)
+Tensor decays(const Tensor &g) {
+    const Tensor t = cast(g, at::kFloat);
+    return t.dim() == 3 && t.stride(1) == 0 && t.size(1) > 1 ? t.contiguous() : t;
+}
 Tensor fp32_dense(const Tensor &t) { return t.defined() ? cast(t, at::kFloat).contiguous() : t; }
 
 struct LinearAttention : torch::autograd::Function<LinearAttention> {
@@ -203,7 +208,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
                                  double scale, int64_t longest, bool want_last) {
         const Dims d = attention_dims(q, k, v, g, get(s0), get(cu));
         const at::ScalarType io = storage(q, k, v);
-        const Tensor q_ = operand(q, io), k_ = operand(k, io), v_ = operand(v, io), g_ = cast(g, at::kFloat);
+        const Tensor q_ = operand(q, io), k_ = operand(k, io), v_ = operand(v, io), g_ = decays(g);
         const Attention r = attention_forward(q_, k_, v_, g_, fp32_dense(get(s0)), get(cu), scale, d, longest, want_last, true);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({q_, k_, v_, g_, get(cu), r.chunks});

@@ -9,7 +9,8 @@
 // with the state in front of the chunk as one more column, D as one more row.  It is taken as row sums minus column sums, added
 // up from the chunk's end; pairs that do not cross t cancel there, but only pairs of ONE chunk, and the diagonal, whose terms
 // are the largest and cross nothing, never enters.  The chunk's first decay is crossed by the pairs with the state alone: their sum, exactly 0 at a
-// start without a state.
+// start without a state.  One decay for all tokens of a head (token stride 0) has the sum over t for its gradient: every pair times the number of decays that it
+// crosses, without differences; a chunk's part is left at its first token.
 //
 // A workgroup walks one segment of one sequence and value head from its end to its start with D in accumulator registers (a wave owns
 // 16-column slices of dv).  Segments as in the forward: own contributions, a join in order, the walk.
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
     constexpr int XY = CT * (CT + 1) / 2 * 16 * PP;                  // X, Y: their tiles up to the diagonal
     constexpr int NV = (VT * CT + NW - 1) / NW;                      // tiles of dv a wave owns
     static_assert(KT * CT <= NW && NV <= 2, "tiles of a wave");
-    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * XY + 10 * 64 + NW * 64 + 2 * NW];
+    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * XY + 10 * 64 + NW * 64 + 3 * NW];
     float *Qs = lds, *Ks = Qs + C * PK, *Vs = Ks + C * PK, *Os = Vs + C * PV, *St = Os + C * PV, *Xs = St + DK * PV, *Ys = Xs + XY;
     float *decays = Ys + XY, *parts = decays + 10 * 64, *corners = parts + NW * 64;
     const auto tile_at = [](int it, int jt) { return (it * (it + 1) / 2 + jt) * 16 * PP; };
@@ -203,15 +204,16 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
     };
     auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: gradients of b inside the chunk, summed from its end
         if (wave == 1) {
-            double x = 0.0, e = 0.0, first = 0.0;
+            double x = 0.0, e = 0.0, first = 0.0, all = 0.0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) { x += (double)parts[w * 64 + lane0]; e += (double)corners[w]; first += (double)corners[NW + w]; }
+            for (int w = 0; w < NW; ++w) { x += (double)parts[w * 64 + lane0]; e += (double)corners[w]; first += (double)corners[NW + w]; all += (double)corners[2 * NW + w]; }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_down(x, d, 64);
                 if (lane0 + d < 64) x += o;
             }
-            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(lane0 ? x + e : first);
+            const double dg = p.gl == 0 ? (lane0 ? 0.0 : all) : lane0 ? x + e : first;
+            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)dg;
         }
     };
     auto put_state = [&](const f4 (&x)[TW]) {
@@ -252,6 +254,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
         if (c > c0) fetch(c - 1);
         __syncthreads();
         const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
+        float whole = 0.0f;                                          // every pair times the decays it crosses
         parts[wave * 64 + lane] = 0.0f;
         // X, Y and the sums of M below the diagonal
 #pragma unroll 1
@@ -276,6 +279,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
                 Xs[16 * PP * t + (4 * gq + r) * PP + l16] = j <= i ? x[r] * w : 0.0f;
                 Ys[16 * PP * t + (4 * gq + r) * PP + l16] = yw;
                 colsum += m;
+                whole += m * (float)(i - j);
                 const float rs = row16_sum(m);
                 if (l16 == 0) parts[wave * 64 + i] += rs;
             }
@@ -296,6 +300,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
                 const int i = 16 * qi + 4 * gq + r;
                 const float qs = dq[r] * Qs[i * PK + k], rs = row16_sum(qs);
                 front += qs;
+                whole += qs * (float)(i + 1);
                 if (l16 == 0) parts[wave * 64 + i] += rs;
             }
         }
@@ -316,6 +321,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
         const float eend = tail[0];
         corner *= eend;
         front += corner;
+        whole += corner * (float)nr;
         if (has_q) {
             f4 dk = f4{0, 0, 0, 0};
 #pragma unroll
@@ -327,6 +333,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
                 const int j = 16 * qi + 4 * gq + r;
                 const float kk = dk[r] * Ks[j * PK + k];
                 corner += kk;
+                whole += kk * (float)(nr - 1 - j);
                 const float cs = row16_sum(kk);
                 if (l16 == 0) parts[wave * 64 + j] -= cs;
             }
@@ -346,6 +353,10 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
         corner = lanes_sum<64>(corner);
         front = lanes_sum<64>(front);
         if (lane == 0) { corners[wave] = corner; corners[NW + wave] = front; }
+        if (p.gl == 0) {
+            whole = lanes_sum<64>(whole);
+            if (lane == 0) corners[2 * NW + wave] = whole;
+        }
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
             if (!has_v) break;
@@ -426,7 +437,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
     const auto rows32 = [](int half) { return half ? 32 * (P0 - P1) : 0; };                   // where row 0 would lie at that half's pitch
     constexpr int NB = TIGHT || (DK == 128 && DV == 128) ? 1 : 3;                                      // terms of a state in LDS at once
     constexpr int NI = 4 * KT / NW, NJ = 4 * VT / NW, TW = KT * VT / NW;                               // tiles of a wave: rows of dq / dk, rows of dv, D
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + 2 * NW) * 4];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + 3 * NW) * 4];
     unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + XY, *Yh = Xl + XY,
                   *Yl = Yh + XY, *St = Yl + XY;
     float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + NW * C;
@@ -520,15 +531,16 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
     };
     auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: gradients of b inside the chunk, summed from its end
         if (wave == 1) {
-            double x = 0.0, e = 0.0, first = 0.0;
+            double x = 0.0, e = 0.0, first = 0.0, all = 0.0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) { x += (double)parts[w * C + lane0]; e += (double)corners[w]; first += (double)corners[NW + w]; }
+            for (int w = 0; w < NW; ++w) { x += (double)parts[w * C + lane0]; e += (double)corners[w]; first += (double)corners[NW + w]; all += (double)corners[2 * NW + w]; }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_down(x, d, 64);
                 if (lane0 + d < 64) x += o;
             }
-            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)(lane0 ? x + e : first);
+            const double dg = p.gl == 0 ? (lane0 ? 0.0 : all) : lane0 ? x + e : first;
+            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)dg;
         }
     };
     auto put_terms = [&](const f4 (&x)[TW], int u0) {                // terms u0 ... u0 + NB - 1 of a state -> St, row dv, column k
@@ -572,6 +584,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
         put_terms(sr, 0);
         __syncthreads();
         parts[wave * C + lane0] = 0.0f;
+        float whole = 0.0f;                                          // every pair times the decays it crosses
         // X, Y and the sums of M below the diagonal: ten 16 x 16 tiles dealt to the waves
 #pragma unroll
         for (int tn = 0; tn < (10 + NW - 1) / NW; ++tn) {
@@ -601,6 +614,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
             *reinterpret_cast<bf16x4 *>(Yh + at) = yh;
             *reinterpret_cast<bf16x4 *>(Yl + at) = round4(rest4(y, yh));
             float rowsum = (m.x + m.y) + (m.z + m.w);
+            whole += (rowsum * (float)(i - j) - m.y) - (2.0f * m.z + 3.0f * m.w);
             rowsum += __shfl_xor(rowsum, 16, 64);
             rowsum += __shfl_xor(rowsum, 32, 64);
             const f4 cs = f4{row16_sum(m.x), row16_sum(m.y), row16_sum(m.z), row16_sum(m.w)};
@@ -642,6 +656,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
                 const f2 q0 = bf16pair_to_f2(w.x), q1 = bf16pair_to_f2(w.y);
                 float d = (acc[m].x * q0.x + acc[m].y * q0.y) + (acc[m].z * q1.x + acc[m].w * q1.y);
                 front += d;
+                whole += d * (float)(i + 1);
                 d += __shfl_xor(d, 16, 64);
                 d += __shfl_xor(d, 32, 64);
                 if (gq == 0) parts[wave * C + i] += d;
@@ -710,6 +725,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
             }
             corner *= eend;
             front += corner;
+            whole += corner * (float)nr;
 #pragma unroll
             for (int m = 0; m < NI; ++m) {
                 const int j = 16 * (i0 + m) + l16;
@@ -718,6 +734,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
                 const f2 k0 = bf16pair_to_f2(w.x), k1 = bf16pair_to_f2(w.y);
                 float d = (dk[m].x * k0.x + dk[m].y * k0.y) + (dk[m].z * k1.x + dk[m].w * k1.y);
                 corner += d;
+                whole += d * (float)(nr - 1 - j);
                 d += __shfl_xor(d, 16, 64);
                 d += __shfl_xor(d, 32, 64);
                 if (gq == 0) parts[wave * C + j] -= d;
@@ -725,6 +742,10 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
             corner = lanes_sum<64>(corner);
             front = lanes_sum<64>(front);
             if (lane == 0) { corners[wave] = corner; corners[NW + wave] = front; }
+            if (p.gl == 0) {
+                whole = lanes_sum<64>(whole);
+                if (lane == 0) corners[2 * NW + wave] = whole;
+            }
 #pragma unroll
             for (int m = 0; m < NJ; ++m) dv[m] *= wt[16 * (j0 + m) + l16];
 #pragma unroll

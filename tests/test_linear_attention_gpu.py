@@ -522,6 +522,12 @@ def test_expanded_and_single_row_views(dtype):
             out = linear_attention_fn(*leaves, initial_state=t["s0"])
             res.append([out, *torch.autograd.grad(out, leaves, t["do"])])
         assert all(torch.equal(a, b) for a, b in zip(*res))
+    still = t["g"][:, :1].expand(-1, 70, -1)                       # one decay for all tokens, but given (and differentiated) for each
+    res = []
+    for g in (still, still.contiguous()):
+        g = g.detach().requires_grad_()
+        res.append(torch.autograd.grad(linear_attention_fn(t["q"], t["k"], t["v"], g, initial_state=t["s0"]), g, t["do"])[0])
+    assert torch.equal(*res) and bool((res[0] != 0).all())
     one = {n: t[n][:, :1] for n in names}
     odd = {n: x.as_strided(x.shape, (x.stride(0), 1, *x.stride()[2:])) for n, x in one.items()}
     want = linear_attention_fn(*[one[n].contiguous() for n in names], initial_state=t["s0"])

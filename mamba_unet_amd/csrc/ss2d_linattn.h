@@ -344,10 +344,11 @@ inline int linattn_chunk(int dtype, int dk, int dv) { return dtype || (dk <= 64 
 
 // Segments.  One workgroup walks a segment; with fewer workgroups than the card holds at once it idles, and a segment costs a second pass over k and v (q
 // and dout in the backward) and a state's round trip.  So all tokens of all sequences and heads are dealt to as many workgroups as are resident
-// (forward: three a CU up to 64 x 64 in bf16, else two; backward: one up to 128 wide keys in bf16, else two shifts of one), at least two chunks each, in equal
-// parts of the longest sequence.  Measured, us, for half the workgroups / these / twice: 24 x 3136 tokens, 3 heads of 16 x 64 fp32, forward
-// and backward 322 / 194 / 215; 65536 tokens, 8 heads of 128 x 128 bf16, forward 283 / 252 / 270; not split 521 and 5383.  Short ones: a bf16 chunk takes
-// 3 us and the two further launches cost as much as two chunks: 256 tokens (4 chunks) 15 us in one walk, 19 split; 512 tokens 26 and 19.
+// (forward: three a CU up to 64 x 64 in bf16, else two; backward: one a CU with keys beyond 64 wide in bf16, else two), at least two chunks each, in equal
+// parts of the longest sequence.  Measured, us, for half the workgroups / these / twice / no split: 24 x 3136 tokens, 3 heads of 16 x 64 fp32, forward and
+// backward 271 / 180 / 190 / 574; 4 x 4096 tokens, 16 heads of 128 x 64 bf16, both ways 551 / 364 / 381 / 973; 65536 tokens, 8 heads of 128 x 128 bf16, forward
+// 283 / 250 / 263 / 5402.  Short ones, 4 heads of 64 x 64 bf16: a chunk takes 3 us and the two further launches as much as two chunks: 256 tokens (4 chunks) 16 us in
+// one walk, 19 split; 384 tokens (6) 22 and 19.
 // Returns the segments of the longest sequence in the upper and the chunks a segment in the lower 32 bits; 1 segment: no sequence is split.
 inline long long linattn_segments(int dtype, long long all_tokens, long long max_len, int H, int dk, int dv, int backward) {
     const int C = linattn_chunk(dtype, dk, dv);

@@ -15,9 +15,10 @@
 // A workgroup walks one segment of one sequence and value head from its end to its start with D in accumulator registers (a wave owns
 // 16-column slices of dv).  Segments as in the forward: own contributions, a join in order, the walk.
 //
-// Measured.  4 x 4096 tokens, 16 heads of 128 x 64 on 2 key heads, bf16: contributions 32 us, join 6, walk 195, sum over the heads of a group 47 (5.7 TB/s).  A
+// Measured.  4 x 4096 tokens, 16 heads of 128 x 64 on 2 key heads, bf16: contributions 33 us, join 6, walk 198, sum over the heads of a group 47 (5.7 TB/s).  A
 // chunk takes a workgroup of 16 waves, one a CU (157 KB of LDS), 24,000 cycles: the matrix units are busy 17% of them and LDS 42% (a quarter of that bank
-// conflicts of 8-byte writes), the rest waits between the phases, which need each other's results.  24 x 3136 tokens, 3 heads of 16 x 64 fp32: 15.6 + 4.8 + 96 us.
+// conflicts of 8-byte writes), the rest waits between the phases, which need each other's results.  24 x 3136 tokens, 3 heads of 16 x 64 fp32: 16 + 4.5 + 98 us (matrix
+// units 38%, LDS 29%).
 #include "ss2d_linattn.h"
 #include "../../include/ss2d.h"
 
@@ -94,7 +95,7 @@ __device__ void zero_rows(const Problem &p, IO *o, long long row, int w, int nw)
 constexpr int GAP_WGS = 16;
 
 // fp32: 16 waves a workgroup, so that every result of a chunk -- dq, dk (C x dk) and dv (C x dv) -- is at most one 16 x 16 tile a wave on
-// v_mfma_f32_16x16x4_f32; keys up to 16 wide: 8 waves with two tiles of dv, and two workgroups a CU (24 x 3136 tokens, 3 heads of 16 x 64: 96 us, one
+// v_mfma_f32_16x16x4_f32; keys up to 16 wide: 8 waves with two tiles of dv, and two workgroups a CU (24 x 3136 tokens, 3 heads of 16 x 64: 98 us, one
 // workgroup of 16 waves 120).  A lane holds row / column l16 of an operand and contracted indices 4 gq + r of a 16-block in step r: direct operands are
 // 16-byte LDS reads, transposed ones four 4-byte reads, both free of bank conflicts at a pitch of 4 mod 16 floats.  LDS holds the four tiles, X,
 // Y and one state at a time: S (for dq), then D (for dk, dv).  The next chunk is in flight in registers.

@@ -98,6 +98,12 @@ Tensor dense16(const Tensor &g, at::ScalarType io) {
     return g.to(io).clone(at::MemoryFormat::Contiguous);
 }
 
+// what hooks on saved tensors gave back in the place of a dense fp32 tensor of this shape
+Tensor as_saved(const char *op, const Tensor &t, at::IntArrayRef want) {
+    TORCH_CHECK_VALUE(t.sizes() == want, op, ": a saved tensor came back as ", shape(t.sizes()), ", not ", shape(want));
+    return cast(t, at::kFloat).contiguous();
+}
+
 // ------------------------------------------------------------------------------------------------ linear attention
 
 constexpr int64_t MAX_DIM = 128;
@@ -170,6 +176,10 @@ struct Segments {
 struct Attention {
     Tensor out, last, chunks;
 };
+int64_t chunk_slots(int code, const Dims &d, bool packed) {
+    const int64_t C = api.ss2d_linattn_chunk(code, (int)d.dk, (int)d.dv);
+    return packed ? d.L / C + d.N : d.N * ((d.L + C - 1) / C);
+}
 // operands as `operand` leaves them; s0 fp32 and dense
 Attention attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &s0, const Tensor &cu, double scale, const Dims &d,
                             int64_t longest, bool want_last, bool want_chunks) {
@@ -184,8 +194,7 @@ Attention attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, c
     }
     const int code = code_of(io), dk = (int)d.dk, dv = (int)d.dv;
     if (want_chunks) {
-        const int64_t C = api.ss2d_linattn_chunk(code, dk, dv), slots = cu.defined() ? d.L / C + d.N : d.N * ((d.L + C - 1) / C);
-        r.chunks = empty({slots, d.H, (int64_t)api.ss2d_linattn_state_floats(code, dk, dv)}, dev);
+        r.chunks = empty({chunk_slots(code, d, cu.defined()), d.H, (int64_t)api.ss2d_linattn_state_floats(code, dk, dv)}, dev);
     }
     const Segments seg(code, d, dev, longest, cu.defined(), false);
     const Strides st(q, k, v, g);
@@ -231,13 +240,23 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     }
     static void run(AutogradContext *ctx, const Tensor &dout, const Tensor &dlast, variable_list &res) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &g = saved[3], &cu = saved[4], &chunks = saved[5];
         const std::vector<int64_t> m = ctx->saved_data["meta"].toIntVector();
         const Dims d{m[0], m[1], m[2], m[3], m[4], m[5], m[6]};
         const auto type = [&](int i) { return (at::ScalarType)m[8 + i]; };
         const float scale = (float)ctx->saved_data["scale"].toDouble();
+        const at::ScalarType io = type(0) == at::kBFloat16 && type(1) == at::kBFloat16 && type(2) == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
+        // hooks on saved tensors (offloaded or packed activations) may hand them back in another layout: they are checked and laid out as in the forward
+        const Dims now = attention_dims(saved[0], saved[1], saved[2], saved[3], Tensor(), saved[4]);
+        TORCH_CHECK_VALUE(now.B == d.B && now.L == d.L && now.G == d.G && now.dk == d.dk && now.H == d.H && now.dv == d.dv && now.N == d.N,
+                          "linear_attention_fn: a saved tensor came back with another shape");
+        const Tensor q = operand(saved[0], io), k = operand(saved[1], io), v = operand(saved[2], io), g = decays(saved[3]), &cu = saved[4];
         const at::Device dev = q.device();
-        const at::ScalarType io = q.scalar_type();
+        Tensor chunks;
+        if (d.L > 0) {
+            const int code = code_of(io), dk = (int)d.dk, dv = (int)d.dv;
+            chunks = as_saved("linear_attention_fn", saved[5], {chunk_slots(code, d, cu.defined()), d.H, (int64_t)api.ss2d_linattn_state_floats(code, dk, dv)});
+            check_devices("linear_attention_fn", {{"q", &q}, {"states", &chunks}});
+        }
         const bool want_g = ctx->needs_input_grad(3), want_s0 = m[12] >= 0 && ctx->needs_input_grad(4);
         Tensor dq = empty({d.B, d.L, d.G, d.dk}, dev, io), dk = empty({d.B, d.L, d.G, d.dk}, dev, io), dv = empty({d.B, d.L, d.H, d.dv}, dev, io);
         Tensor dg = empty({d.B, d.L, d.H}, dev), ds0;
@@ -359,7 +378,7 @@ struct Rows {
         else t = t.contiguous();
     }
 };
-at::ScalarType store_type(const Tensor &t) { return t.scalar_type() == at::kBFloat16 ? at::kBFloat16 : at::kFloat; }
+at::ScalarType store_type(at::ScalarType t) { return t == at::kBFloat16 ? at::kBFloat16 : at::kFloat; }
 Tensor fp32_param(const Tensor &t) { return t.defined() && (t.scalar_type() != at::kFloat || !t.is_contiguous()) ? t.detach().to(at::kFloat).contiguous() : t; }
 
 struct Norms {
@@ -371,7 +390,7 @@ Norms norms_forward(const Tensor &x, const Tensor &y, const Tensor &z, const Ten
     Norms r;
     r.D = x.size(-1);
     r.rows = x.numel() / r.D;
-    const at::ScalarType rt = store_type(x), io = store_type(y);
+    const at::ScalarType rt = store_type(x.scalar_type()), io = store_type(y.scalar_type());
     const Rows rx(x, rt, r.D), ry(y, io, r.D), rz(z, io, r.D);
     r.x = rx.t; r.y = ry.t; r.z = rz.t; r.ldx = rx.ld; r.ldy = ry.ld; r.ldz = rz.ld;
     r.w1 = fp32_param(w1); r.b1 = fp32_param(b1); r.a = fp32_param(a); r.w2 = fp32_param(w2); r.b2 = fp32_param(b2); r.drop = fp32_param(drop);
@@ -395,7 +414,7 @@ struct NormGateResidual : torch::autograd::Function<NormGateResidual> {
         const Norms r = norms_forward(x, y, get(z), w1, get(b1), get(a), w2, get(b2), get(drop), eps, rms, true);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({r.x, r.y, r.z, r.w1, r.b1, r.a, r.w2, r.drop, r.stats});
-        std::vector<int64_t> m{r.D, r.rows, r.ldx, r.ldy, r.ldz, r.rps, rms};
+        std::vector<int64_t> m{r.D, r.rows, r.rps, rms};
         for (const Maybe &t : {Maybe(x), Maybe(y), z, Maybe(w1), b1, a, Maybe(w2), b2}) m.push_back(t ? (int64_t)t->scalar_type() : -1);
         for (const int64_t n : x.sizes()) m.push_back(n);
         ctx->saved_data["meta"] = std::move(m);
@@ -412,10 +431,25 @@ struct NormGateResidual : torch::autograd::Function<NormGateResidual> {
     }
     static void run(AutogradContext *ctx, const Tensor &dxo, const Tensor &dh, variable_list &res) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &y = saved[1], &z = saved[2], &w1 = saved[3], &b1 = saved[4], &a = saved[5], &w2 = saved[6], &drop = saved[7], &stats = saved[8];
         const std::vector<int64_t> m = ctx->saved_data["meta"].toIntVector();
         const int64_t D = m[0], rows = m[1];
-        const at::IntArrayRef sizes(m.data() + 15, m.size() - 15);
+        const at::IntArrayRef sizes(m.data() + 12, m.size() - 12);
+        const auto type = [&](int i) { return (at::ScalarType)m[4 + i]; };
+        // hooks on saved tensors (offloaded or packed activations) may hand them back in another layout: rows are found anew
+        const char *op = "norm_gate_residual";
+        check_devices(op, {{"x", &saved[0]}, {"y", &saved[1]}, {"z", &saved[2]}, {"post_weight", &saved[3]}, {"post_bias", &saved[4]}, {"res_scale", &saved[5]},
+                           {"pre_weight", &saved[6]}, {"drop_scale", &saved[7]}, {"statistics", &saved[8]}});
+        const auto rows_of = [&](int i) {
+            const Tensor &t = saved[i];
+            TORCH_CHECK_VALUE(!t.defined() || t.sizes() == sizes, op, ": a saved tensor came back with another shape");
+            return Rows(t, store_type(type(i)), D);
+        };
+        const auto dense = [&](int i, at::IntArrayRef want) { return saved[i].defined() ? as_saved(op, saved[i], want) : saved[i]; };
+        const Rows rx = rows_of(0), ry = rows_of(1), rz = rows_of(2);
+        const Tensor &x = rx.t, &y = ry.t, &z = rz.t;
+        const Tensor w1 = dense(3, {D}), b1 = dense(4, {D}), a = dense(5, {D}), w2 = dense(6, {D}), stats = dense(8, {rows, 4});
+        const Tensor drop = saved[7].defined() ? as_saved(op, saved[7], saved[7].sizes()) : saved[7];
+        TORCH_CHECK_VALUE(!drop.defined() || drop.numel() * m[2] == rows, op, ": a saved tensor came back with another shape");
         const at::Device dev = x.device();
         const Tensor gx = dense16(dxo, x.scalar_type()), gh = dense16(dh, y.scalar_type());
         Tensor dx = empty(sizes, dev, x.scalar_type()), dy = empty(sizes, dev, y.scalar_type()), dz, dp;
@@ -425,18 +459,18 @@ struct NormGateResidual : torch::autograd::Function<NormGateResidual> {
             const Tensor ws = empty({(int64_t)api.ss2d_block_norm_bwd_workspace_floats(rows, (int)D)}, dev);
             const Here here(dev);
             check_rc(api.ss2d_block_norm_bwd(code_of(x.scalar_type()), code_of(y.scalar_type()), ptr(gx), ptr(gh), ptr(x), ptr(y), ptr(z), ptr<float>(w1), ptr<float>(b1),
-                                             ptr<float>(w2), ptr<float>(a), ptr<float>(drop), m[5], ptr<float>(stats), ptr(dx), ptr(dy), ptr(dz), ptr<float>(dp),
-                                             ptr<float>(ws), rows, (int)D, m[2], m[3], m[4], (int)m[6], here.stream),
+                                             ptr<float>(w2), ptr<float>(a), ptr<float>(drop), m[2], ptr<float>(stats), ptr(dx), ptr(dy), ptr(dz), ptr<float>(dp),
+                                             ptr<float>(ws), rows, (int)D, rx.ld, ry.ld, rz.ld, (int)m[3], here.stream),
                      "ss2d_block_norm_bwd");
         } else {
             dp = at::zeros({5, D}, w1.options());
         }
         size_t edge = 0;                               // counts the tensors that are there
         for (int i = 0; i < 8; ++i) {
-            if (m[7 + i] < 0) continue;
+            if (m[4 + i] < 0) continue;
             if (!ctx->needs_input_grad(edge++)) continue;
             const Tensor t = i == 0 ? dx : i == 1 ? dy : i == 2 ? dz : dp.select(0, i - 3);
-            res[i] = cast(t, (at::ScalarType)m[7 + i]);
+            res[i] = cast(t, type(i));
         }
     }
 };

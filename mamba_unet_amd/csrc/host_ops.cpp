@@ -69,8 +69,13 @@ struct Named {
     const char *name;
     const Tensor *t;
 };
-// the first tensor that is not on the GPU, or on another one than the first, raises
-void check_devices(const char *op, std::initializer_list<Named> all) {
+// Forward-mode derivatives: the kernels carry no tangents, and leaving them out would make a function's derivative wrong without a word.
+void check_no_tangent(const char *op, const Tensor &t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), op, ": forward-mode derivatives are not implemented (a tensor with a tangent was given)");
+}
+// a tensor with a tangent raises, and the first one that is not on the GPU, or on another one than the first
+void check_tensors(const char *op, std::initializer_list<Named> all) {
+    for (const Named &n : all) check_no_tangent(op, *n.t);
     const Named *first = nullptr;
     for (const Named &n : all) {
         if (!n.t->defined()) continue;
@@ -127,7 +132,7 @@ Tensor operand(const Tensor &t0, at::ScalarType io) {
 }
 
 Dims attention_dims(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &s0, const Tensor &cu) {
-    check_devices("linear_attention_fn", {{"q", &q}, {"k", &k}, {"v", &v}, {"log_decay", &g}, {"initial_state", &s0}, {"cu_seqlens", &cu}});
+    check_tensors("linear_attention_fn", {{"q", &q}, {"k", &k}, {"v", &v}, {"log_decay", &g}, {"initial_state", &s0}, {"cu_seqlens", &cu}});
     TORCH_CHECK_VALUE(q.is_floating_point() && k.is_floating_point() && v.is_floating_point() && g.is_floating_point() && (!s0.defined() || s0.is_floating_point()),
                       "linear_attention_fn: q, k, v, log_decay and initial_state must be floating-point tensors");
     TORCH_CHECK_VALUE(q.dim() == 4 && k.sizes() == q.sizes() && v.dim() == 4 && v.size(0) == q.size(0) && v.size(1) == q.size(1),
@@ -230,6 +235,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         const Tensor dout = grads[0], dlast = grads.size() > 1 ? grads[1] : Tensor();
+        for (const Tensor &t : grads) check_no_tangent("linear_attention_fn", t);
         variable_list res(9);
         if (!dout.defined() && !dlast.defined()) return res;
         {
@@ -255,7 +261,7 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         if (d.L > 0) {
             const int code = code_of(io), dk = (int)d.dk, dv = (int)d.dv;
             chunks = as_saved("linear_attention_fn", saved[5], {chunk_slots(code, d, cu.defined()), d.H, (int64_t)api.ss2d_linattn_state_floats(code, dk, dv)});
-            check_devices("linear_attention_fn", {{"q", &q}, {"states", &chunks}});
+            check_tensors("linear_attention_fn", {{"q", &q}, {"states", &chunks}});
         }
         const bool want_g = ctx->needs_input_grad(3), want_s0 = m[12] >= 0 && ctx->needs_input_grad(4);
         Tensor dq = empty({d.B, d.L, d.G, d.dk}, dev, io), dk = empty({d.B, d.L, d.G, d.dk}, dev, io), dv = empty({d.B, d.L, d.H, d.dv}, dev, io);
@@ -320,7 +326,7 @@ Tensor token(const Tensor &t0, at::ScalarType io) {
 
 Tensor attention_step(const Tensor &state, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, std::optional<double> scale, const Maybe &indices) {
     const Tensor idx = get(indices);
-    check_devices("linear_attention_step", {{"state", &state}, {"q", &q}, {"k", &k}, {"v", &v}, {"log_decay", &g}, {"state_indices", &idx}});
+    check_tensors("linear_attention_step", {{"state", &state}, {"q", &q}, {"k", &k}, {"v", &v}, {"log_decay", &g}, {"state_indices", &idx}});
     TORCH_CHECK(!at::GradMode::is_enabled() || !any_requires_grad({{"", &state}, {"", &q}, {"", &k}, {"", &v}, {"", &g}}),
                 "linear_attention_step updates its state in place and has no gradient: call it under torch.no_grad(), or linear_attention_fn");
     TORCH_CHECK_VALUE(q.is_floating_point() && k.is_floating_point() && v.is_floating_point() && g.is_floating_point(),
@@ -422,6 +428,7 @@ struct NormGateResidual : torch::autograd::Function<NormGateResidual> {
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         variable_list res(11);
+        for (const Tensor &t : grads) check_no_tangent("norm_gate_residual", t);
         if (!grads[0].defined() && !grads[1].defined()) return res;
         {
             const at::NoGradGuard no_grad;
@@ -437,7 +444,7 @@ struct NormGateResidual : torch::autograd::Function<NormGateResidual> {
         const auto type = [&](int i) { return (at::ScalarType)m[4 + i]; };
         // hooks on saved tensors (offloaded or packed activations) may hand them back in another layout: rows are found anew
         const char *op = "norm_gate_residual";
-        check_devices(op, {{"x", &saved[0]}, {"y", &saved[1]}, {"z", &saved[2]}, {"post_weight", &saved[3]}, {"post_bias", &saved[4]}, {"res_scale", &saved[5]},
+        check_tensors(op, {{"x", &saved[0]}, {"y", &saved[1]}, {"z", &saved[2]}, {"post_weight", &saved[3]}, {"post_bias", &saved[4]}, {"res_scale", &saved[5]},
                            {"pre_weight", &saved[6]}, {"drop_scale", &saved[7]}, {"statistics", &saved[8]}});
         const auto rows_of = [&](int i) {
             const Tensor &t = saved[i];
@@ -478,7 +485,7 @@ struct NormGateResidual : torch::autograd::Function<NormGateResidual> {
 std::tuple<Tensor, Tensor> norm_gate_residual(const Tensor &x, const Tensor &y, const Tensor &w1, const Tensor &w2, const Maybe &b1, const Maybe &b2, const Maybe &z,
                                               const Maybe &a, const Maybe &drop, double eps, bool rms) {
     const Tensor tb1 = get(b1), tb2 = get(b2), tz = get(z), ta = get(a), td = get(drop);
-    check_devices("norm_gate_residual", {{"x", &x}, {"y", &y}, {"post_weight", &w1}, {"pre_weight", &w2}, {"z", &tz}, {"post_bias", &tb1}, {"pre_bias", &tb2},
+    check_tensors("norm_gate_residual", {{"x", &x}, {"y", &y}, {"post_weight", &w1}, {"pre_weight", &w2}, {"z", &tz}, {"post_bias", &tb1}, {"pre_bias", &tb2},
                                          {"res_scale", &ta}, {"drop_scale", &td}});
     TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) >= 1 && x.size(-1) <= 8192, "norm_gate_residual: the last axis must hold 1 ... 8192 channels, got ", shape(x.sizes()));
     const auto same = [&](const char *name, const Tensor &t, at::IntArrayRef want) {
@@ -526,6 +533,7 @@ Tensor clip_grad_norm(const py::object &given, double max_norm, double norm_type
     std::vector<std::pair<size_t, Tensor>> copies;     // of what is not dense in any order of its axes
     for (size_t i = 0; i < n; ++i) {
         const Tensor &g = grads[i];
+        check_no_tangent("clip_grad_norm", g);
         TORCH_CHECK(g.is_cuda(), "clip_grad_norm: GPU tensors required (no CPU path in mamba_unet_amd)");
         TORCH_CHECK_VALUE(g.device() == dev, "clip_grad_norm: gradients on several devices: ", dev, ", ", g.device());
         TORCH_CHECK_VALUE(g.layout() == at::kStrided && (g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16),

@@ -6,11 +6,12 @@
 //   dv_j = sum_i X_ij do_i + exp(b_C - b_j) D^T k_j        D_prev = exp(b_C) D + sum_i scale exp(b_i) q_i do_i^T
 // A decay g_t scales every path that crosses it, so its gradient is the sum over the pairs on both sides of it,
 //   dg_t = sum_{i >= t > j} M_ij,  M_ij = w_ij (q_i . k_j)(do_i . v_j),
-// with the state in front of the chunk as one more column, D as one more row.  It is taken as row sums minus column sums, added
-// up from the chunk's end; pairs that do not cross t cancel there, but only pairs of ONE chunk, and the diagonal, whose terms
-// are the largest and cross nothing, never enters.  The chunk's first decay is crossed by the pairs with the state alone: their sum, exactly 0 at a
-// start without a state.  One decay for all tokens of a head (token stride 0) has the sum over t for its gradient: every pair times the number of decays that it
-// crosses, without differences; a chunk's part is left at its first token.
+// with the state in front of the chunk as one more column, D as one more row.  Only pairs that cross t are added, none is taken off again: behind a
+// strong decay exp(g_t) all of them are small, and the others, a factor exp(-g_t) larger, would leave their rounding (as row sums minus column sums in fp32 the
+// gradient of a decay of log(1e-6) between chunks of ordinary ones was off by its own size).  For a 16 x 16 tile of M the tokens of its rows take sums of its rows
+// from the end, the tokens of its columns sums of its columns from the start, the tokens between them its total; a tile on the diagonal a scan in both
+// directions; the pairs with S (q . S do) count as rows, those with D (k . D v) as columns, <D, S> for every token.  One decay for all tokens of a head (token
+// stride 0) has the sum over t for its gradient; a chunk's part is left at its first token.
 //
 // A workgroup walks one segment of one sequence and value head from its end to its start with D in accumulator registers (a wave owns
 // 16-column slices of dv).  Segments as in the forward: own contributions, a join in order, the walk.
@@ -46,6 +47,62 @@ __device__ __forceinline__ float row16_sum(float v) {
     v += dpp_mov<DPP_ROW_ROR(2), 0xf, false>(0.0f, v);
     v += dpp_mov<DPP_ROW_ROR(1), 0xf, false>(0.0f, v);
     return v;
+}
+
+// ---- the gradients of the decays: a lane is a token of the chunk (lane = 16 gq + l16, tile gq) and adds the pairs that cross it
+// sums over the 16 lanes of a DPP row from its end, from its start; lane N of the row in every lane of it
+__device__ __forceinline__ float row16_from_end(float v) {
+    v += dpp_mov<DPP_ROW_SHL(1), 0xf, true>(0.0f, v);
+    v += dpp_mov<DPP_ROW_SHL(2), 0xf, true>(0.0f, v);
+    v += dpp_mov<DPP_ROW_SHL(4), 0xf, true>(0.0f, v);
+    return v + dpp_mov<DPP_ROW_SHL(8), 0xf, true>(0.0f, v);
+}
+__device__ __forceinline__ float row16_from_start(float v) {
+    v += dpp_mov<DPP_ROW_SHR(1), 0xf, true>(0.0f, v);
+    v += dpp_mov<DPP_ROW_SHR(2), 0xf, true>(0.0f, v);
+    v += dpp_mov<DPP_ROW_SHR(4), 0xf, true>(0.0f, v);
+    return v + dpp_mov<DPP_ROW_SHR(8), 0xf, true>(0.0f, v);
+}
+__device__ __forceinline__ float row16_shift(float v) { return dpp_mov<DPP_ROW_SHR(1), 0xf, true>(0.0f, v); }      // of the lane before, 0 in the first
+template <int N>
+__device__ __forceinline__ float row16_lane(float v) { return dpp_mov<0x150 + N, 0xf, false>(0.0f, v); }
+__device__ __forceinline__ float rows_sum(float v) {                 // over the four rows of 16 lanes
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+// Four values a lane, of indices 4 gq + r, alike in all l16: sums in every row from index l16 on, up to and with it, in front of it
+__device__ __forceinline__ float four_from(const f4 &v, int l16, int gq) {
+    float s = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s += 4 * gq + r >= l16 ? v[r] : 0.0f;
+    return rows_sum(s);
+}
+__device__ __forceinline__ float four_up_to(const f4 &v, int l16, int gq) {
+    float s = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s += 4 * gq + r <= l16 ? v[r] : 0.0f;
+    return rows_sum(s);
+}
+__device__ __forceinline__ float four_before(const f4 &v, int l16, int gq) {
+    float s = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s += 4 * gq + r < l16 ? v[r] : 0.0f;
+    return rows_sum(s);
+}
+// of a tile's row sums from the end (rows): the tokens of the tile take theirs, those of earlier tiles the whole
+__device__ __forceinline__ float cross_rows(float from_end, int tile, int gq) {
+    const float all = row16_lane<0>(from_end);
+    return gq < tile ? all : gq == tile ? from_end : 0.0f;
+}
+// of a tile's column sums from the start: the tokens of the tile take the columns before them, those of later tiles the whole
+__device__ __forceinline__ float cross_columns(float from_start, int tile, int gq) {
+    const float all = row16_lane<15>(from_start), before = row16_shift(from_start);
+    return gq > tile ? all : gq == tile ? before : 0.0f;
+}
+// of a tile below the diagonal: row sums from the end for its rows' tokens, columns before them for its columns' tokens, the total between
+__device__ __forceinline__ float cross_tile(float rows_from_end, float columns_before, int it, int jt, int gq) {
+    const float all = row16_lane<0>(rows_from_end);
+    return gq == it ? rows_from_end : gq == jt ? columns_before : gq > jt && gq < it ? all : 0.0f;
 }
 
 // seg_states[slot] = D behind the segment; one thread W elements
@@ -106,7 +163,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
     constexpr int XY = CT * (CT + 1) / 2 * 16 * PP;                  // X, Y: their tiles up to the diagonal
     constexpr int NV = (VT * CT + NW - 1) / NW;                      // tiles of dv a wave owns
     static_assert(KT * CT <= NW && NV <= 2, "tiles of a wave");
-    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * XY + 10 * 64 + NW * 64 + 3 * NW];
+    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * XY + 10 * 64 + NW * 64 + NW];
     float *Qs = lds, *Ks = Qs + C * PK, *Vs = Ks + C * PK, *Os = Vs + C * PV, *St = Os + C * PV, *Xs = St + DK * PV, *Ys = Xs + XY;
     float *decays = Ys + XY, *parts = decays + 10 * 64, *corners = parts + NW * 64;
     const auto tile_at = [](int it, int jt) { return (it * (it + 1) / 2 + jt) * 16 * PP; };
@@ -203,18 +260,18 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
             if (lane0 == 63) d[256] = hw_exp2((float)bend);
         }
     };
-    auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: gradients of b inside the chunk, summed from its end
+    auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: the waves' parts of its decays' gradients
         if (wave == 1) {
-            double x = 0.0, e = 0.0, first = 0.0, all = 0.0;
+            double x = 0.0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) { x += (double)parts[w * 64 + lane0]; e += (double)corners[w]; first += (double)corners[NW + w]; all += (double)corners[2 * NW + w]; }
+            for (int w = 0; w < NW; ++w) x += (double)parts[w * 64 + lane0] + (double)corners[w];
+            if (p.gl == 0) {                                         // one decay for all tokens
+                if (lane0 >= rows_of(c)) x = 0.0;
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double o = __shfl_down(x, d, 64);
-                if (lane0 + d < 64) x += o;
+                for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
+                if (lane0) x = 0.0;
             }
-            const double dg = p.gl == 0 ? (lane0 ? 0.0 : all) : lane0 ? x + e : first;
-            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)dg;
+            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)x;
         }
     };
     auto put_state = [&](const f4 (&x)[TW]) {
@@ -255,8 +312,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
         if (c > c0) fetch(c - 1);
         __syncthreads();
         const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
-        float whole = 0.0f;                                          // every pair times the decays it crosses
-        parts[wave * 64 + lane] = 0.0f;
+        float cross = 0.0f;                                          // what this wave's pairs add to the decay of token `lane`
         // X, Y and the sums of M below the diagonal
 #pragma unroll 1
         for (int t = wave; t < CT * (CT + 1) / 2; t += NW) {
@@ -271,39 +327,39 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
             const int j = 16 * jt + l16;
             const float hj = bh[j], lj = bl[j];
             const f4 hi = *reinterpret_cast<const f4 *>(bh + 16 * it + 4 * gq), li = *reinterpret_cast<const f4 *>(bl + 16 * it + 4 * gq);
-            float colsum = 0.0f;
+            f4 m;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * it + 4 * gq + r;
                 const float w = p.scale * hw_exp2((hi[r] - hj) + (li[r] - lj));
-                const float yw = j <= i ? y[r] * w : 0.0f, m = j < i ? x[r] * yw : 0.0f;
+                const float yw = j <= i ? y[r] * w : 0.0f;
                 Xs[16 * PP * t + (4 * gq + r) * PP + l16] = j <= i ? x[r] * w : 0.0f;
                 Ys[16 * PP * t + (4 * gq + r) * PP + l16] = yw;
-                colsum += m;
-                whole += m * (float)(i - j);
-                const float rs = row16_sum(m);
-                if (l16 == 0) parts[wave * 64 + i] += rs;
+                m[r] = j < i ? x[r] * yw : 0.0f;
             }
-            colsum += __shfl_xor(colsum, 16, 64);
-            colsum += __shfl_xor(colsum, 32, 64);
-            if (gq == 0) parts[wave * 64 + j] -= colsum;
+            if (it == jt) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m[r] = row16_shift(row16_from_start(m[r]));      // of row i, the columns in front of token l16
+                const float d = four_from(m, l16, gq);
+                cross += gq == it ? d : 0.0f;
+            } else {
+                const float columns = row16_shift(row16_from_start(rows_sum((m.x + m.y) + (m.z + m.w))));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m[r] = row16_sum(m[r]);
+                cross += cross_tile(four_from(m, l16, gq), columns, it, jt, gq);
+            }
         }
         const int k = 16 * qk + l16;
         f4 dq = f4{0, 0, 0, 0};
-        float front = 0.0f;                                          // pairs with the state in front of the chunk: all that crosses its first decay
         if (has_q) {
 #pragma unroll
             for (int v = 0; v < VT; ++v)
                 dq = dot4(*reinterpret_cast<const f4 *>(Os + (16 * qi + l16) * PV + 16 * v + 4 * gq), *reinterpret_cast<const f4 *>(St + k * PV + 16 * v + 4 * gq), dq);
             dq *= *reinterpret_cast<const f4 *>(eb + 16 * qi + 4 * gq);
+            f4 d;                                                    // pairs with the state in front of the chunk
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * qi + 4 * gq + r;
-                const float qs = dq[r] * Qs[i * PK + k], rs = row16_sum(qs);
-                front += qs;
-                whole += qs * (float)(i + 1);
-                if (l16 == 0) parts[wave * 64 + i] += rs;
-            }
+            for (int r = 0; r < 4; ++r) d[r] = row16_sum(dq[r] * Qs[(16 * qi + 4 * gq + r) * PK + k]);
+            cross += cross_rows(four_from(d, l16, gq), qi, gq);
         }
         __syncthreads();                                              // X, Y are there; S is done with
         put_state(D);
@@ -320,24 +376,16 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
         }
         __syncthreads();                                              // D is there
         const float eend = tail[0];
-        corner *= eend;
-        front += corner;
-        whole += corner * (float)nr;
         if (has_q) {
             f4 dk = f4{0, 0, 0, 0};
 #pragma unroll
             for (int v = 0; v < VT; ++v)
                 dk = dot4(*reinterpret_cast<const f4 *>(Vs + (16 * qi + l16) * PV + 16 * v + 4 * gq), *reinterpret_cast<const f4 *>(St + k * PV + 16 * v + 4 * gq), dk);
             dk *= *reinterpret_cast<const f4 *>(wt + 16 * qi + 4 * gq);
+            f4 d;                                                    // pairs with D
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = 16 * qi + 4 * gq + r;
-                const float kk = dk[r] * Ks[j * PK + k];
-                corner += kk;
-                whole += kk * (float)(nr - 1 - j);
-                const float cs = row16_sum(kk);
-                if (l16 == 0) parts[wave * 64 + j] -= cs;
-            }
+            for (int r = 0; r < 4; ++r) d[r] = row16_sum(dk[r] * Ks[(16 * qi + 4 * gq + r) * PK + k]);
+            cross += cross_columns(four_up_to(d, l16, gq), qi, gq);
             for (int it = qi; it < CT; ++it) {
                 f4 x, y;
 #pragma unroll
@@ -351,13 +399,9 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) out.put1(dk[r], 16 * qi + 4 * gq + r, k, ldq, p.dk);
         }
-        corner = lanes_sum<64>(corner);
-        front = lanes_sum<64>(front);
-        if (lane == 0) { corners[wave] = corner; corners[NW + wave] = front; }
-        if (p.gl == 0) {
-            whole = lanes_sum<64>(whole);
-            if (lane == 0) corners[2 * NW + wave] = whole;
-        }
+        parts[wave * 64 + lane] = cross;
+        corner = lanes_sum<64>(corner * eend);
+        if (lane == 0) corners[wave] = corner;
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
             if (!has_v) break;
@@ -438,7 +482,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
     const auto rows32 = [](int half) { return half ? 32 * (P0 - P1) : 0; };                   // where row 0 would lie at that half's pitch
     constexpr int NB = TIGHT || (DK == 128 && DV == 128) ? 1 : 3;                                      // terms of a state in LDS at once
     constexpr int NI = 4 * KT / NW, NJ = 4 * VT / NW, TW = KT * VT / NW;                               // tiles of a wave: rows of dq / dk, rows of dv, D
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + 3 * NW) * 4];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + NW) * 4];
     unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + XY, *Yh = Xl + XY,
                   *Yl = Yh + XY, *St = Yl + XY;
     float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + NW * C;
@@ -530,18 +574,18 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
             if (lane0 == 63) d[4 * C] = hw_exp2((float)bend);
         }
     };
-    auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: gradients of b inside the chunk, summed from its end
+    auto finish_dg = [&](int c) {                                    // behind a barrier after chunk c: the waves' parts of its decays' gradients
         if (wave == 1) {
-            double x = 0.0, e = 0.0, first = 0.0, all = 0.0;
+            double x = 0.0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) { x += (double)parts[w * C + lane0]; e += (double)corners[w]; first += (double)corners[NW + w]; all += (double)corners[2 * NW + w]; }
+            for (int w = 0; w < NW; ++w) x += (double)parts[w * C + lane0] + (double)corners[w];
+            if (p.gl == 0) {                                         // one decay for all tokens
+                if (lane0 >= rows_of(c)) x = 0.0;
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double o = __shfl_down(x, d, 64);
-                if (lane0 + d < 64) x += o;
+                for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
+                if (lane0) x = 0.0;
             }
-            const double dg = p.gl == 0 ? (lane0 ? 0.0 : all) : lane0 ? x + e : first;
-            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)dg;
+            if (lane0 < rows_of(c)) DG[((long long)c * C + lane0) * p.H] = (float)x;
         }
     };
     auto put_terms = [&](const f4 (&x)[TW], int u0) {                // terms u0 ... u0 + NB - 1 of a state -> St, row dv, column k
@@ -584,8 +628,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
         for (int t = 0; t < TW; ++t) corner += (sr[t].x * D[t].x + sr[t].y * D[t].y) + (sr[t].z * D[t].z + sr[t].w * D[t].w);
         put_terms(sr, 0);
         __syncthreads();
-        parts[wave * C + lane0] = 0.0f;
-        float whole = 0.0f;                                          // every pair times the decays it crosses
+        float cross = 0.0f;                                          // what this wave's pairs add to the decay of token `lane`
         // X, Y and the sums of M below the diagonal: ten 16 x 16 tiles dealt to the waves
 #pragma unroll
         for (int tn = 0; tn < (10 + NW - 1) / NW; ++tn) {
@@ -614,15 +657,18 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
             *reinterpret_cast<bf16x4 *>(Xl + at) = round4(rest4(x, xh));
             *reinterpret_cast<bf16x4 *>(Yh + at) = yh;
             *reinterpret_cast<bf16x4 *>(Yl + at) = round4(rest4(y, yh));
-            float rowsum = (m.x + m.y) + (m.z + m.w);
-            whole += (rowsum * (float)(i - j) - m.y) - (2.0f * m.z + 3.0f * m.w);
-            rowsum += __shfl_xor(rowsum, 16, 64);
-            rowsum += __shfl_xor(rowsum, 32, 64);
-            const f4 cs = f4{row16_sum(m.x), row16_sum(m.y), row16_sum(m.z), row16_sum(m.w)};
-            if (l16 == 0) *reinterpret_cast<f4 *>(parts + wave * C + j) -= cs;
-            if (gq == 0) parts[wave * C + i] += rowsum;
+            if (it == jt) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m[r] = row16_from_end(m[r]);        // of column j, the rows from token l16 on
+                const float d = four_before(m, l16, gq);
+                cross += gq == it ? d : 0.0f;
+            } else {
+                const float rows = row16_from_end(rows_sum((m.x + m.y) + (m.z + m.w)));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m[r] = row16_sum(m[r]);
+                cross += cross_tile(rows, four_before(m, l16, gq), it, jt, gq);
+            }
         }
-        float front = 0.0f;                                          // pairs with the state in front of the chunk: all that crosses its first decay
         {   // dq
             const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
             f4 acc[NI];
@@ -655,12 +701,8 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
                 acc[m] *= eb[i];
                 const u32x2 w = *reinterpret_cast<const u32x2 *>(Qs + i * QP + 2 * k);
                 const f2 q0 = bf16pair_to_f2(w.x), q1 = bf16pair_to_f2(w.y);
-                float d = (acc[m].x * q0.x + acc[m].y * q0.y) + (acc[m].z * q1.x + acc[m].w * q1.y);
-                front += d;
-                whole += d * (float)(i + 1);
-                d += __shfl_xor(d, 16, 64);
-                d += __shfl_xor(d, 32, 64);
-                if (gq == 0) parts[wave * C + i] += d;
+                const float d = rows_sum((acc[m].x * q0.x + acc[m].y * q0.y) + (acc[m].z * q1.x + acc[m].w * q1.y));
+                cross += cross_rows(row16_from_end(d), i0 + m, gq);                  // pairs with the state in front of the chunk
             }
             __syncthreads();                                          // X, Y are there; S is done with
             put_terms(D, 0);
@@ -724,29 +766,18 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
                     }
                 }
             }
-            corner *= eend;
-            front += corner;
-            whole += corner * (float)nr;
 #pragma unroll
             for (int m = 0; m < NI; ++m) {
                 const int j = 16 * (i0 + m) + l16;
                 dk[m] *= wt[j];
                 const u32x2 w = *reinterpret_cast<const u32x2 *>(Ks + j * QP + 2 * (16 * kt + 4 * gq));
                 const f2 k0 = bf16pair_to_f2(w.x), k1 = bf16pair_to_f2(w.y);
-                float d = (dk[m].x * k0.x + dk[m].y * k0.y) + (dk[m].z * k1.x + dk[m].w * k1.y);
-                corner += d;
-                whole += d * (float)(nr - 1 - j);
-                d += __shfl_xor(d, 16, 64);
-                d += __shfl_xor(d, 32, 64);
-                if (gq == 0) parts[wave * C + j] -= d;
+                const float d = rows_sum((dk[m].x * k0.x + dk[m].y * k0.y) + (dk[m].z * k1.x + dk[m].w * k1.y));
+                cross += cross_columns(row16_from_start(d), i0 + m, gq);             // pairs with D
             }
-            corner = lanes_sum<64>(corner);
-            front = lanes_sum<64>(front);
-            if (lane == 0) { corners[wave] = corner; corners[NW + wave] = front; }
-            if (p.gl == 0) {
-                whole = lanes_sum<64>(whole);
-                if (lane == 0) corners[2 * NW + wave] = whole;
-            }
+            parts[wave * C + lane] = cross;
+            corner = lanes_sum<64>(corner * eend);
+            if (lane == 0) corners[wave] = corner;
 #pragma unroll
             for (int m = 0; m < NJ; ++m) dv[m] *= wt[16 * (j0 + m) + l16];
 #pragma unroll

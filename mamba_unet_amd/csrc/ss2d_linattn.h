@@ -139,6 +139,19 @@ __device__ __forceinline__ void widen8(bf16x8 v, f4 &a, f4 &b) {
     a = f4{__builtin_bit_cast(float, w0 << 16), __builtin_bit_cast(float, w0 & 0xffff0000u), __builtin_bit_cast(float, w1 << 16), __builtin_bit_cast(float, w1 & 0xffff0000u)};
     b = f4{__builtin_bit_cast(float, w2 << 16), __builtin_bit_cast(float, w2 & 0xffff0000u), __builtin_bit_cast(float, w3 << 16), __builtin_bit_cast(float, w3 & 0xffff0000u)};
 }
+// NaN and infinities -> 0; whether there were any
+__device__ __forceinline__ bool finite_only(bf16x8 &v) {
+    u32x4 w = __builtin_bit_cast(u32x4, v);
+    unsigned any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned m = ((w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;       // the halves that are not finite
+        any |= m;
+        w[i] &= ~(m | (m - (m >> 15)));
+    }
+    v = __builtin_bit_cast(bf16x8, w);
+    return any;
+}
 // eight fp32 values -> NT bf16 operands that add up to them
 template <int N>
 __device__ __forceinline__ void split8(f4 a, f4 b, bf16x8 (&o)[N]) {

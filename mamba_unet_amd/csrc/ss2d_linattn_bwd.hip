@@ -105,6 +105,32 @@ __device__ __forceinline__ float cross_tile(float rows_from_end, float columns_b
     return gq == it ? rows_from_end : gq == jt ? columns_before : gq > jt && gq < it ? all : 0.0f;
 }
 
+// ---- values that are not finite.  In dq = Y k, dk = Y^T q and dv = X^T dout a NaN or an infinity would meet the zero weights beyond the diagonal and so
+// reach rows that do not depend on its own.  In a chunk that holds one they stay out of the products and are added to the rows they belong to alone.
+__device__ __forceinline__ float finite_or_0(float x) { return __builtin_isfinite(x) ? x : 0.0f; }
+// column c of a tile of `rows` rows: add(row, value) for each value that is not finite
+template <typename F>
+__device__ __forceinline__ void each_not_finite(const float *column, int pitch, int rows, F add) {
+#pragma unroll 1
+    for (int t = 0; t < rows; ++t) {
+        const float x = column[t * pitch];
+        if (!__builtin_isfinite(x)) add(t, x);
+    }
+}
+// the same for four columns of bf16: add(row, r, value)
+template <typename F>
+__device__ __forceinline__ void each_not_finite4(const unsigned char *columns, int pitch, int rows, F add) {
+#pragma unroll 1
+    for (int t = 0; t < rows; ++t) {
+        const u32x2 w = *reinterpret_cast<const u32x2 *>(columns + t * pitch);
+        const f2 a = bf16pair_to_f2(w.x), b = bf16pair_to_f2(w.y);
+        const float x[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (!__builtin_isfinite(x[r])) add(t, r, x[r]);
+    }
+}
+
 // seg_states[slot] = D behind the segment; one thread W elements
 template <int W>
 __global__ __launch_bounds__(NT) void la_join_bwd_kernel(const BwdArgs a, int C) {
@@ -163,9 +189,10 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
     constexpr int XY = CT * (CT + 1) / 2 * 16 * PP;                  // X, Y: their tiles up to the diagonal
     constexpr int NV = (VT * CT + NW - 1) / NW;                      // tiles of dv a wave owns
     static_assert(KT * CT <= NW && NV <= 2, "tiles of a wave");
-    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * XY + 10 * 64 + NW * 64 + NW];
+    __shared__ __attribute__((aligned(16))) float lds[2 * C * PK + 2 * C * PV + DK * PV + 2 * XY + 10 * 64 + NW * 64 + NW + 4];
     float *Qs = lds, *Ks = Qs + C * PK, *Vs = Ks + C * PK, *Os = Vs + C * PV, *St = Os + C * PV, *Xs = St + DK * PV, *Ys = Xs + XY;
     float *decays = Ys + XY, *parts = decays + 10 * 64, *corners = parts + NW * 64;
+    int *poison = reinterpret_cast<int *>(corners + NW);             // the last chunk that held a NaN or an infinity in q, k or dout
     const auto tile_at = [](int it, int jt) { return (it * (it + 1) / 2 + jt) * 16 * PP; };
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
@@ -294,6 +321,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
     scan(c1 - 1);
     fetch_g(c1 - 2);
     if (c0 < c1) fetch(c1 - 1);
+    if (tid == 0) *poison = -1;
 #pragma unroll 1
     for (int c = c1 - 1; c >= c0; --c) {
         const int nr = rows_of(c);
@@ -304,6 +332,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
         kr.put(Ks, p.dk);
         vr.put(Vs, p.dv);
         orr.put(Os, p.dv);
+        if (qr.not_finite() || kr.not_finite() || orr.not_finite()) *poison = c;
         put_state(sr);
         float corner = 0.0f;                                         // <D, S>
 #pragma unroll
@@ -311,6 +340,7 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
         Q -= C * p.ql; K -= C * p.kl; V -= C * p.vl; DO -= C * ldv; saved -= p.H * sz;
         if (c > c0) fetch(c - 1);
         __syncthreads();
+        const bool poisoned = __builtin_amdgcn_readfirstlane(*poison) == c;
         const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
         float cross = 0.0f;                                          // what this wave's pairs add to the decay of token `lane`
         // X, Y and the sums of M below the diagonal
@@ -368,8 +398,18 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
                 f4 y;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) y[r] = Ks[(16 * jt + 4 * gq + r) * PK + k];
+                if (poisoned) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = finite_or_0(y[r]);
+                }
                 dq = dot4(*reinterpret_cast<const f4 *>(Ys + tile_at(qi, jt) + l16 * PP + 4 * gq), y, dq);
             }
+            if (poisoned)
+                each_not_finite(Ks + k, PK, 16 * qi + 16, [&](int j, float x) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (j <= 16 * qi + 4 * gq + r) dq[r] += Ys[tile_at(qi, j >> 4) + (4 * gq + r) * PP + (j & 15)] * x;
+                });
             const RowsOut out(DQ, nr, ldq);
 #pragma unroll
             for (int r = 0; r < 4; ++r) out.put1(dq[r], 16 * qi + 4 * gq + r, k, ldq, p.dk);
@@ -393,8 +433,18 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
                     x[r] = Ys[tile_at(it, qi) + (4 * gq + r) * PP + l16];
                     y[r] = Qs[(16 * it + 4 * gq + r) * PK + k];
                 }
+                if (poisoned) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = finite_or_0(y[r]);
+                }
                 dk = dot4(x, y, dk);
             }
+            if (poisoned)
+                each_not_finite(Qs + k, PK, C, [&](int i, float x) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i >= 16 * qi + 4 * gq + r) dk[r] += Ys[tile_at(i >> 4, qi) + (i & 15) * PP + 4 * gq + r] * x;
+                });
             const RowsOut out(DKp, nr, ldq);
 #pragma unroll
             for (int r = 0; r < 4; ++r) out.put1(dk[r], 16 * qi + 4 * gq + r, k, ldq, p.dk);
@@ -422,8 +472,18 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
                     x[r] = Xs[tile_at(it, vj) + (4 * gq + r) * PP + l16];
                     y[r] = Os[(16 * it + 4 * gq + r) * PV + col];
                 }
+                if (poisoned) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = finite_or_0(y[r]);
+                }
                 dv = dot4(x, y, dv);
             }
+            if (poisoned)
+                each_not_finite(Os + col, PV, C, [&](int i, float x) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i >= 16 * vj + 4 * gq + r) dv[r] += Xs[tile_at(i >> 4, vj) + (i & 15) * PP + 4 * gq + r] * x;
+                });
             const RowsOut out(DVp, nr, ldv);
 #pragma unroll
             for (int r = 0; r < 4; ++r) out.put1(dv[r], 16 * vj + 4 * gq + r, col, ldv, p.dv);
@@ -482,10 +542,11 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
     const auto rows32 = [](int half) { return half ? 32 * (P0 - P1) : 0; };                   // where row 0 would lie at that half's pitch
     constexpr int NB = TIGHT || (DK == 128 && DV == 128) ? 1 : 3;                                      // terms of a state in LDS at once
     constexpr int NI = 4 * KT / NW, NJ = 4 * VT / NW, TW = KT * VT / NW;                               // tiles of a wave: rows of dq / dk, rows of dv, D
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + NW) * 4];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + NW + 4) * 4];
     unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + XY, *Yh = Xl + XY,
                   *Yl = Yh + XY, *St = Yl + XY;
     float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + NW * C;
+    int *poison = reinterpret_cast<int *>(corners + NW);             // the last chunk that held a NaN or an infinity in q, k or dout
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -611,6 +672,7 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
         *reinterpret_cast<u32x2 *>(Yh + at) = u32x2{0, 0};
         *reinterpret_cast<u32x2 *>(Yl + at) = u32x2{0, 0};
     }
+    if (tid == 0) *poison = -1;
     scan(c1 - 1);
     fetch_g(c1 - 2);
 #pragma unroll 1
@@ -623,11 +685,18 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
         kr.put(Ks, QP, p.dk);
         vr.put(Vs, VP, p.dv);
         orr.put(Os, VP, p.dv);
+        if (qr.not_finite() || kr.not_finite() || orr.not_finite()) *poison = c;
         float corner = 0.0f;                                         // <D, S>
 #pragma unroll
         for (int t = 0; t < TW; ++t) corner += (sr[t].x * D[t].x + sr[t].y * D[t].y) + (sr[t].z * D[t].z + sr[t].w * D[t].w);
         put_terms(sr, 0);
         __syncthreads();
+        const bool poisoned = __builtin_amdgcn_readfirstlane(*poison) == c;
+        // elements of X and Y
+        const auto pair_of = [&](const unsigned char *hi, const unsigned char *lo, int i, int j) {
+            const int at = rows32(i >> 5) + i * pitch(i >> 5) + 2 * j;
+            return (float)*reinterpret_cast<const bf16 *>(hi + at) + (float)*reinterpret_cast<const bf16 *>(lo + at);
+        };
         float cross = 0.0f;                                          // what this wave's pairs add to the decay of token `lane`
         // X, Y and the sums of M below the diagonal: ten 16 x 16 tiles dealt to the waves
 #pragma unroll
@@ -708,7 +777,8 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
             put_terms(D, 0);
 #pragma unroll
             for (int js = 0; js < 2; ++js) {
-                const bf16x8 kf = frag_tc(Ks, QP, kt, js, lane);
+                bf16x8 kf = frag_tc(Ks, QP, kt, js, lane);
+                if (poisoned) finite_only(kf);
 #pragma unroll
                 for (int m = 0; m < NI; ++m) {
                     if (js > (i0 + m) / 2) continue;
@@ -716,6 +786,12 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
                     acc[m] = mfma8(kf, frag_c(Yl + rows32((i0 + m) / 2), pitch((i0 + m) / 2), 16 * (i0 + m) + l16, js, gq), acc[m]);
                 }
             }
+            if (poisoned)
+                each_not_finite4(Ks + 2 * k, QP, C, [&](int j, int r, float x) {
+#pragma unroll
+                    for (int m = 0; m < NI; ++m)
+                        if (j <= 16 * (i0 + m) + l16) acc[m][r] += pair_of(Yh, Yl, 16 * (i0 + m) + l16, j) * x;
+                });
             const RowsOut out(DQ, nr, ldq);
 #pragma unroll
             for (int m = 0; m < NI; ++m) out.template put4<VEC>(DQ, 16 * (i0 + m) + l16, k, ldq, p.dk, acc[m]);
@@ -782,7 +858,11 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
             for (int m = 0; m < NJ; ++m) dv[m] *= wt[16 * (j0 + m) + l16];
 #pragma unroll
             for (int is = 0; is < 2; ++is) {
-                const bf16x8 qf = frag_t(Qs, QP, kt, is, lane), of = frag_t(Os, VP, vt, is, lane);
+                bf16x8 qf = frag_t(Qs, QP, kt, is, lane), of = frag_t(Os, VP, vt, is, lane);
+                if (poisoned) {
+                    finite_only(qf);
+                    finite_only(of);
+                }
 #pragma unroll
                 for (int m = 0; m < NI; ++m) {
                     if (is < (i0 + m) / 2) continue;
@@ -797,6 +877,18 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
                 }
             }
             const int k = 16 * kt + 4 * gq, v = 16 * vt + 4 * gq;
+            if (poisoned) {
+                each_not_finite4(Qs + 2 * k, QP, C, [&](int i, int r, float x) {
+#pragma unroll
+                    for (int m = 0; m < NI; ++m)
+                        if (i >= 16 * (i0 + m) + l16) dk[m][r] += pair_of(Yh, Yl, i, 16 * (i0 + m) + l16) * x;
+                });
+                each_not_finite4(Os + 2 * v, VP, C, [&](int i, int r, float x) {
+#pragma unroll
+                    for (int m = 0; m < NJ; ++m)
+                        if (i >= 16 * (j0 + m) + l16) dv[m][r] += pair_of(Xh, Xl, i, 16 * (j0 + m) + l16) * x;
+                });
+            }
             const RowsOut outk(DKp, nr, ldq), outv(DVp, nr, ldv);
 #pragma unroll
             for (int m = 0; m < NI; ++m) outk.template put4<VEC>(DKp, 16 * (i0 + m) + l16, k, ldq, p.dk, dk[m]);

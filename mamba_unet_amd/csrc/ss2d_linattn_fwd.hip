@@ -435,16 +435,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
             if (poisoned) {
                 int bad = 0;
 #pragma unroll
-                for (int js = 0; js < 2; ++js) {
-                    u32x4 w = __builtin_bit_cast(u32x4, vf[js]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const unsigned m = ((w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;       // the halves that are not finite
-                        bad |= m != 0;
-                        w[i] &= ~(m | (m - (m >> 15)));
-                    }
-                    vf[js] = __builtin_bit_cast(bf16x8, w);
-                }
+                for (int js = 0; js < 2; ++js) bad |= finite_only(vf[js]);
                 bad |= __shfl_xor(bad, 16, 64);
                 bad |= __shfl_xor(bad, 32, 64);
                 if (bad) eend = __builtin_nanf("");

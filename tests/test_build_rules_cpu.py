@@ -27,3 +27,12 @@ def test_no_packed_fp32_in_the_operators_beside_the_scan(args):
 def test_a_variant_is_compiled_as_the_file_itself(name):
     line = [x for x in commands("variant", f"SRC={name}", "NAME=other", "DEFS=-DX") if f"-c {name}.hip" in x and "-DX" in x]
     assert len(line) == 1 and "-packed-fp32-ops" in line[0]
+
+
+def test_the_library_alone_is_built_without_torch():
+    host, library = "host_ops.cpp", "-shared -o ../libss2d_hip.so"
+    both = "\n".join(commands())
+    assert host in both and library in both
+    for args in (("PYTHON=false",), ("lib",)):
+        only = "\n".join(commands(*args))
+        assert host not in only and library in only

@@ -73,9 +73,23 @@ struct Named {
 void check_no_tangent(const char *op, const Tensor &t) {
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), op, ": forward-mode derivatives are not implemented (a tensor with a tangent was given)");
 }
-// a tensor with a tangent raises, and the first one that is not on the GPU, or on another one than the first
+constexpr c10::DispatchKeySet WITHOUT_MEMORY({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+// most tensors need neither check (reading the tangent itself takes a lock: 15 ns a tensor)
+inline bool plain(const Tensor &t) {
+    const auto *meta = static_cast<const torch::autograd::AutogradMeta *>(t.unsafeGetTensorImpl()->autograd_meta());
+    return (!meta || !meta->fw_grad_) && !t.key_set().has_any(WITHOUT_MEMORY);
+}
+// Views that stand for other values than their memory holds (the imaginary part of a conjugate: the sign is left to whoever reads it) or for none
+void check_memory(const char *op, const Tensor &t) {
+    TORCH_CHECK_VALUE(!t.defined() || !t.key_set().has_any(WITHOUT_MEMORY), op, ": a negated view or a tensor without memory was given: call resolve_neg() or clone() on it first");
+}
+// a tensor with a tangent or without memory of its values raises, and the first one that is not on the GPU, or on another one than the first
 void check_tensors(const char *op, std::initializer_list<Named> all) {
-    for (const Named &n : all) check_no_tangent(op, *n.t);
+    for (const Named &n : all)
+        if (n.t->defined() && !plain(*n.t)) {
+            check_no_tangent(op, *n.t);
+            check_memory(op, *n.t);
+        }
     const Named *first = nullptr;
     for (const Named &n : all) {
         if (!n.t->defined()) continue;
@@ -98,7 +112,8 @@ variable_list once(variable_list out) {
     return torch::autograd::DelayedError("trying to differentiate twice an operator whose backward is a kernel", (int)out.size())(std::move(out));
 }
 // dense, in the storage type, on a 16-byte boundary
-Tensor dense16(const Tensor &g, at::ScalarType io) {
+Tensor dense16(const Tensor &g0, at::ScalarType io) {
+    const Tensor g = !g0.defined() ? g0 : g0._is_zerotensor() ? at::zeros(g0.sizes(), g0.options()) : g0.resolve_neg();
     if (!g.defined() || (g.scalar_type() == io && g.is_contiguous() && (uintptr_t)g.data_ptr() % 16 == 0)) return g;
     return g.to(io).clone(at::MemoryFormat::Contiguous);
 }
@@ -533,7 +548,10 @@ Tensor clip_grad_norm(const py::object &given, double max_norm, double norm_type
     std::vector<std::pair<size_t, Tensor>> copies;     // of what is not dense in any order of its axes
     for (size_t i = 0; i < n; ++i) {
         const Tensor &g = grads[i];
-        check_no_tangent("clip_grad_norm", g);
+        if (!plain(g)) {
+            check_no_tangent("clip_grad_norm", g);
+            check_memory("clip_grad_norm", g);
+        }
         TORCH_CHECK(g.is_cuda(), "clip_grad_norm: GPU tensors required (no CPU path in mamba_unet_amd)");
         TORCH_CHECK_VALUE(g.device() == dev, "clip_grad_norm: gradients on several devices: ", dev, ", ", g.device());
         TORCH_CHECK_VALUE(g.layout() == at::kStrided && (g.scalar_type() == at::kFloat || g.scalar_type() == at::kBFloat16),

@@ -118,8 +118,7 @@ __device__ __forceinline__ int fresh(int v) { asm volatile("" : "+v"(v)); return
 // ---- bf16 operands on v_mfma_f32_16x16x32_bf16.  A lane (l16 = lane & 15, gq = lane >> 4) holds row / column l16 of an operand and eight of the 32
 // contracted indices.  Here they are 4 gq + {0..3} and 16 + 4 gq + {0..3} for every operand: the two halves are then exactly the rows that
 // the lane holds of two neighbouring 16 x 16 results, so a state in accumulators is an operand without moving data.
-// fp32 factors (states, weighted values, weights) enter as sums of two or three bf16 values: two leave 2^-17 of a term, below the rounding
-// of a bf16 result; three leave nothing of its 24 bits, for what stays in fp32 (states, gradients of the decays).
+// fp32 factors (states, weighted values, weights) enter as sums of three bf16 values, which leave nothing of their 24 bits.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -191,6 +190,23 @@ __device__ __forceinline__ bf16x8 frag_tc(const unsigned char *tile, int pitch, 
 }
 __device__ __forceinline__ bf16x8 frag_c(const unsigned char *tile, int pitch, int row, int s, int gq) {
     return *reinterpret_cast<const bf16x8 *>(tile + row * pitch + (32 * s + 8 * gq) * 2);
+}
+
+// The weights of a chunk's pairs (64 x 64, below the diagonal) in LDS, three planes of PAIRS bytes, a bf16 term each: rows 0 ... 31 hold 32 columns, rows 32 ... 63
+// hold 64.  pair_row(half, i): row i from a plane's start (row 0 where its pitch would put it).
+constexpr int PAIR_PITCH0 = 64 + 16, PAIR_PITCH1 = 128 + 16, PAIRS = 32 * (PAIR_PITCH0 + PAIR_PITCH1);
+__device__ __forceinline__ constexpr int pair_pitch(int half) { return half ? PAIR_PITCH1 : PAIR_PITCH0; }
+__device__ __forceinline__ constexpr int pair_row(int half, int i) { return (half ? 32 * (PAIR_PITCH0 - PAIR_PITCH1) : 0) + i * pair_pitch(half); }
+__device__ __forceinline__ void put_pairs(unsigned char *at, f4 v) {
+#pragma unroll
+    for (int u = 0; u < 3; ++u) {
+        const bf16x4 w = round4(v);
+        *reinterpret_cast<bf16x4 *>(at + u * PAIRS) = w;
+        v = rest4(v, w);
+    }
+}
+__device__ __forceinline__ float get_pair(const unsigned char *at) {
+    return ((float)*reinterpret_cast<const bf16 *>(at + 2 * PAIRS) + (float)*reinterpret_cast<const bf16 *>(at + PAIRS)) + (float)*reinterpret_cast<const bf16 *>(at);
 }
 
 // A C x DP tile of bf16 on its way from memory to LDS, in 16-byte pieces of a row that wait in registers, so a chunk is in flight while the previous

@@ -522,29 +522,26 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
     }
 }
 
-// The same walk for bf16 tensors on the bf16 matrix instruction: chunks of 64, 16 waves a workgroup (dk <= 32 and 64 x 64: 8).  LDS holds the four tiles, X and Y (two terms
-// each) and the terms of ONE state at a time, transposed (dv x dk): first S (for dq), then D (for dk and dv); with NB = 1 (64 x 64, 128 x 128) one
-// term at a time.  States enter with three terms where dg is taken from the product (q . S do, k . D v), with two in dv.
+// The same walk for bf16 tensors on the bf16 matrix instruction: chunks of 64, 16 waves a workgroup (dk <= 32 and 64 x 64: 8).  LDS holds the four tiles, X and Y packed
+// below the diagonal and the terms of ONE state at a time, transposed (dv x dk): first S (for dq), then D (for dk and dv); with NB = 1 (64 x 64, 128 x 128) one
+// term at a time.  X, Y, S and D all enter in three terms: nothing between the inputs and the rounded gradients has less than 24 bits (two terms of X, Y, and of D in
+// dv, which leave 2^-17 of a term, took 356 us for 4 x 4096 tokens, 16 heads of 128 x 64, forward and backward, three take 371; of 64 x 64, 208 and 212).
 // Direct operands are eight values in a row (one 16-byte LDS read); what they are multiplied with, where it is read transposed, takes its contracted
 // rows in the same order (frag_tc).  Products of two transposed operands (over tokens) use frag_t for both.
 //
-// Up to 64 x 64 two workgroups of eight waves share a CU, so that one works while the other waits at its barriers: X and Y are packed below the diagonal,
-// and at 64 x 64 rows are half a pitch step shorter and a state's terms take turns (24 x 3136 tokens, 3 heads of 16 x 64, forward and
+// Up to 64 x 64 two workgroups of eight waves share a CU, so that one works while the other waits at its barriers: X waits in registers until dk is done with Y
+// and takes its place, and at 64 x 64 rows are half a pitch step shorter and a state's terms take turns (24 x 3136 tokens, 3 heads of 16 x 64, forward and
 // backward: 142 us with one workgroup of eight waves a CU, 123 with two; 4 x 4096, 16 heads of 64 x 64: 220 with one of sixteen, 208 with two of eight).
 template <int DK, int DV, int NW, bool VEC, typename QT>
 __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la_bwd_bf16_kernel(const BwdArgs a) {
     constexpr int NT = 64 * NW, C = 64, KT = DK / 16, KS = DK / 32, VT = DV / 16, VS = DV / 32;
-    constexpr bool PACKED = DK <= 64 && DV <= 64, TIGHT = DK == 64 && DV == 64;
+    constexpr bool TURNS = DK <= 64 && DV <= 64, TIGHT = DK == 64 && DV == 64;
     constexpr int QP = 2 * DK + (TIGHT ? 16 : 32), VP = 2 * DV + (TIGHT ? 16 : 32), SP = 2 * DK + 16;      // bytes a row
-    // X and Y: the first 32 rows need one block of 32 columns, the others two
-    constexpr int P0 = PACKED ? C + 16 : 2 * C + 32, P1 = PACKED ? 2 * C + 16 : 2 * C + 32, XY = 32 * (P0 + P1);
-    const auto pitch = [](int half) { return half ? P1 : P0; };
-    const auto rows32 = [](int half) { return half ? 32 * (P0 - P1) : 0; };                   // where row 0 would lie at that half's pitch
     constexpr int NB = TIGHT || (DK == 128 && DV == 128) ? 1 : 3;                                      // terms of a state in LDS at once
     constexpr int NI = 4 * KT / NW, NJ = 4 * VT / NW, TW = KT * VT / NW;                               // tiles of a wave: rows of dq / dk, rows of dv, D
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + 4 * XY + NB * DV * SP + (10 * C + NW * C + NW + 4) * 4];
-    unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Xh = Os + C * VP, *Xl = Xh + XY, *Yh = Xl + XY,
-                  *Yl = Yh + XY, *St = Yl + XY;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * C * QP + 2 * C * VP + (TURNS ? 3 : 6) * PAIRS + NB * DV * SP + (10 * C + NW * C + NW + 4) * 4];
+    unsigned char *Qs = lds, *Ks = Qs + C * QP, *Vs = Ks + C * QP, *Os = Vs + C * VP, *Ys = Os + C * VP,
+                  *Xs = TURNS ? Ys : Ys + 3 * PAIRS, *St = Xs + 3 * PAIRS;
     float *decays = reinterpret_cast<float *>(St + NB * DV * SP), *parts = decays + 10 * C, *corners = parts + NW * C;
     int *poison = reinterpret_cast<int *>(corners + NW);             // the last chunk that held a NaN or an infinity in q, k or dout
     const Problem &p = a.p;
@@ -666,11 +663,9 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
         }
     };
     if (tid < 128) {                             // the tiles of X and Y behind the diagonal that are read with it (32 columns at a time): zero for good
-        const int half = tid >> 6, i = 32 * half + (tid & 15), at = rows32(half) + i * pitch(half) + 2 * (32 * half + 16 + 4 * ((tid >> 4) & 3));
-        *reinterpret_cast<u32x2 *>(Xh + at) = u32x2{0, 0};
-        *reinterpret_cast<u32x2 *>(Xl + at) = u32x2{0, 0};
-        *reinterpret_cast<u32x2 *>(Yh + at) = u32x2{0, 0};
-        *reinterpret_cast<u32x2 *>(Yl + at) = u32x2{0, 0};
+        const int half = tid >> 6, at = pair_row(half, 32 * half + (tid & 15)) + 2 * (32 * half + 16 + 4 * ((tid >> 4) & 3));
+#pragma unroll
+        for (int u = 0; u < (TURNS ? 3 : 6); ++u) *reinterpret_cast<u32x2 *>(Ys + u * PAIRS + at) = u32x2{0, 0};
     }
     if (tid == 0) *poison = -1;
     scan(c1 - 1);
@@ -692,15 +687,13 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
         put_terms(sr, 0);
         __syncthreads();
         const bool poisoned = __builtin_amdgcn_readfirstlane(*poison) == c;
-        // elements of X and Y
-        const auto pair_of = [&](const unsigned char *hi, const unsigned char *lo, int i, int j) {
-            const int at = rows32(i >> 5) + i * pitch(i >> 5) + 2 * j;
-            return (float)*reinterpret_cast<const bf16 *>(hi + at) + (float)*reinterpret_cast<const bf16 *>(lo + at);
-        };
+        const auto pair_of = [](const unsigned char *pairs, int i, int j) { return get_pair(pairs + pair_row(i >> 5, i) + 2 * j); };
         float cross = 0.0f;                                          // what this wave's pairs add to the decay of token `lane`
         // X, Y and the sums of M below the diagonal: ten 16 x 16 tiles dealt to the waves
+        constexpr int NTL = (10 + NW - 1) / NW;
+        f4 xs[NTL];                                                  // X, where it takes Y's place later
 #pragma unroll
-        for (int tn = 0; tn < (10 + NW - 1) / NW; ++tn) {
+        for (int tn = 0; tn < NTL; ++tn) {
             const int t = wave + tn * NW;
             if (t >= 10) break;
             const int lane = fresh(lane0), l16 = lane & 15, gq = lane >> 4;
@@ -720,12 +713,10 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
                 m[r] = j + r < i ? x[r] * y[r] : 0.0f;
                 x[r] = j + r <= i ? x[r] * w : 0.0f;
             }
-            const int at = rows32(it / 2) + i * pitch(it / 2) + 2 * j;
-            const bf16x4 xh = round4(x), yh = round4(y);
-            *reinterpret_cast<bf16x4 *>(Xh + at) = xh;
-            *reinterpret_cast<bf16x4 *>(Xl + at) = round4(rest4(x, xh));
-            *reinterpret_cast<bf16x4 *>(Yh + at) = yh;
-            *reinterpret_cast<bf16x4 *>(Yl + at) = round4(rest4(y, yh));
+            const int at = pair_row(it / 2, i) + 2 * j;
+            put_pairs(Ys + at, y);
+            if (TURNS) xs[tn] = x;
+            else put_pairs(Xs + at, x);
             if (it == jt) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) m[r] = row16_from_end(m[r]);        // of column j, the rows from token l16 on
@@ -782,15 +773,17 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
 #pragma unroll
                 for (int m = 0; m < NI; ++m) {
                     if (js > (i0 + m) / 2) continue;
-                    acc[m] = mfma8(kf, frag_c(Yh + rows32((i0 + m) / 2), pitch((i0 + m) / 2), 16 * (i0 + m) + l16, js, gq), acc[m]);
-                    acc[m] = mfma8(kf, frag_c(Yl + rows32((i0 + m) / 2), pitch((i0 + m) / 2), 16 * (i0 + m) + l16, js, gq), acc[m]);
+                    const int half = (i0 + m) / 2;
+#pragma unroll
+                    for (int u = 0; u < 3; ++u)
+                        acc[m] = mfma8(kf, frag_c(Ys + u * PAIRS + pair_row(half, 0), pair_pitch(half), 16 * (i0 + m) + l16, js, gq), acc[m]);
                 }
             }
             if (poisoned)
                 each_not_finite4(Ks + 2 * k, QP, C, [&](int j, int r, float x) {
 #pragma unroll
                     for (int m = 0; m < NI; ++m)
-                        if (j <= 16 * (i0 + m) + l16) acc[m][r] += pair_of(Yh, Yl, 16 * (i0 + m) + l16, j) * x;
+                        if (j <= 16 * (i0 + m) + l16) acc[m][r] += pair_of(Ys, 16 * (i0 + m) + l16, j) * x;
                 });
             const RowsOut out(DQ, nr, ldq);
 #pragma unroll
@@ -827,18 +820,16 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
                         for (int m = 0; m < NI; ++m) dk[m] = mfma8(df, vf[m], dk[m]);
                     }
                 }
-                if (u0 < 2) {
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        bf16x8 kf[NJ];
+                for (int ks = 0; ks < KS; ++ks) {
+                    bf16x8 kf[NJ];
 #pragma unroll
-                        for (int m = 0; m < NJ; ++m) kf[m] = frag_c(Ks, QP, 16 * (j0 + m) + l16, ks, gq);
+                    for (int m = 0; m < NJ; ++m) kf[m] = frag_c(Ks, QP, 16 * (j0 + m) + l16, ks, gq);
 #pragma unroll
-                        for (int u = 0; u < (NB == 3 ? 2 : 1); ++u) {
-                            const bf16x8 df = frag_c(St + u * DV * SP, SP, vrow, ks, gq);
+                    for (int u = 0; u < NB; ++u) {
+                        const bf16x8 df = frag_c(St + u * DV * SP, SP, vrow, ks, gq);
 #pragma unroll
-                            for (int m = 0; m < NJ; ++m) dv[m] = mfma8(df, kf[m], dv[m]);
-                        }
+                        for (int m = 0; m < NJ; ++m) dv[m] = mfma8(df, kf[m], dv[m]);
                     }
                 }
             }
@@ -856,42 +847,53 @@ __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la
             if (lane == 0) corners[wave] = corner;
 #pragma unroll
             for (int m = 0; m < NJ; ++m) dv[m] *= wt[16 * (j0 + m) + l16];
+            const int k = 16 * kt + 4 * gq, v = 16 * vt + 4 * gq;
+            const RowsOut outk(DKp, nr, ldq), outv(DVp, nr, ldv);
 #pragma unroll
             for (int is = 0; is < 2; ++is) {
-                bf16x8 qf = frag_t(Qs, QP, kt, is, lane), of = frag_t(Os, VP, vt, is, lane);
-                if (poisoned) {
-                    finite_only(qf);
-                    finite_only(of);
-                }
+                bf16x8 qf = frag_t(Qs, QP, kt, is, lane);
+                if (poisoned) finite_only(qf);
 #pragma unroll
                 for (int m = 0; m < NI; ++m) {
                     if (is < (i0 + m) / 2) continue;
-                    dk[m] = mfma8(qf, frag_t(Yh + rows32(is), pitch(is), i0 + m, is, lane), dk[m]);
-                    dk[m] = mfma8(qf, frag_t(Yl + rows32(is), pitch(is), i0 + m, is, lane), dk[m]);
-                }
 #pragma unroll
-                for (int m = 0; m < NJ; ++m) {
-                    if (is < (j0 + m) / 2) continue;
-                    dv[m] = mfma8(of, frag_t(Xh + rows32(is), pitch(is), j0 + m, is, lane), dv[m]);
-                    dv[m] = mfma8(of, frag_t(Xl + rows32(is), pitch(is), j0 + m, is, lane), dv[m]);
+                    for (int u = 0; u < 3; ++u) dk[m] = mfma8(qf, frag_t(Ys + u * PAIRS + pair_row(is, 0), pair_pitch(is), i0 + m, is, lane), dk[m]);
                 }
             }
-            const int k = 16 * kt + 4 * gq, v = 16 * vt + 4 * gq;
-            if (poisoned) {
+            if (poisoned)
                 each_not_finite4(Qs + 2 * k, QP, C, [&](int i, int r, float x) {
 #pragma unroll
                     for (int m = 0; m < NI; ++m)
-                        if (i >= 16 * (i0 + m) + l16) dk[m][r] += pair_of(Yh, Yl, i, 16 * (i0 + m) + l16) * x;
+                        if (i >= 16 * (i0 + m) + l16) dk[m][r] += pair_of(Ys, i, 16 * (i0 + m) + l16) * x;
                 });
+#pragma unroll
+            for (int m = 0; m < NI; ++m) outk.template put4<VEC>(DKp, 16 * (i0 + m) + l16, k, ldq, p.dk, dk[m]);
+            if (TURNS) {
+                __syncthreads();                                      // Y is done with
+#pragma unroll
+                for (int tn = 0; tn < NTL; ++tn) {
+                    const int t = wave + tn * NW, it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
+                    if (t < 10) put_pairs(Xs + pair_row(it / 2, 16 * it + l16) + 2 * (16 * jt + 4 * gq), xs[tn]);
+                }
+                __syncthreads();                                      // X is there
+            }
+#pragma unroll
+            for (int is = 0; is < 2; ++is) {
+                bf16x8 of = frag_t(Os, VP, vt, is, lane);
+                if (poisoned) finite_only(of);
+#pragma unroll
+                for (int m = 0; m < NJ; ++m) {
+                    if (is < (j0 + m) / 2) continue;
+#pragma unroll
+                    for (int u = 0; u < 3; ++u) dv[m] = mfma8(of, frag_t(Xs + u * PAIRS + pair_row(is, 0), pair_pitch(is), j0 + m, is, lane), dv[m]);
+                }
+            }
+            if (poisoned)
                 each_not_finite4(Os + 2 * v, VP, C, [&](int i, int r, float x) {
 #pragma unroll
                     for (int m = 0; m < NJ; ++m)
-                        if (i >= 16 * (j0 + m) + l16) dv[m][r] += pair_of(Xh, Xl, i, 16 * (j0 + m) + l16) * x;
+                        if (i >= 16 * (j0 + m) + l16) dv[m][r] += pair_of(Xs, i, 16 * (j0 + m) + l16) * x;
                 });
-            }
-            const RowsOut outk(DKp, nr, ldq), outv(DVp, nr, ldv);
-#pragma unroll
-            for (int m = 0; m < NI; ++m) outk.template put4<VEC>(DKp, 16 * (i0 + m) + l16, k, ldq, p.dk, dk[m]);
 #pragma unroll
             for (int m = 0; m < NJ; ++m) outv.template put4<VEC>(DVp, 16 * (j0 + m) + l16, v, ldv, p.dv, dv[m]);
         }

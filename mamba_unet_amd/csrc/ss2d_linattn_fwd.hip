@@ -269,16 +269,20 @@ __global__ __launch_bounds__(NT) void la_fwd_kernel(const FwdArgs a) {
 }
 
 // The same walk for bf16 tensors on the bf16 matrix instruction; a workgroup owns all of dv (a wave 16 columns: NW = 4 or 8 waves), the next chunk is in
-// flight in registers during the products.  Per chunk: P (two-term weights, to LDS), then for all rows i  O^T = S^T Q^T (S in two terms), scaled by
-// exp(b_i), plus V^T P^T, then S += K^T (exp(b_C - b_j) V) with the weighted V in three terms: the state keeps 24 bits.
+// flight in registers during the products.  Per chunk: P (weights, to LDS), then for all rows i  O^T = S^T Q^T, scaled by exp(b_i), plus V^T P^T, then
+// S += K^T (exp(b_C - b_j) V), with P, S and the weighted V in three bf16 terms: nothing between the inputs and the rounded results has less than 24
+// bits.  (Two terms of P and S, which leave 2^-17 of a term, took 245 us for 65536 tokens, 8 heads of 128 x 128, three take 263; 9 prompts of 7121 tokens, 16 heads of
+// 64 x 64, 38 and 40.)
 // LDS rows are an odd number of 32-byte pieces long: 16-byte direct reads (4 cycles) and transposed ones (2) are then free of bank conflicts (measured
-// over pitches of 128 ... 320 bytes); q and P lie in operand order, so a lane's eight values are one read.
+// over pitches of 128 ... 320 bytes); q and P lie in operand order, so a lane's eight values are one read.  P is packed below the diagonal (and q's rows at 64 wide
+// keys are half a piece shorter), so that as many workgroups share a CU as with two terms.
 template <int DK, int NW, int MODE, bool VEC>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fwd_bf16_kernel(const FwdArgs a) {
-    constexpr int NT = 64 * NW, C = 64, DV = 16 * NW, KT = DK / 16, KS = DK / 32, QP = 2 * DK + 32, KP = 2 * DK + 32, VP = 2 * DV + 32, PP = 2 * C + 32;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[C * (KP + VP) + (MODE == 0 ? C * (QP + 2 * PP) : 0) + 10 * C * 4];
-    unsigned char *Ks = lds, *Vs = Ks + C * KP, *Qs = Vs + C * VP, *Ph = Qs + C * QP, *Pl = Ph + C * PP;
-    float *decays = reinterpret_cast<float *>(MODE == 0 ? Pl + C * PP : Qs);     // two chunks of: b (two terms), scale exp(b), exp(b_C - b), exp(b_C)
+    constexpr int NT = 64 * NW, C = 64, DV = 16 * NW, KT = DK / 16, KS = DK / 32, QP = 2 * DK + (DK == 64 && NW == 4 ? 16 : 32), KP = 2 * DK + 32,
+                  VP = 2 * DV + 32;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[C * (KP + VP) + (MODE == 0 ? C * QP + 3 * PAIRS : 0) + 10 * C * 4];
+    unsigned char *Ks = lds, *Vs = Ks + C * KP, *Qs = Vs + C * VP, *Ps = Qs + C * QP;
+    float *decays = reinterpret_cast<float *>(MODE == 0 ? Ps + 3 * PAIRS : Qs);     // two chunks of: b (two terms), scale exp(b), exp(b_C - b), exp(b_C)
     const Problem &p = a.p;
     const int tid = threadIdx.x, lane0 = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -354,9 +358,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
     scan(first);
     fetch_g(first + STEP);
     if (MODE == 0 && tid < 128) {                // the tiles of P behind the diagonal that are read with it (32 columns at a time): zero for good
-        const int i = 32 * (tid >> 6) + (tid & 15), at = i * PP + 2 * operand_pos(32 * (tid >> 6) + 16 + 4 * ((tid >> 4) & 3));
-        *reinterpret_cast<u32x2 *>(Ph + at) = u32x2{0, 0};
-        *reinterpret_cast<u32x2 *>(Pl + at) = u32x2{0, 0};
+        const int half = tid >> 6, at = pair_row(half, 32 * half + (tid & 15)) + 2 * operand_pos(32 * half + 16 + 4 * ((tid >> 4) & 3));
+#pragma unroll
+        for (int u = 0; u < 3; ++u) *reinterpret_cast<u32x2 *>(Ps + u * PAIRS + at) = u32x2{0, 0};
     }
     // A NaN or an infinity in v_j times the zero weight of an earlier row would reach that row.  Once one has been met, such values stay out of the
     // products and are added to the rows from j on alone, and their columns of the state become NaN.
@@ -401,10 +405,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
                 const f4 h4 = *reinterpret_cast<const f4 *>(bh + j), l4 = *reinterpret_cast<const f4 *>(bl + j);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[n][r] = j + r <= i ? acc[n][r] * p.scale * hw_exp2((hi - h4[r]) + (li - l4[r])) : 0.0f;
-                const bf16x4 x = round4(acc[n]);
-                const int at = i * PP + 2 * operand_pos(j);
-                *reinterpret_cast<bf16x4 *>(Ph + at) = x;
-                *reinterpret_cast<bf16x4 *>(Pl + at) = round4(rest4(acc[n], x));
+                put_pairs(Ps + pair_row(it / 2, i) + 2 * operand_pos(j), acc[n]);
             }
             __syncthreads();
         }
@@ -419,13 +420,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
             for (int it = 0; it < 4; ++it) acc[it] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                bf16x8 sf[2];
-                split8<2>(S[2 * ks], S[2 * ks + 1], sf);
+                bf16x8 sf[3];
+                split8<3>(S[2 * ks], S[2 * ks + 1], sf);
 #pragma unroll
                 for (int it = 0; it < 4; ++it) {
                     const bf16x8 q = frag_p(Qs, QP, 16 * it + l16, ks, gq);
-                    acc[it] = mfma8(sf[0], q, acc[it]);
-                    acc[it] = mfma8(sf[1], q, acc[it]);
+#pragma unroll
+                    for (int u = 0; u < 3; ++u) acc[it] = mfma8(sf[u], q, acc[it]);
                 }
                 if (NW == 8) __builtin_amdgcn_sched_barrier(0);
             }
@@ -444,8 +445,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
             for (int it = 0; it < 4; ++it) {
 #pragma unroll
                 for (int js = 0; js <= it / 2; ++js) {
-                    acc[it] = mfma8(vf[js], frag_p(Ph, PP, 16 * it + l16, js, gq), acc[it]);
-                    acc[it] = mfma8(vf[js], frag_p(Pl, PP, 16 * it + l16, js, gq), acc[it]);
+#pragma unroll
+                    for (int u = 0; u < 3; ++u)
+                        acc[it] = mfma8(vf[js], frag_p(Ps + u * PAIRS + pair_row(it / 2, 0), pair_pitch(it / 2), 16 * it + l16, js, gq), acc[it]);
                 }
             }
             if (poisoned) {
@@ -457,11 +459,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 4 : DK <= 64 ? 3 : 2) void la_fw
                     const int at = 2 * (operand_pos(j & ~3) + (j & 3));
 #pragma unroll
                     for (int it = 0; it < 4; ++it) {
-                        const unsigned char *w = Ph + (16 * it + l16) * PP + at;
-                        const float ph = (float)*reinterpret_cast<const bf16 *>(w), pl = (float)*reinterpret_cast<const bf16 *>(w + (Pl - Ph));
+                        if (j > 16 * it + l16) continue;
+                        const float w = get_pair(Ps + pair_row(it / 2, 16 * it + l16) + at);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (j <= 16 * it + l16 && !__builtin_isfinite(v[r])) acc[it][r] += (ph + pl) * v[r];
+                            if (!__builtin_isfinite(v[r])) acc[it][r] += w * v[r];
                     }
                 }
             }

@@ -372,9 +372,12 @@ __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_a
 inline int linattn_chunk(int dtype, int dk, int dv) { return dtype || (dk <= 64 && dv <= 64) ? 64 : 32; }
 
 // Segments.  One workgroup walks a segment; with fewer workgroups than the card holds at once it idles, and a segment costs a second pass over k and v (q
-// and dout in the backward) and a state's round trip.  So all tokens of all sequences and heads are dealt to as many workgroups as are resident
-// (forward: three a CU up to 64 x 64 in bf16, else two; backward: one a CU with keys beyond 64 wide in bf16, else two), at least two chunks each, in equal
-// parts of the longest sequence.  Measured, us, for half the workgroups / these / twice / no split: 24 x 3136 tokens, 3 heads of 16 x 64 fp32, forward and
+// and dout in the backward) and a state's round trip.  So all tokens of all sequences and heads are dealt to a number of workgroups, at
+// least two chunks each, in equal parts of the longest sequence: in the forward to as many as are resident (three a CU up to 64 x 64 in bf16, else two); in the
+// backward to one a CU with keys beyond 64 wide in bf16, else to two.  Two are resident with keys up to 16 wide in fp32 and up to 64 x 64 in bf16; the others in
+// fp32, and 64 x 128 in bf16, hold one a CU and take two rounds of pieces half as long: a few per cent more for few long sequences, less where the pieces of a batch
+// would not divide by the CUs (us, forward and backward, 256 / 512 workgroups: 2 x 16384 tokens, 4 heads of 64 x 64 fp32 227 / 237, 24 x 784 tokens, 6 heads 265 /
+// 233; 64 x 128 bf16 163 / 175 and 183 / 165; 4 x 4096, 16 heads of 128 x 128 fp32 1257 / 1291).  Measured, us, for half the workgroups / these / twice / no split: 24 x 3136 tokens, 3 heads of 16 x 64 fp32, forward and
 // backward 271 / 180 / 190 / 574; 4 x 4096 tokens, 16 heads of 128 x 64 bf16, both ways 551 / 364 / 381 / 973; 65536 tokens, 8 heads of 128 x 128 bf16, forward
 // 283 / 250 / 263 / 5402.  Short ones, 4 heads of 64 x 64 bf16: a chunk takes 3 us and the two further launches as much as two chunks: 256 tokens (4 chunks) 16 us in
 // one walk, 19 split; 384 tokens (6) 22 and 19.

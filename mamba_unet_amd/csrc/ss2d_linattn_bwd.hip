@@ -16,10 +16,10 @@
 // A workgroup walks one segment of one sequence and value head from its end to its start with D in accumulator registers (a wave owns
 // 16-column slices of dv).  Segments as in the forward: own contributions, a join in order, the walk.
 //
-// Measured.  4 x 4096 tokens, 16 heads of 128 x 64 on 2 key heads, bf16: contributions 33 us, join 6, walk 198, sum over the heads of a group 47 (5.7 TB/s).  A
-// chunk takes a workgroup of 16 waves, one a CU (157 KB of LDS), 24,000 cycles: the matrix units are busy 17% of them and LDS 42% (a quarter of that bank
-// conflicts of 8-byte writes), the rest waits between the phases, which need each other's results.  24 x 3136 tokens, 3 heads of 16 x 64 fp32: 16 + 4.5 + 98 us (matrix
-// units 38%, LDS 29%).
+// Measured.  4 x 4096 tokens, 16 heads of 128 x 64 on 2 key heads, bf16: contributions 30 us, join 5.5, walk 182, sum over the heads of a group 47 (5.7 TB/s).  A
+// chunk takes a workgroup of 16 waves, one a CU (159 KB of LDS), 24,000 cycles: the matrix units are busy 19% of them and LDS 49% (a third of that bank
+// conflicts, most of 8-byte writes), the rest waits between the phases, which need each other's results.  24 x 3136 tokens, 3 heads of 16 x 64 fp32: 15.5 + 5 + 91 us
+// (matrix units 39%, LDS 28%).
 #include "ss2d_linattn.h"
 #include "../../include/ss2d.h"
 
@@ -178,7 +178,7 @@ __device__ void zero_rows(const Problem &p, IO *o, long long row, int w, int nw)
 constexpr int GAP_WGS = 16;
 
 // fp32: 16 waves a workgroup, so that every result of a chunk -- dq, dk (C x dk) and dv (C x dv) -- is at most one 16 x 16 tile a wave on
-// v_mfma_f32_16x16x4_f32; keys up to 16 wide: 8 waves with two tiles of dv, and two workgroups a CU (24 x 3136 tokens, 3 heads of 16 x 64: 98 us, one
+// v_mfma_f32_16x16x4_f32; keys up to 16 wide: 8 waves with two tiles of dv, and two workgroups a CU (24 x 3136 tokens, 3 heads of 16 x 64: 96 us, one
 // workgroup of 16 waves 120).  A lane holds row / column l16 of an operand and contracted indices 4 gq + r of a 16-block in step r: direct operands are
 // 16-byte LDS reads, transposed ones four 4-byte reads, both free of bank conflicts at a pitch of 4 mod 16 floats.  LDS holds the four tiles, X,
 // Y and one state at a time: S (for dq), then D (for dk, dv).  The next chunk is in flight in registers.
@@ -530,8 +530,9 @@ __global__ __launch_bounds__(64 * NW, 4) void la_bwd_kernel(const BwdArgs a) {
 // rows in the same order (frag_tc).  Products of two transposed operands (over tokens) use frag_t for both.
 //
 // Up to 64 x 64 two workgroups of eight waves share a CU, so that one works while the other waits at its barriers: X waits in registers until dk is done with Y
-// and takes its place, and at 64 x 64 rows are half a pitch step shorter and a state's terms take turns (24 x 3136 tokens, 3 heads of 16 x 64, forward and
-// backward: 142 us with one workgroup of eight waves a CU, 123 with two; 4 x 4096, 16 heads of 64 x 64: 220 with one of sixteen, 208 with two of eight).
+// and takes its place, and at 64 x 64 rows are half a pitch step shorter and a state's terms take turns (with two terms of X and Y, 24 x 3136 tokens,
+// 3 heads of 16 x 64, forward and backward: 142 us with one workgroup of eight waves a CU, 123 with two; 4 x 4096, 16 heads of 64 x 64: 220 with one of sixteen, 208
+// with two of eight; three terms then 212).
 template <int DK, int DV, int NW, bool VEC, typename QT>
 __global__ __launch_bounds__(64 * NW, DK <= 64 && DV <= 64 ? 4 : NW / 4) void la_bwd_bf16_kernel(const BwdArgs a) {
     constexpr int NT = 64 * NW, C = 64, KT = DK / 16, KS = DK / 32, VT = DV / 16, VS = DV / 32;

@@ -7,10 +7,10 @@
 // leaves every segment's own contribution, a small pass joins them in order, and the main pass starts each segment from its
 // true state.
 //
-// Measured (a 1 GB copy reaches 5.0 TB/s).  65536 tokens, 8 heads of 128 x 128 bf16: contributions 71 us (268 MB, 3.8 TB/s), join 15, walk 166 (537 MB, 3.2
-// TB/s): the walk keeps the matrix units busy 35% of its time and LDS 40%; the rest is the splitting of fp32 factors and the wait at three
-// barriers a chunk (about 10,000 cycles a workgroup, two workgroups a CU).  24 x 3136 tokens, 3 heads of 16 x 64 fp32 with the states for the backward:
-// 15.5 + 4.6 + 45 us (159 MB, 3.5 TB/s).  One prompt of 17 tokens: 7.5 us, of which 4 are a launch.
+// Measured (a 1 GB copy reaches 5.0 TB/s).  65536 tokens, 8 heads of 128 x 128 bf16: contributions 70 us (268 MB, 3.8 TB/s), join 15, walk 182 (537 MB, 2.9
+// TB/s): the walk keeps the matrix units busy 38% of its time and LDS 42% (a quarter of that bank conflicts of 8-byte writes); the rest is the splitting of
+// fp32 factors and the wait at three barriers a chunk (about 11,000 cycles a workgroup, two workgroups a CU).  24 x 3136 tokens, 3 heads of 16 x 64 fp32 with the
+// states for the backward: 15 + 5 + 42 us (159 MB, 3.8 TB/s).  One prompt of 17 tokens: 7.7 us, of which 4 are a launch.
 #include "ss2d_linattn.h"
 #include "../../include/ss2d.h"
 

@@ -7,7 +7,9 @@
 // 16 heads of 64 x 64, 4.7 us, a launch; 128 requests, 16 heads of 64 x 65 (a second workgroup for the last column) 27 us, of 64 x 64 16.
 //
 // With slot indices two requests may name one slot.  Then the first of them applies all of that slot's tokens in request order,
-// and the others leave: the result does not depend on the order of execution.
+// and the others leave: the result does not depend on the order of execution.  Every workgroup looks through all B indices for that, which costs
+// nothing up to a thousand requests and more than the states beyond ten thousand (4 heads of 64 x 64, us without / with indices: 1024 requests 25 / 29, 4096 97 / 139,
+// 16384 392 / 911).
 #include "ss2d_common.h"
 #include "../../include/ss2d.h"
 

@@ -12,10 +12,11 @@ from . import _lib
 
 def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, cu_seqlens=None, max_seqlen=None, return_last_state=False):
     """q, k (b, l, g, dk); v (b, l, h, dv), h a multiple of g: value head j uses key head j // (h // g); log_decay (h,) or
-    (b, l, h), normally <= 0 (a decay below -150, -inf included, resets the state); scale defaults to dk ** -0.5; initial_state (n, h, dk, dv).
+    (b, l, h), normally <= 0 (a decay below -150, -inf included, is a factor of 0: it resets a finite state); scale defaults to dk ** -0.5; initial_state (n, h, dk, dv).
     Returns out (b, l, h, dv) in v's dtype [, last_state (n, h, dk, dv) fp32, differentiable].  dk, dv <= 128.
 
-    bf16 tensors (all of q, k, v) stay bf16 in memory, everything else is fp32; states, decays and sums are fp32 or wider.
+    bf16 tensors (all of q, k, v) stay bf16 in memory, everything else is fp32: states, weights, decays and sums keep at least 24 bits, also as factors on the
+    bf16 matrix units, and results are rounded once.  Gradients once; forward-mode derivatives and differentiating twice raise.
     cu_seqlens (n + 1 int32 offsets, non-decreasing): l tokens of one row (b = 1) hold n sequences, some possibly empty; rows that
     belong to none give zeros.  max_seqlen: an estimate of the longest of them (a hint whether to split any, default l).
     Without cu_seqlens n = b."""

@@ -774,7 +774,7 @@ def norm_gate_residual(x, y, post_weight, pre_weight, post_bias=None, pre_bias=N
     Returns (x', h): the new residual stream in x's dtype and the next block's input in y's dtype.  norm: LayerNorm over the last axis, or RMS norm
     with `rms`; statistics in fp32, h from the unrounded x'.  z (y's shape; a channel slice of a wider tensor is read in place), the biases,
     res_scale (D,) and drop_scale (one factor per sample, not differentiated) are optional.  bf16 x and y / z stay bf16 in memory (x may be fp32 with a bf16
-    branch); D <= 8192."""
+    branch); D <= 8192.  Gradients once; forward-mode derivatives and differentiating twice raise."""
     return _lib.host().norm_gate_residual(x, y, post_weight, pre_weight, post_bias, pre_bias, z, res_scale, drop_scale, eps, bool(rms))
 
 

@@ -267,10 +267,11 @@ struct LinearAttention : torch::autograd::Function<LinearAttention> {
         const float scale = (float)ctx->saved_data["scale"].toDouble();
         const at::ScalarType io = type(0) == at::kBFloat16 && type(1) == at::kBFloat16 && type(2) == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
         // hooks on saved tensors (offloaded or packed activations) may hand them back in another layout: they are checked and laid out as in the forward
-        const Dims now = attention_dims(saved[0], saved[1], saved[2], saved[3], Tensor(), saved[4]);
+        const Tensor cu = saved[4].defined() ? saved[4].contiguous() : saved[4];
+        const Dims now = attention_dims(saved[0], saved[1], saved[2], saved[3], Tensor(), cu);
         TORCH_CHECK_VALUE(now.B == d.B && now.L == d.L && now.G == d.G && now.dk == d.dk && now.H == d.H && now.dv == d.dv && now.N == d.N,
                           "linear_attention_fn: a saved tensor came back with another shape");
-        const Tensor q = operand(saved[0], io), k = operand(saved[1], io), v = operand(saved[2], io), g = decays(saved[3]), &cu = saved[4];
+        const Tensor q = operand(saved[0], io), k = operand(saved[1], io), v = operand(saved[2], io), g = decays(saved[3]);
         const at::Device dev = q.device();
         Tensor chunks;
         if (d.L > 0) {

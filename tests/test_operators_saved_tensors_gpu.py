@@ -101,3 +101,13 @@ def test_saved_tensors_of_another_shape_or_place_are_refused():
                 out = call()
             with pytest.raises(error):
                 torch.autograd.grad(out.sum(), leaf)
+
+
+def test_offsets_of_packed_sequences_come_back_with_gaps():
+    q, v = rnd(0, 1, 100, 2, 16).requires_grad_(), rnd(1, 1, 100, 4, 24)
+    g, cu = -rnd(2, 1, 100, 4).abs(), torch.tensor([0, 30, 30, 100], dtype=torch.int32).cuda()
+    call = lambda: linear_attention_fn(q, q, v, g, cu_seqlens=cu).sum()  # noqa: E731
+    want, = torch.autograd.grad(call(), q)
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: spread(x.detach())):
+        out = call()
+    assert torch.equal(torch.autograd.grad(out, q)[0], want)

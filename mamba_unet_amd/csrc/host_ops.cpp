@@ -2,6 +2,8 @@
 // launches, in one native call each.  Their smallest calls (one new token, a prompt of 17, a network's gradients) take the GPU 5 to 25 us; written
 // in Python on the ctypes binding the host took 10 to 55.  The kernels are reached through the addresses that _lib hands over (so that an
 // A/B build of the library serves both), on torch's current stream of the tensors' device.
+#include <algorithm>
+
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
@@ -521,6 +523,22 @@ std::tuple<Tensor, Tensor> norm_gate_residual(const Tensor &x, const Tensor &y, 
 
 // ------------------------------------------------------------------------------------------------ gradient clipping
 
+// whether the first element of `inner` is an element of `t` too (strides in falling order: each index is as large as what is left allows)
+bool holds_start_of(const Tensor &t, const Tensor &inner) {
+    if (!t.numel() || !inner.numel()) return false;
+    int64_t left = (const char *)inner.data_ptr() - (const char *)t.data_ptr();
+    const int64_t size = (int64_t)t.element_size();
+    if (left < 0 || left % size) return false;
+    left /= size;
+    std::vector<std::pair<int64_t, int64_t>> axes;
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1) axes.emplace_back(t.stride(i), t.size(i));
+    std::sort(axes.rbegin(), axes.rend());
+    for (const auto &[stride, n] : axes)
+        if (stride > 0) left -= std::min(left / stride, n - 1) * stride;
+    return left == 0;
+}
+
 Tensor clip_grad_norm(const py::object &given, double max_norm, double norm_type) {
     std::vector<Tensor> grads;
     const auto take = [&](PyObject *o) {
@@ -566,6 +584,11 @@ Tensor clip_grad_norm(const py::object &given, double max_norm, double norm_type
         sizes[i] = w.numel();
         is_bf16[i] = g.scalar_type() == at::kBFloat16;
     }
+    // the library looks at the dense ones; a tensor with gaps is clipped in a copy, which shares nothing
+    for (const auto &c : copies)
+        for (size_t i = 0; i < n; ++i)
+            TORCH_CHECK_VALUE(i == c.first || !(holds_start_of(grads[i], grads[c.first]) || holds_start_of(grads[c.first], grads[i])), "clip_grad_norm: tensor ",
+                              c.first, " shares memory with another one");
     const size_t bytes = api.ss2d_grad_clip_workspace_bytes((int)n);
     const Tensor norm = empty({}, dev), ws = empty({(int64_t)(bytes / 8)}, dev, at::kDouble);
     {
